@@ -329,6 +329,71 @@ int32_t origami_fused_prefix_attention_noalloc(
     void* d_output, uint32_t* d_error_flags, origami_stream_t stream);
 
 /* ---------------------------------------------------------------------------------
+ * New tokens of a step: per-head norm, position rotation, append to the paged cache
+ * ------------------------------------------------------------------------------- */
+
+/* Rows [tokens, num_heads, head_dim] of one tensor: strides in elements, head_dim contiguous
+ * (a slice of a fused projection's output qualifies). dtype is an ORIGAMI_DTYPE_*. */
+typedef struct origami_head_rows {
+  void* d_data;
+  int32_t dtype;
+  int64_t num_heads;
+  int64_t token_stride;
+  int64_t head_stride;
+} origami_head_rows;
+
+/* Position rotation of the first rotary_dim dims of a head: row p of d_cos_sin
+ * ([max_positions, rotary_dim], table_dtype, row_stride elements apart) holds rotary_dim / 2
+ * cosines, then as many sines. Pair i is dims (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * interleaved; (a, b) becomes (a cos - b sin, b cos + a sin). d_positions: one int32 or int64
+ * (position_bytes 4 or 8) per token. */
+typedef struct origami_rotation {
+  const void* d_cos_sin;
+  int32_t table_dtype;
+  int32_t interleaved;
+  int64_t max_positions;
+  int64_t rotary_dim;
+  int64_t row_stride;
+  const void* d_positions;
+  int32_t position_bytes;
+} origami_rotation;
+
+/* RMS norm of each head before the rotation, y = x * w / sqrt(mean(x^2) + eps), with weights
+ * [head_dim] shared by the heads; a null weight leaves that tensor's heads as they are. */
+typedef struct origami_head_norm {
+  const void* d_query_weight;
+  const void* d_key_weight;
+  int32_t query_weight_dtype;
+  int32_t key_weight_dtype;
+  double eps;
+} origami_head_norm;
+
+/* Norm (norm nullable) and rotation of a step's queries and keys in one pass, fp32 arithmetic,
+ * one rounding. query and key share a dtype; each output has its input's dtype and heads and
+ * may be the input itself (same pointer and strides) but must not overlap it otherwise.
+ * A token whose position lies outside the table is skipped: its rows are not written and
+ * d_error_count (nullable) grows by their number. No counterpart in the reference. */
+int32_t origami_norm_rope(const origami_head_rows* query, const origami_head_rows* query_out,
+                          const origami_head_rows* key, const origami_head_rows* key_out, int64_t tokens,
+                          int64_t head_dim, const origami_rotation* rotation, const origami_head_norm* norm,
+                          uint32_t* d_error_count, origami_stream_t stream);
+
+/* Append of a step's keys and values to one layer's paged cache, keys normed and rotated on
+ * the way (norm, rotation nullable), and with query / query_out (nullable) the queries as in
+ * origami_norm_rope in the same launch. d_slots holds one cache row per token (int32 or
+ * int64): slot = block id * block_size + offset; -1 means no row (a padded token: only its
+ * query is written). Slots must differ: of two tokens with one slot, which one's elements
+ * land is not defined. key, value and query share a dtype (F16, BF16 or F32); rows are stored
+ * as cache_dtype (F16 or BF16). Any other slot outside the cache, and any token whose
+ * position lies outside the table, is skipped and counted per row (token and head of query,
+ * key and value) in d_error_count (nullable). Cache rows that no slot names are not touched.
+ * No counterpart in the reference, which leaves the append to the engine. */
+int32_t origami_append_kv(const origami_head_rows* key, const origami_head_rows* value, const origami_head_rows* query,
+                          const origami_head_rows* query_out, const origami_paged_kv* cache, int32_t cache_dtype,
+                          const void* d_slots, int32_t slot_bytes, int64_t tokens, const origami_rotation* rotation,
+                          const origami_head_norm* norm, uint32_t* d_error_count, origami_stream_t stream);
+
+/* ---------------------------------------------------------------------------------
  * Host codec boundary (CPU only; no CUDA calls): the ORIGQZ1 chunk bundle and raw-deflate
  * chunk coding between caller-owned host buffers (pinned staging on the restore path)
  * ------------------------------------------------------------------------------- */

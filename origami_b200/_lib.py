@@ -58,6 +58,39 @@ class LayerJob(ctypes.Structure):
     ]
 
 
+class HeadRows(ctypes.Structure):
+    _fields_ = [
+        ("d_data", _vp),
+        ("dtype", ctypes.c_int32),
+        ("num_heads", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [
+        ("d_cos_sin", _vp),
+        ("table_dtype", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("max_positions", ctypes.c_int64),
+        ("rotary_dim", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("d_positions", _vp),
+        ("position_bytes", ctypes.c_int32),
+    ]
+
+
+class HeadNorm(ctypes.Structure):
+    _fields_ = [
+        ("d_query_weight", _vp),
+        ("d_key_weight", _vp),
+        ("query_weight_dtype", ctypes.c_int32),
+        ("key_weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_double),
+    ]
+
+
 class OrigamiError(RuntimeError):
     """A liborigami_b200 entry point returned an error status."""
 
@@ -117,6 +150,12 @@ def _declare(L: ctypes.CDLL) -> None:
         _vp, i64, i64, i64, i64, i64, i64, i64, i64, i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, i32, _vp, i32, i64, i64,
         i64, P(PagedKV), i32, _vp, i64, i64, i64, i64, ctypes.c_double, _vp, _vp, _vp]
     L.origami_fused_prefix_attention_noalloc.restype = i32
+    L.origami_norm_rope.argtypes = [P(HeadRows), P(HeadRows), P(HeadRows), P(HeadRows), i64, i64, P(Rotation),
+                                    P(HeadNorm), _vp, _vp]
+    L.origami_norm_rope.restype = i32
+    L.origami_append_kv.argtypes = [P(HeadRows), P(HeadRows), P(HeadRows), P(HeadRows), P(PagedKV), i32, _vp, i32, i64,
+                                    P(Rotation), P(HeadNorm), _vp, _vp]
+    L.origami_append_kv.restype = i32
     L.origami_selftest_wait_timeout.argtypes = [_vp, i32, _vp]
     L.origami_selftest_wait_timeout.restype = i32
     L.origami_origqz1_parse.argtypes = [_vp, i64, _vp, i64, _vp, _vp, _vp, _vp]
@@ -171,6 +210,8 @@ EXPORTS = (
     "origami_fused_prefix_attention",
     "origami_fused_prefix_attention_workspace",
     "origami_fused_prefix_attention_noalloc",
+    "origami_norm_rope",
+    "origami_append_kv",
     "origami_origqz1_parse",
     "origami_deflate_bound",
     "origami_deflate_chunks",

@@ -1,0 +1,180 @@
+"""The new tokens of a step on their way to the paged cache (kernels: csrc/append_kernels.cuh).
+
+norm_rope : RMS norm of queries and keys for each head and the position rotation, one pass.
+append_kv : keys and values of new tokens written into one layer's paged cache at their slots
+            (slot = block id * block_size + offset, as vLLM's slot_mapping; -1 = no row), the
+            keys normed and rotated on the way and, when given, the queries in the same launch.
+
+A row is one head of one token. With a weight, y = x * w / sqrt(mean(x^2) + eps); then pair i
+of the first R dims, (i, i + R/2) or (2i, 2i + 1) when interleaved, turns by the angle whose
+cosine and sine are cos_sin[position, i] and cos_sin[position, R/2 + i] (R = the table's
+width). Arithmetic is fp32 with one rounding at the store. Ops enqueue on the given (or
+current) stream of the tensors' device and never synchronise; ``error_count`` (an int32 CUDA
+tensor, optional) grows by one for every row that a position outside the table or a slot
+outside the cache left unwritten. An output that the call allocates belongs to the stream it
+runs on. The reference connector leaves these steps to the serving engine.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from origami_b200 import _lib
+from origami_b200.layer import _stream_handle, paged_desc
+
+_DTYPE = {torch.float16: _lib.ORIGAMI_DTYPE_F16, torch.bfloat16: _lib.ORIGAMI_DTYPE_BF16,
+          torch.float32: _lib.ORIGAMI_DTYPE_F32}
+
+
+def _on(device: torch.device, t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on the device of the others")
+
+
+def _rows(t: torch.Tensor, name: str, tokens: int, head_dim: int, device: torch.device) -> _lib.HeadRows:
+    _on(device, t, name)
+    if t.dim() != 3 or int(t.shape[0]) != tokens or int(t.shape[2]) != head_dim:
+        raise ValueError(f"{name} must have shape [{tokens}, heads, {head_dim}], got {tuple(t.shape)}")
+    if t.dtype not in _DTYPE:
+        raise ValueError(f"{name} must be float16, bfloat16 or float32")
+    if head_dim > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    return _lib.HeadRows(t.data_ptr(), _DTYPE[t.dtype], int(t.shape[1]), int(t.stride(0)), int(t.stride(1)))
+
+
+def _index(t: torch.Tensor, name: str, tokens: int, device: torch.device) -> int:
+    """Bytes per element of a contiguous int32 / int64 vector of one entry per token."""
+    _on(device, t, name)
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be int32 or int64")
+    if t.dim() != 1 or int(t.shape[0]) != tokens or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of {tokens} entries, one per token")
+    return t.element_size()
+
+
+def _rotation(positions: torch.Tensor | None, cos_sin: torch.Tensor | None, interleaved: bool, tokens: int,
+              device: torch.device):
+    if positions is None and cos_sin is None:
+        return None
+    if positions is None or cos_sin is None:
+        raise ValueError("positions and cos_sin go together")
+    width = _index(positions, "positions", tokens, device)
+    _on(device, cos_sin, "cos_sin")
+    if cos_sin.dim() != 2 or cos_sin.dtype not in _DTYPE:
+        raise ValueError("cos_sin must be a float16, bfloat16 or float32 matrix [max_positions, rotated dims]")
+    if cos_sin.shape[1] > 1 and cos_sin.stride(1) != 1:
+        raise ValueError("cos_sin must be contiguous in its last dimension")
+    # a table of one row has no row stride to speak of
+    stride = int(cos_sin.stride(0)) if cos_sin.shape[0] > 1 else int(cos_sin.shape[1])
+    return _lib.Rotation(cos_sin.data_ptr(), _DTYPE[cos_sin.dtype], int(bool(interleaved)), int(cos_sin.shape[0]),
+                         int(cos_sin.shape[1]), stride, positions.data_ptr(), width)
+
+
+def _norm(query_weight: torch.Tensor | None, key_weight: torch.Tensor | None, eps: float, head_dim: int,
+          device: torch.device):
+    if query_weight is None and key_weight is None:
+        return None
+    n = _lib.HeadNorm(None, None, 0, 0, float(eps))
+    for w, name in ((query_weight, "query_weight"), (key_weight, "key_weight")):
+        if w is None:
+            continue
+        _on(device, w, name)
+        if w.dtype not in _DTYPE or tuple(w.shape) != (head_dim,) or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float16, bfloat16 or float32 vector of {head_dim} elements")
+        setattr(n, f"d_{name}", w.data_ptr())
+        setattr(n, f"{name}_dtype", _DTYPE[w.dtype])
+    return n
+
+
+def _error(error_count: torch.Tensor | None, device: torch.device):
+    if error_count is None:
+        return None
+    _on(device, error_count, "error_count")
+    if error_count.dtype not in (torch.int32, torch.uint32) or error_count.numel() < 1:
+        raise ValueError("error_count must be an int32 tensor of one element")
+    return error_count.data_ptr()
+
+
+def _alloc_like(t: torch.Tensor, stream: torch.cuda.Stream | None, device: torch.device) -> torch.Tensor:
+    """A contiguous tensor of t's shape from the pool of the stream that will write it."""
+    with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device)):
+        return torch.empty(t.shape, dtype=t.dtype, device=device)
+
+
+def _ref(struct):
+    return ctypes.byref(struct) if struct is not None else None
+
+
+def norm_rope(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, *,
+              query_weight: torch.Tensor | None = None, key_weight: torch.Tensor | None = None, eps: float = 1e-6,
+              interleaved: bool = False, query_out: torch.Tensor | None = None, key_out: torch.Tensor | None = None,
+              stream: torch.cuda.Stream | None = None,
+              error_count: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm (where a weight is given) and rotate query [T, Hq, D] and key [T, Hk, D].
+
+    query and key may be strided slices of one projection's output; query_out / key_out may
+    be query / key themselves (in place). Returns (query_out, key_out)."""
+    device = query.device
+    if query.dim() != 3:
+        raise ValueError(f"query must have shape [tokens, heads, head_dim], got {tuple(query.shape)}")
+    tokens, head_dim = int(query.shape[0]), int(query.shape[2])
+    q = _rows(query, "query", tokens, head_dim, device)
+    k = _rows(key, "key", tokens, head_dim, device)
+    if positions is None or cos_sin is None:
+        raise ValueError("norm_rope needs positions and cos_sin")
+    rot = _rotation(positions, cos_sin, interleaved, tokens, device)
+    norm = _norm(query_weight, key_weight, eps, head_dim, device)
+    err = _error(error_count, device)
+    query_out = _alloc_like(query, stream, device) if query_out is None else query_out
+    key_out = _alloc_like(key, stream, device) if key_out is None else key_out
+    qo = _rows(query_out, "query_out", tokens, head_dim, device)
+    ko = _rows(key_out, "key_out", tokens, head_dim, device)
+    if tokens == 0:
+        return query_out, key_out
+    with torch.cuda.device(device):
+        rc = _lib.lib().origami_norm_rope(ctypes.byref(q), ctypes.byref(qo), ctypes.byref(k), ctypes.byref(ko), tokens,
+                                          head_dim, _ref(rot), _ref(norm), err, _stream_handle(stream, device))
+    _lib.check(rc, "origami_norm_rope")
+    return query_out, key_out
+
+
+def append_kv(kv_layer: torch.Tensor, key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, *,
+              query: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+              cos_sin: torch.Tensor | None = None, query_weight: torch.Tensor | None = None,
+              key_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+              query_out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None,
+              error_count: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Write key / value [T, Hk, D] of new tokens into the cache rows `slots` names, the keys
+    normed and rotated; returns the normed and rotated query (None without one).
+
+    kv_layer is a paged cache layer in either layout of `layer.cache_layout`, bf16 or fp16;
+    key, value and query share a type (bf16, fp16 or fp32). A token with slot -1 gets no
+    cache row; its query is still written. Slots must differ from one another. query_out may
+    be query itself."""
+    device = kv_layer.device
+    desc = paged_desc(kv_layer)
+    if kv_layer.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("the paged KV cache must be float16 or bfloat16")
+    tokens, head_dim = int(key.shape[0]), int(desc.head_dim)
+    k = _rows(key, "key", tokens, head_dim, device)
+    v = _rows(value, "value", tokens, head_dim, device)
+    width = _index(slots, "slots", tokens, device)
+    rot = _rotation(positions, cos_sin, interleaved, tokens, device)
+    norm = _norm(query_weight, key_weight, eps, head_dim, device)
+    err = _error(error_count, device)
+    q = qo = None
+    if query is not None:
+        q = _rows(query, "query", tokens, head_dim, device)
+        query_out = _alloc_like(query, stream, device) if query_out is None else query_out
+        qo = _rows(query_out, "query_out", tokens, head_dim, device)
+    elif query_out is not None or query_weight is not None:
+        raise ValueError("query_out and query_weight need a query")
+    if tokens == 0:
+        return query_out
+    with torch.cuda.device(device):
+        rc = _lib.lib().origami_append_kv(ctypes.byref(k), ctypes.byref(v), _ref(q), _ref(qo), ctypes.byref(desc),
+                                          _DTYPE[kv_layer.dtype], slots.data_ptr(), width, tokens, _ref(rot),
+                                          _ref(norm), err, _stream_handle(stream, device))
+    _lib.check(rc, "origami_append_kv")
+    return query_out
