@@ -394,6 +394,40 @@ int32_t origami_append_kv(const origami_head_rows* key, const origami_head_rows*
                           const origami_head_norm* norm, uint32_t* d_error_count, origami_stream_t stream);
 
 /* ---------------------------------------------------------------------------------
+ * Attention of a batch over a shared paged prefix and each request's own paged suffix
+ * ------------------------------------------------------------------------------- */
+
+/* Query token j of request b (tokens query_start[b] .. query_start[b + 1] of `query`, n of
+ * them) attends to all prefix_tokens keys of the shared prefix, in the cache blocks
+ * d_prefix_blocks, and to the first suffix_lens[b] - n + j + 1 keys (none if that is not
+ * positive) of the request's own suffix, in the blocks d_suffix_blocks[b * suffix_stride ..]:
+ * a request's suffix includes its new tokens, already in the cache. The scores are scaled by
+ * softmax_scale (finite, positive); query head qh reads KV head qh / (query_heads /
+ * kv_heads). A row without keys gives zeros and lse -inf; an out-of-range block id reads as
+ * zero K and V (the key still takes part in the softmax with score 0); query tokens outside
+ * [query_start[0], query_start[requests]) are left as they are in output and lse. The lists
+ * are device int32; lengths are clamped to the tables (suffix_lens to suffix_width *
+ * block_size, query_start to [0, tokens]).
+ * query, output and cache share a type (F16 or BF16); head_dim is 64 or 128, the query heads
+ * of a KV head at most 128. lse (nullable, [tokens, query_heads] contiguous) gets the natural
+ * logarithm of each row's sum of exponentials. Keys and values past the last one that any of
+ * a request's rows sees are never read.
+ * d_workspace: origami_shared_prefix_attention_workspace() bytes, 16-byte aligned; its
+ * contents need no preparation and mean nothing between calls; calls that share it must not
+ * overlap. d_error_flags (nullable) gets bit 31 if a bounded wait inside the kernel ran out.
+ * No counterpart in the reference, whose attention takes one request a call. */
+int32_t origami_shared_prefix_attention(
+    const origami_head_rows* query, const origami_head_rows* output, float* d_lse, int64_t tokens, int64_t head_dim,
+    const origami_paged_kv* cache, int32_t cache_dtype, const int32_t* d_prefix_blocks, int64_t num_prefix_blocks,
+    int64_t prefix_tokens, const int32_t* d_suffix_blocks, int64_t suffix_stride, int64_t suffix_width,
+    const int32_t* d_suffix_lens, const int32_t* d_query_start, int64_t requests, double softmax_scale,
+    void* d_workspace, int64_t workspace_bytes, uint32_t* d_error_flags, origami_stream_t stream);
+
+/* Workspace bytes origami_shared_prefix_attention needs for these shapes on the current device. */
+int32_t origami_shared_prefix_attention_workspace(int64_t tokens, int64_t query_heads, int64_t kv_heads,
+                                                  int64_t head_dim, int64_t requests, int64_t* workspace_bytes);
+
+/* ---------------------------------------------------------------------------------
  * Host codec boundary (CPU only; no CUDA calls): the ORIGQZ1 chunk bundle and raw-deflate
  * chunk coding between caller-owned host buffers (pinned staging on the restore path)
  * ------------------------------------------------------------------------------- */

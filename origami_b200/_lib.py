@@ -156,6 +156,12 @@ def _declare(L: ctypes.CDLL) -> None:
     L.origami_append_kv.argtypes = [P(HeadRows), P(HeadRows), P(HeadRows), P(HeadRows), P(PagedKV), i32, _vp, i32, i64,
                                     P(Rotation), P(HeadNorm), _vp, _vp]
     L.origami_append_kv.restype = i32
+    L.origami_shared_prefix_attention.argtypes = [
+        P(HeadRows), P(HeadRows), _vp, i64, i64, P(PagedKV), i32, _vp, i64, i64, _vp, i64, i64, _vp, _vp, i64,
+        ctypes.c_double, _vp, i64, _vp, _vp]
+    L.origami_shared_prefix_attention.restype = i32
+    L.origami_shared_prefix_attention_workspace.argtypes = [i64, i64, i64, i64, i64, _vp]
+    L.origami_shared_prefix_attention_workspace.restype = i32
     L.origami_selftest_wait_timeout.argtypes = [_vp, i32, _vp]
     L.origami_selftest_wait_timeout.restype = i32
     L.origami_origqz1_parse.argtypes = [_vp, i64, _vp, i64, _vp, _vp, _vp, _vp]
@@ -212,6 +218,8 @@ EXPORTS = (
     "origami_fused_prefix_attention_noalloc",
     "origami_norm_rope",
     "origami_append_kv",
+    "origami_shared_prefix_attention",
+    "origami_shared_prefix_attention_workspace",
     "origami_origqz1_parse",
     "origami_deflate_bound",
     "origami_deflate_chunks",

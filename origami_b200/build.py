@@ -17,7 +17,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OBJ = HERE / "_build"
 LIB = HERE / "liborigami_b200.so"
-SOURCES = ["abi.cu", "quant.cu", "attention.cu", "append.cu", "host_codec.cpp"]
+SOURCES = ["abi.cu", "quant.cu", "attention.cu", "append.cu", "shared_prefix.cu", "host_codec.cpp"]
 HEADERS = [CSRC / p for p in sorted(os.listdir(CSRC)) if p.endswith((".cuh", ".h"))] + [
     HERE.parent / "include" / "origami_b200.h"]
 

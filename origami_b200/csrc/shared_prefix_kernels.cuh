@@ -1,0 +1,978 @@
+// Attention of a ragged batch over a paged prefix that all its requests share and each
+// request's own paged suffix.
+//
+// Mathematics. Row (token t, query head qh) of KV head h: with scores s_k = scale q.k over
+// its visible keys, out = sum_k e^(s_k - m) v_k / sum_k e^(s_k - m). The keys are split into
+// pieces; a piece leaves (O, m, l) = (sum e^(s - m) v, reference maximum, sum e^(s - m)) and
+// pieces join as O = sum O_i e^(m_i - m), l = sum l_i e^(m_i - m). Softmax statistics, O and
+// the joins are fp32; the probabilities are rounded to the type of V for the product (the
+// tensor cores take both operands in one type; half a step, 2^-9 bf16 / 2^-12 fp16, relative
+// to each probability, is below the output's own rounding after averaging over keys).
+//
+// Work. The prefix is one attention problem per KV head whose rows are the new tokens of ALL
+// requests x the query heads of the group: its K and V are read once for every 128 or 256
+// rows instead of once per request. The suffixes are one small problem per (KV head, request).
+// Both are cut into "items" (rows x one key range), every item into tiles of 128 keys, and the
+// tiles of all items, laid end to end with a cost each, are dealt to one persistent CTA per SM
+// in equal contiguous shares: no tail, no atomics, a fixed order of summation. A share's piece
+// of an item (a "segment") writes one partial; merge_partials joins each row's partials.
+//
+// A CTA (13 warps): 4 loader warps gather K and V tiles through the block tables with 16-byte
+// cp.async into a ring of 128-byte-swizzled tiles (any block size; rows past the end become
+// zeros, so garbage there cannot reach the products); one thread issues tcgen05.mma; two
+// softmax warpgroups own one stream each, a stream being one (S, O) accumulator pair in TMEM:
+//   S_s [128 rows x 128 keys] = Q K^T (shared memory operands),
+//   O_s [128 rows x D]       += P V   (P in TMEM over S's second half, V as the N-major B operand).
+// One thread owns one row, so the softmax needs no exchange. O is rescaled only when the
+// maximum grew by more than 2^8 (P stays below 2^8, exact in the same relative precision).
+// With more than 128 rows an item has two row tiles, one per stream, that share each K and V
+// tile ("pair"); with fewer, the streams take alternate key tiles of one row tile and join at
+// the end of the segment ("split"). Either way one stream's softmax runs under the other's
+// products.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "attention_kernels.cuh"
+#include "common.cuh"
+
+namespace origami {
+
+namespace spa {
+
+constexpr int kThreadsS = 416;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12: MMA
+constexpr int kTile = 128;      // keys per tile, rows per row tile
+// Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of a segment.
+constexpr int kCostTile = 8, kCostPair = 8, kCostItem = 4;
+
+// Shared memory: Q tiles, then the ring of K / V tiles (each [128][D] 16-bit), then scalars.
+template <int D>
+struct Smem {
+  static constexpr int tile = kTile * D * 2;
+  static constexpr int stages = D == 128 ? 5 : 10;
+  static constexpr int lag = D == 128 ? 3 : 6;  // stages a loader keeps in flight
+  static constexpr int ring = 2 * tile;
+  static constexpr int scalars = ring + stages * tile;
+  static constexpr int bytes = scalars + 2 * kTile * 8 + 512;
+};
+
+}  // namespace spa
+
+struct SharedArgs {
+  const uint16_t* query;
+  uint16_t* output;
+  float* lse;
+  int64_t q_token, q_head, o_token, o_head;
+  const uint16_t* cache;
+  int64_t kv_stride, row_elems;  // elements from K to V; elements of one token row (heads * D)
+  int64_t num_blocks;
+  int32_t block_size, block_rows;  // token rows from one block to the next
+  const int32_t* prefix_blocks;
+  const int32_t* suffix_blocks;
+  int64_t suffix_stride;
+  const int32_t* suffix_lens;
+  const int32_t* query_start;
+  int32_t tokens, requests, prefix, suffix_cap;
+  int32_t q_heads, kv_heads, group, tile_tokens;  // tokens per row tile
+  int32_t item_rows_p, item_rows_s;               // partial rows a CTA may need for a prefix / suffix item
+  int32_t q_vec, o_vec, ctas;
+  float scale_log2;
+  // workspace
+  int64_t* head;      // {prefix cost per head, suffix cost per head}
+  int64_t* req_cost;  // [requests] suffix cost of the requests before this one
+  float* ml;          // [rows][2]
+  float* o;           // [rows][D]
+  uint32_t* err;
+};
+
+namespace spa {
+
+using attn::mma_commit;
+using attn::pack2;
+using attn::proxy_fence;
+using attn::tc_fence_after;
+using attn::tc_fence_before;
+
+__device__ __forceinline__ int clampi(int64_t v, int64_t lo, int64_t hi) {
+  return static_cast<int>(v < lo ? lo : v > hi ? hi : v);
+}
+
+// ---------------------------------------------------------------------------------------
+// The deal: items in order (prefix items of head 0, 1, ..; then suffix items of head 0, 1,
+// .. by request and row tile), each with a start on the cost axis.
+// ---------------------------------------------------------------------------------------
+struct Item {
+  int64_t start;   // on the cost axis
+  int64_t tok0;    // first token
+  int32_t ntok;    // its tokens
+  int32_t kend;    // keys its last row sees
+  int32_t vis0;    // suffix: keys its first token sees (may be negative)
+  int32_t h, b;    // KV head; request, -1 for the prefix
+  int32_t tile_cost;
+  bool pair;
+  __device__ __forceinline__ int tiles() const { return (kend + kTile - 1) / kTile; }
+  __device__ __forceinline__ int64_t cost() const { return kend > 0 ? kCostItem + static_cast<int64_t>(tiles()) * tile_cost : 0; }
+  // First tile that a share beginning at w takes.
+  __device__ __forceinline__ int tile_at(int64_t w) const {
+    const int64_t x = w - start - kCostItem;
+    if (x <= 0) return 0;
+    const int64_t t = (x + tile_cost - 1) / tile_cost;
+    return t > tiles() ? tiles() : static_cast<int>(t);
+  }
+};
+
+__device__ __forceinline__ int used_tokens(const SharedArgs& a) {
+  return clampi(__ldg(a.query_start + a.requests), 0, a.tokens);
+}
+__device__ __forceinline__ int prefix_item_tokens(const SharedArgs& a, int used) {
+  return used > a.tile_tokens ? 2 * a.tile_tokens : a.tile_tokens;
+}
+__device__ __forceinline__ Item prefix_item(const SharedArgs& a, int used, int h, int64_t tok0, int64_t start) {
+  Item it;
+  it.start = start;
+  it.tok0 = tok0;
+  it.ntok = clampi(used - tok0, 0, prefix_item_tokens(a, used));
+  it.kend = a.prefix;
+  it.vis0 = a.prefix;
+  it.h = h;
+  it.b = -1;
+  it.pair = it.ntok > a.tile_tokens;
+  it.tile_cost = it.pair ? kCostPair : kCostTile;
+  return it;
+}
+// Cost of all prefix items of one head.
+__device__ __forceinline__ int64_t prefix_cost(const SharedArgs& a, int used) {
+  if (used == 0 || a.prefix == 0) return 0;
+  const int per = prefix_item_tokens(a, used);
+  const int64_t items = (used + per - 1) / per;
+  const Item first = prefix_item(a, used, 0, 0, 0);
+  const Item last = prefix_item(a, used, 0, (items - 1) * per, 0);
+  return (items - 1) * first.cost() + last.cost();
+}
+
+struct Request {
+  int32_t begin, n, len;
+  __device__ __forceinline__ Request(const SharedArgs& a, int b) {
+    begin = clampi(__ldg(a.query_start + b), 0, a.tokens);
+    n = clampi(__ldg(a.query_start + b + 1), begin, a.tokens) - begin;
+    len = clampi(__ldg(a.suffix_lens + b), 0, a.suffix_cap);
+  }
+};
+__device__ __forceinline__ Item suffix_item(const SharedArgs& a, const Request& r, int h, int b, int tile, int64_t start) {
+  Item it;
+  it.start = start;
+  const int t0 = tile * a.tile_tokens;
+  it.tok0 = r.begin + t0;
+  it.ntok = min(a.tile_tokens, r.n - t0);
+  it.vis0 = r.len - r.n + t0 + 1;
+  it.kend = clampi(static_cast<int64_t>(it.vis0) + it.ntok - 1, 0, r.len);
+  it.h = h;
+  it.b = b;
+  it.pair = false;
+  it.tile_cost = kCostTile;
+  return it;
+}
+__device__ __forceinline__ int64_t request_cost(const SharedArgs& a, const Request& r) {
+  int64_t c = 0;
+  for (int t = 0; t * a.tile_tokens < r.n; ++t) c += suffix_item(a, r, 0, 0, t, 0).cost();
+  return c;
+}
+
+// Where the shares begin, known to every thread of a CTA.
+struct Deal {
+  int64_t wp, ws;  // cost of one head's prefix / suffix items
+  int64_t w0, w1;  // this CTA's share
+  int32_t used;
+  // the first suffix item of the share
+  int32_t h, b, tile;
+  int64_t start;
+};
+
+// Walks the segments of a CTA's share. Every role runs its own copy.
+struct Walk {
+  const SharedArgs& a;
+  const Deal& d;
+  Item it;
+  int t0, t1;      // tiles of the segment
+  int64_t next;    // start of the item after `it`
+  int h, b, tile;  // next suffix item
+  int ph;          // next prefix item: head and first token
+  int64_t ptok;
+  bool in_prefix;
+  Request r;
+  __device__ __forceinline__ Walk(const SharedArgs& args, const Deal& deal) : a(args), d(deal), r(args, deal.b < 0 ? 0 : deal.b) {
+    const int64_t all = d.wp * a.kv_heads;
+    in_prefix = d.w0 < all;
+    h = d.h;
+    b = d.b;
+    tile = d.tile;
+    next = d.start;
+    ph = 0;
+    ptok = 0;
+    if (in_prefix) {
+      const int per = prefix_item_tokens(a, d.used);
+      ph = static_cast<int>(d.w0 / d.wp);
+      const int64_t in_head = d.w0 - ph * d.wp;
+      const int64_t first = prefix_item(a, d.used, 0, 0, 0).cost();
+      const int64_t i = min64(in_head / first, (d.used + per - 1) / per - 1);
+      ptok = i * per;
+      next = ph * d.wp + i * first;
+    }
+  }
+  __device__ __forceinline__ bool step() {
+    while (next < d.w1) {
+      if (in_prefix) {
+        it = prefix_item(a, d.used, ph, ptok, next);
+        next += it.cost();
+        ptok += it.ntok;
+        if (ptok >= d.used) {
+          ptok = 0;
+          ++ph;
+        }
+        if (ph >= a.kv_heads) {
+          in_prefix = false;
+          h = b = tile = 0;
+          r = Request(a, 0);
+        }
+      } else {
+        // stop past the last head (requests without any tile cost nothing and end nowhere)
+        if (h >= a.kv_heads) return false;
+        if (tile * a.tile_tokens >= r.n) {
+          tile = 0;
+          if (++b >= a.requests) {
+            b = 0;
+            ++h;
+          }
+          r = Request(a, b);
+          continue;
+        }
+        it = suffix_item(a, r, h, b, tile, next);
+        next += it.cost();
+        ++tile;
+      }
+      if (it.kend <= 0) continue;
+      t0 = it.tile_at(d.w0);
+      t1 = it.tile_at(d.w1);
+      if (t1 > t0) return true;
+    }
+    return false;
+  }
+  // Partial row of the segment's first row.
+  __device__ __forceinline__ int64_t partial_row(int cta) const;
+};
+
+// Partial rows: an item's rows begin at its place among all rows of its kind plus its CTA's
+// index times the rows one item may have. Two segments never overlap: a later CTA's segment of
+// one item lies item_rows further, a later item at least this item's rows further.
+__device__ __forceinline__ int64_t partial_base(const SharedArgs& a, const Item& it, int cta) {
+  const int64_t rows = (static_cast<int64_t>(it.h) * a.tokens + it.tok0) * a.group;
+  if (it.b < 0) return rows + static_cast<int64_t>(cta) * a.item_rows_p;
+  return static_cast<int64_t>(a.q_heads) * a.tokens + static_cast<int64_t>(a.ctas) * a.item_rows_p + rows +
+         static_cast<int64_t>(cta) * a.item_rows_s;
+}
+__device__ __forceinline__ int64_t Walk::partial_row(int cta) const { return partial_base(a, it, cta); }
+
+// ---------------------------------------------------------------------------------------
+// tcgen05 helpers
+// ---------------------------------------------------------------------------------------
+// Descriptors of 128-byte-swizzled tiles [rows][64 elements] (8-row groups 1024 bytes apart).
+// K-major (Q, K): a further 64 dims are another 16 KB tile, addressed by the start.
+// N-major (V): 64-dim columns of the tile lie 16 KB (the leading byte offset) apart.
+__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lbo) {
+  return (static_cast<uint64_t>(addr >> 4) & 0x3FFFull) | (static_cast<uint64_t>(lbo >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(ta), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// 32 consecutive TMEM columns of this thread's lane.
+__device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31,%32};\n" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Bounded wait that gives up early when another role has: 2 s, far beyond any copy or product.
+constexpr uint64_t kWaitNs = 2000000000ull;
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (mbar_wait_bounded(bar, parity, 64)) return true;
+  const uint64_t begin = now_ns();
+  while (!mbar_wait_bounded(bar, parity, 64)) {
+    if (*abort) return false;
+    if (now_ns() - begin > kWaitNs) {
+      *abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// Copy of 16 bytes, or 16 zero bytes where `valid` is false (the source is then not read).
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool valid) {
+  const uint32_t n = valid ? 16u : 0u;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+// 32 consecutive floats of a partial row.
+__device__ __forceinline__ void store_o(float* p, const uint32_t (&o)[32]) {
+  uint4* dst = reinterpret_cast<uint4*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+}
+
+// Byte offset of 16-byte chunk c of row r in a swizzled [128][D] tile.
+__device__ __forceinline__ uint32_t chunk_off(int r, int c) {
+  return static_cast<uint32_t>((c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+struct Bars {
+  uint64_t full[10], empty[10], q_empty[2], s_full[2], p_full[2], pv[2], o_free, xch, done;
+};
+
+}  // namespace spa
+
+// ---------------------------------------------------------------------------------------
+// One persistent CTA per SM.
+// ---------------------------------------------------------------------------------------
+template <typename QT, int D>
+__global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(const __grid_constant__ SharedArgs a) {
+  using namespace spa;
+  using S = Smem<D>;
+  extern __shared__ __align__(1024) uint8_t spa_smem[];
+  uint8_t* sm = spa_smem;
+  float2* ml_sm = reinterpret_cast<float2*>(sm + S::scalars);  // [2 streams][128 rows]
+  Bars* bars = reinterpret_cast<Bars*>(ml_sm + 2 * kTile);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 1);
+  int* abort_sm = reinterpret_cast<int*>(tslot + 1);
+  Deal* deal_sm = reinterpret_cast<Deal*>(tslot + 2);
+  static_assert(sizeof(Bars) + 8 + sizeof(Deal) <= 512, "scalars fit");
+  static_assert(S::bytes <= 227 * 1024, "shared memory of one SM");
+  constexpr bool kBf16 = attn::is_bf16<QT>();
+  constexpr uint32_t kIdescS = attn::instr_desc(kBf16, kTile);
+  constexpr uint32_t kIdescO = attn::instr_desc(kBf16, D) | (1u << 16);  // B (V) is N-major
+  constexpr uint32_t kS[2] = {0, 128}, kO[2] = {256, 384};
+  constexpr uint32_t kPCol = 64;  // P lies over the second half of S
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = static_cast<int>(blockIdx.x);
+  // the tiles' swizzle is a function of the address: they must begin on a 1024-byte boundary
+  if (smem_u32(sm) & 1023) {
+    if (tid == 0 && a.err) atomicOr(a.err, kWaitTimeoutFlag);
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < S::stages; ++i) {
+      mbar_init(&bars->full[i], 4);
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->q_empty[i], 1);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], kTile);
+      mbar_init(&bars->pv[i], 1);
+    }
+    mbar_init(&bars->o_free, 2 * kTile);
+    mbar_init(&bars->xch, 2 * kTile);
+    mbar_init(&bars->done, 1);
+    *abort_sm = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tslot)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+  }
+  // dependent launch: everything above overlaps the kernel before this one
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  // The deal: suffix costs of contiguous runs of requests, scanned over the CTA.
+  {
+    int64_t* scan = reinterpret_cast<int64_t*>(sm);  // [13] warp sums
+    const int per = (a.requests + kThreadsS - 1) / kThreadsS;
+    const int b0 = min(tid * per, a.requests), b1 = min(b0 + per, a.requests);
+    int64_t sum = 0;
+    for (int b = b0; b < b1; ++b) sum += request_cost(a, Request(a, b));
+    int64_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < kThreadsS / 32; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    const int64_t excl = before + incl - sum;
+    const int used = used_tokens(a);
+    const int64_t wp = prefix_cost(a, used), all_p = wp * a.kv_heads, all = all_p + total * a.kv_heads;
+    const int64_t w0 = all * cta / a.ctas, w1 = all * (cta + 1) / a.ctas;
+    // the share's first suffix item: in the run of requests that holds its cost
+    const int64_t y = w0 <= all_p ? 0 : w0 - all_p;
+    const int64_t fh = total > 0 ? y / total : 0, rem = y - fh * total;
+    if (tid == 0) {
+      deal_sm->wp = wp;
+      deal_sm->ws = total;
+      deal_sm->w0 = w0;
+      deal_sm->w1 = w1;
+      deal_sm->used = used;
+      if (total == 0) {
+        deal_sm->h = a.kv_heads;  // no suffix anywhere
+        deal_sm->b = deal_sm->tile = 0;
+        deal_sm->start = all_p;
+      }
+      if (cta == 0) {
+        a.head[0] = wp;
+        a.head[1] = total;
+      }
+    }
+    if (sum > 0 && rem >= excl && rem < excl + sum) {
+      int64_t at = excl;
+      int b = b0;
+      for (; b < b1; ++b) {
+        const int64_t c = request_cost(a, Request(a, b));
+        if (rem < at + c) break;
+        at += c;
+      }
+      const Request r(a, b);
+      int t = 0;
+      for (;; ++t) {
+        const int64_t c = suffix_item(a, r, 0, 0, t, 0).cost();
+        if (rem < at + c) break;
+        at += c;
+      }
+      deal_sm->h = static_cast<int>(fh);
+      deal_sm->b = b;
+      deal_sm->tile = t;
+      deal_sm->start = all_p + fh * total + at;
+    }
+    if (cta == 0) {
+      int64_t at = excl;
+      for (int b = b0; b < b1; ++b) {
+        a.req_cost[b] = at;
+        at += request_cost(a, Request(a, b));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  const Deal deal = *deal_sm;
+  volatile int* abort = abort_sm;
+  Walk w(a, deal);
+
+  if (warp >= 8 && warp < 12) {
+    // ---------------------------------------------------------------- loaders
+    // Warp lw fills rows 32 lw .. 32 lw + 31 of every tile; lane l knows row 32 lw + l.
+    constexpr int kChunks = D / 8;          // 16-byte chunks per row
+    constexpr int kRowsPer = 32 / kChunks;  // rows a warp copies at once
+    const int lw = warp - 8;
+    const int sub = lane / kChunks, chunk = lane % kChunks;
+    const uint32_t base = smem_u32(sm);
+    int ring = 0, signalled = 0;  // stages issued / signalled
+    uint32_t q_uses[2] = {0u, 0u};
+    int q_next = 0;
+    bool ok = true;
+    auto signal_one = [&]() {
+      proxy_fence();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->full[signalled % S::stages]);
+      ++signalled;
+    };
+    auto drain = [&]() {
+      asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+      while (signalled < ring) signal_one();
+    };
+    // cache row of key `key` of this item, -1 past its end, -2 outside the cache
+    auto row_of = [&](int64_t key) -> int {
+      if (key >= w.it.kend) return -1;
+      const uint32_t k = static_cast<uint32_t>(key), page = k / static_cast<uint32_t>(a.block_size);
+      const int32_t* table = w.it.b < 0 ? a.prefix_blocks : a.suffix_blocks + w.it.b * a.suffix_stride;
+      const int pb = __ldg(table + page);
+      if (pb < 0 || pb >= a.num_blocks) return -2;
+      return pb * a.block_rows + static_cast<int>(k - page * static_cast<uint32_t>(a.block_size));
+    };
+    // Waits until stage `ring` may be refilled.
+    auto acquire = [&]() {
+      const int st = ring % S::stages, use = ring / S::stages;
+      if (use == 0) return;
+      const uint32_t parity = static_cast<uint32_t>((use - 1) & 1);
+      bool ready = mbar_wait_bounded(&bars->empty[st], parity, 1);
+      ready = __all_sync(0xffffffffu, ready);
+      if (!ready) {
+        drain();  // whoever frees the stage may need the ones in flight
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->empty[st], parity, abort));
+      }
+    };
+    auto emit = [&](int row, int which) {
+      acquire();
+      if (!ok) return;
+      const uint32_t dst = base + S::ring + (ring % S::stages) * S::tile;
+      const uint16_t* src = a.cache + which * a.kv_stride + static_cast<int64_t>(w.it.h) * D + chunk * 8;
+#pragma unroll 8
+      for (int i = 0; i < 32 / kRowsPer; ++i) {
+        const int r = i * kRowsPer + sub;
+        const int cr = __shfl_sync(0xffffffffu, row, r);
+        cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
+      }
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+      ++ring;
+      if (ring - signalled > S::lag) {
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(S::lag) : "memory");
+        signal_one();
+      }
+    };
+    while (ok && w.step()) {
+      // Q: one row tile, into the buffer after the last one used, or both for a pair
+      const int tiles_q = w.it.pair ? 2 : 1;
+      if (w.it.pair) q_next = 0;
+      for (int q = 0; q < tiles_q && ok; ++q) {
+        const int buf = q_next;
+        q_next ^= 1;
+        if (q_uses[buf] > 0) {
+          const uint32_t parity = (q_uses[buf] - 1) & 1u;
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars->q_empty[buf], parity, 1))) {
+            drain();
+            ok = __all_sync(0xffffffffu, wait_or_abort(&bars->q_empty[buf], parity, abort));
+            if (!ok) break;
+          }
+        }
+        ++q_uses[buf];
+        const int rows = min(a.tile_tokens, w.it.ntok - q * a.tile_tokens) * a.group;
+        const int64_t tok = w.it.tok0 + q * a.tile_tokens;
+        const uint32_t dst = base + buf * S::tile;
+#pragma unroll 4
+        for (int i = 0; i < 32 / kRowsPer; ++i) {
+          const int r = 32 * lw + i * kRowsPer + sub;
+          const bool valid = r < rows;
+          const int64_t t = tok + (valid ? r / a.group : 0);
+          const int qh = w.it.h * a.group + (valid ? r % a.group : 0);
+          const uint16_t* src = a.query + t * a.q_token + qh * a.q_head + chunk * 8;
+          if (a.q_vec) {
+            cp16_or_zero(dst + chunk_off(r, chunk), src, valid);
+          } else {
+            uint32_t v[4] = {0u, 0u, 0u, 0u};
+            if (valid) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] = src[2 * j] | (static_cast<uint32_t>(src[2 * j + 1]) << 16);
+            }
+            *reinterpret_cast<uint4*>(sm + buf * S::tile + chunk_off(r, chunk)) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+      if (!ok) break;
+      // pair: K V K V ..; split: K K V K V .. V, the order in which the products first use them
+      const int n = w.t1 - w.t0;
+      int row = row_of(static_cast<int64_t>(w.t0) * kTile + 32 * lw + lane), prev = -1;
+      for (int i = 0; i <= n && ok; ++i) {
+        const int next_row = i + 1 < n ? row_of(static_cast<int64_t>(w.t0 + i + 1) * kTile + 32 * lw + lane) : -1;
+        if (i < n) emit(row, 0);
+        if (w.it.pair) {
+          if (i < n && ok) emit(row, 1);
+        } else if (i > 0 && ok) {
+          emit(prev, 1);
+        }
+        prev = row;
+        row = next_row;
+      }
+    }
+    drain();
+  } else if (warp == 12) {
+    // ---------------------------------------------------------------- products
+    if (lane == 0) {
+      const uint32_t base = smem_u32(sm);
+      int ring = 0;  // stage index at which the segment begins
+      uint32_t p_phase[2] = {0u, 0u}, pv_phase[2] = {0u, 0u}, o_phase = 0u;
+      int q_next = 0;
+      bool pending[2] = {false, false};  // a product of the stream that was not waited for
+      bool first_seg = true, ok = true;
+      while (ok && w.step()) {
+        const int n = w.t1 - w.t0;
+        const bool pair = w.it.pair;
+        const int ns[2] = {pair ? n : (n + 1) / 2, pair ? n : n / 2};
+        if (pair) q_next = 0;
+        const int qb[2] = {q_next, pair ? 1 : q_next};
+        if (!pair) q_next ^= 1;
+        auto stage_k = [&](int t) { return ring + (pair ? 2 * t : t == 0 ? 0 : 2 * t - 1); };
+        auto stage_v = [&](int t) { return ring + (pair ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1)); };
+        auto wait_full = [&](int st) {
+          return wait_or_abort(&bars->full[st % S::stages], static_cast<uint32_t>((st / S::stages) & 1), abort);
+        };
+        auto tile_of = [&](int s, int i) { return pair ? i : 2 * i + s; };
+        auto issue_s = [&](int s, int i) {
+          const int st = stage_k(tile_of(s, i));
+          if (!wait_full(st)) return false;
+          // P lies in S: the product that reads it must have ended before S is written again
+          if (pending[s] && !wait_or_abort(&bars->pv[s], pv_phase[s] ^ 1u, abort)) return false;
+          pending[s] = false;
+          tc_fence_after();
+          const uint32_t qa = base + qb[s] * S::tile, ka = base + S::ring + (st % S::stages) * S::tile;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = (k >> 2) * (kTile * 128) + (k & 3) * 32;
+            mma_ss(tmem + kS[s], desc128(qa + off, 16), desc128(ka + off, 16), kIdescS, k > 0 ? 1u : 0u);
+          }
+          mma_commit(&bars->s_full[s]);
+          if (!pair || s == 1) mma_commit(&bars->empty[st % S::stages]);
+          // the last product that reads a Q buffer frees it
+          if (i == ns[s] - 1) {
+            if (pair) mma_commit(&bars->q_empty[s]);
+            else if (tile_of(s, i) == n - 1) mma_commit(&bars->q_empty[qb[0]]);
+          }
+          return true;
+        };
+        for (int s = 0; s < 2 && ok; ++s)
+          if (ns[s] > 0) ok = issue_s(s, 0);
+        for (int i = 0; i < ns[0] && ok; ++i) {
+          for (int s = 0; s < 2 && ok; ++s) {
+            if (i >= ns[s]) continue;
+            const int st = stage_v(tile_of(s, i));
+            ok = wait_full(st) && wait_or_abort(&bars->p_full[s], p_phase[s], abort);
+            if (!ok) break;
+            p_phase[s] ^= 1u;
+            if (i == 0 && s == 0 && !first_seg) {  // the last segment's O has been read
+              ok = wait_or_abort(&bars->o_free, o_phase, abort);
+              if (!ok) break;
+              o_phase ^= 1u;
+            }
+            tc_fence_after();
+            const uint32_t va = base + S::ring + (st % S::stages) * S::tile;
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+              mma_ts(tmem + kO[s], tmem + kS[s] + kPCol + k * 8, desc128(va + k * 2048, kTile * 128), kIdescO,
+                     (i > 0 || k > 0) ? 1u : 0u);
+            mma_commit(&bars->pv[s]);
+            if (!pair || s == 1) mma_commit(&bars->empty[st % S::stages]);
+            pending[s] = true;
+            pv_phase[s] ^= 1u;
+            if (i + 1 < ns[s]) ok = issue_s(s, i + 1);
+          }
+        }
+        first_seg = false;
+        ring += 2 * n;
+      }
+      // nothing may be in flight when the columns are released
+      mma_commit(&bars->done);
+      wait_or_abort(&bars->done, 0u, abort);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax of stream s
+    const int s = warp >> 2;
+    const int row = tid & (kTile - 1);
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lane_base + (s == 0 ? kS[0] : kS[1]);
+    const uint32_t to = tmem + lane_base + (s == 0 ? kO[0] : kO[1]);
+    uint32_t s_phase = 0u, pv_parity = 0u, x_phase = 0u;
+    bool ok = true;
+    while (ok && w.step()) {
+      const int n = w.t1 - w.t0;
+      const bool pair = w.it.pair;
+      const int steps = pair ? n : s == 0 ? (n + 1) / 2 : n / 2;
+      const int first_tok = pair ? s * a.tile_tokens : 0;
+      const int rows = min(a.tile_tokens, w.it.ntok - first_tok) * a.group;
+      const bool warp_live = (warp & 3) * 32 < rows;
+      // keys of the item this row sees
+      int visible = 0;
+      if (row < rows)
+        visible = w.it.b < 0 ? w.it.kend : clampi(static_cast<int64_t>(w.it.vis0) + row / a.group, 0, w.it.kend);
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < steps; ++i) {
+        const int t = w.t0 + (pair ? i : 2 * i + s);
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->s_full[s], s_phase, abort));
+        if (!ok) break;
+        s_phase ^= 1u;
+        tc_fence_after();
+        if (warp_live) {
+          const int lim = visible - t * kTile;  // columns below lim are seen
+          const bool all_seen = __all_sync(0xffffffffu, lim >= kTile || row >= rows);
+          uint32_t x[4][32];  // the last 64 columns stay; P goes where they were
+          float mt = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            ld32(ts + 32 * c, x[c]);
+            if (all_seen) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) mt = fmaxf(mt, __uint_as_float(x[c][j]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (32 * c + j < lim) mt = fmaxf(mt, __uint_as_float(x[c][j]));
+            }
+          }
+          mt *= a.scale_log2;
+          const bool grow = mt > m + 8.f || (m == -INFINITY && mt > -INFINITY);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float mn = grow ? mt : m;
+            const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mn)) : 1.f;
+            if (i > 0) {
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                ld32(to + 32 * c, o);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                st32(to + 32 * c, o);
+              }
+            }
+            l *= alpha;
+            m = mn;
+          }
+          const float neg = m == -INFINITY ? 0.f : -m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t p[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const int c = 2 * half + (j >> 4), e = (2 * j) & 31;
+              float p0 = ex2(fmaf(__uint_as_float(x[c][e]), a.scale_log2, neg));
+              float p1 = ex2(fmaf(__uint_as_float(x[c][e + 1]), a.scale_log2, neg));
+              if (!all_seen) {
+                if (64 * half + 2 * j >= lim) p0 = 0.f;
+                if (64 * half + 2 * j + 1 >= lim) p1 = 0.f;
+              }
+              sum[j & 1] += p0;
+              sum[2 + (j & 1)] += p1;
+              p[j] = pack2<QT>(p0, p1);
+            }
+            st32(ts + kPCol + 32 * half, p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          st_wait();
+        }
+        tc_fence_before();
+        mbar_arrive(&bars->p_full[s]);
+        if (i == steps - 1) break;
+        pv_parity ^= 1u;
+      }
+      if (!ok) break;
+      // ------------------------------------------------------------ the segment's partial
+      // scores that are all NaN leave no maximum: any reference carries their NaN on
+      if (l != l && m == -INFINITY) m = 0.f;
+      if (steps > 0) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->pv[s], pv_parity, abort));
+        if (!ok) break;
+        pv_parity ^= 1u;
+      }
+      if (!pair) {
+        // Both streams' sums belong to the same rows: exchange (m, l), then each stream joins
+        // and writes half of the dims. A stream without a tile waits here too, so that it
+        // cannot arrive twice in one phase of o_free. (m, l) of the segment before were read
+        // before this segment's first product could begin.
+        if (steps > 0) ml_sm[s * kTile + row] = make_float2(m, l);
+        tc_fence_before();
+        mbar_arrive(&bars->xch);
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->xch, x_phase, abort));
+        if (!ok) break;
+        x_phase ^= 1u;
+      }
+      tc_fence_after();
+      if (warp_live) {
+        const int64_t prow = w.partial_row(cta) + first_tok * a.group + row;
+        if (pair) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            ld32(to + 32 * c, o);
+            if (row < rows) store_o(a.o + prow * D + 32 * c, o);
+          }
+          if (row < rows) reinterpret_cast<float2*>(a.ml)[prow] = make_float2(m, l);
+        } else {
+          const float2 ml0 = ml_sm[row], ml1 = n > 1 ? ml_sm[kTile + row] : make_float2(-INFINITY, 0.f);
+          const float mm = fmaxf(ml0.x, ml1.x);
+          const float w0 = ml0.x == -INFINITY ? 0.f : ex2(ml0.x - mm), w1 = ml1.x == -INFINITY ? 0.f : ex2(ml1.x - mm);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            const int col = s * (D / 2) + 32 * c;
+            uint32_t o0[32], o1[32];
+            ld32(tmem + lane_base + kO[0] + col, o0);
+            if (n > 1) {
+              ld32(tmem + lane_base + kO[1] + col, o1);
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                o0[j] = __float_as_uint(fmaf(__uint_as_float(o0[j]), w0, __uint_as_float(o1[j]) * w1));
+            }
+            if (row < rows) store_o(a.o + prow * D + col, o0);
+          }
+          if (row < rows && s == 0)
+            reinterpret_cast<float2*>(a.ml)[prow] = n > 1 ? make_float2(mm, fmaf(ml0.y, w0, ml1.y * w1)) : ml0;
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&bars->o_free);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_sm && tid == 0 && a.err) atomicOr(a.err, kWaitTimeoutFlag);
+  if (warp == 12) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Joins the partials of each row: one warp per (token, query head).
+// ---------------------------------------------------------------------------------------
+template <typename QT, int D>
+__global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ SharedArgs a) {
+  using namespace spa;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  constexpr int kPer = D / 32;  // dims per lane
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t t = blockIdx.x;
+  const int qh = static_cast<int>(blockIdx.y) * 8 + warp;
+  const int used = used_tokens(a);
+  if (qh >= a.q_heads || t >= used || t < clampi(__ldg(a.query_start), 0, a.tokens)) return;
+  const int h = qh / a.group, g = qh - h * a.group;
+  const int64_t wp = __ldcg(a.head), ws = __ldcg(a.head + 1);
+  const int64_t all = (wp + ws) * a.kv_heads;
+  // the request: token t itself in a step of one token each, else by bisection
+  int b = clampi(t, 0, a.requests - 1);
+  if (!(__ldg(a.query_start + b) <= t && t < __ldg(a.query_start + b + 1))) {
+    int lo = 0, hi = a.requests;  // query_start[lo] <= t < query_start[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(a.query_start + mid) <= t) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+  }
+  const Request r(a, b);
+  Item its[2];
+  {
+    const int per = prefix_item_tokens(a, used);
+    const int64_t i = t / per;
+    its[0] = prefix_item(a, used, h, i * per, h * wp + i * prefix_item(a, used, 0, 0, 0).cost());
+    const int tile = clampi((t - r.begin) / a.tile_tokens, 0, r.n > 0 ? (r.n - 1) / a.tile_tokens : 0);
+    int64_t start = a.kv_heads * wp + h * ws + __ldcg(a.req_cost + b);
+    for (int k = 0; k < tile; ++k) start += suffix_item(a, r, h, b, k, 0).cost();
+    its[1] = suffix_item(a, r, h, b, tile, start);
+  }
+  float acc[kPer], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    const Item& it = its[k];
+    if (it.kend <= 0) continue;
+    // shares that can hold a tile of the item
+    int c0 = static_cast<int>(it.start * a.ctas / all), c1 = static_cast<int>((it.start + it.cost()) * a.ctas / all);
+    c0 = max(c0 - 1, 0);
+    c1 = min(c1 + 1, a.ctas - 1);
+    for (int cb = c0; cb <= c1; cb += 32) {
+      const int c = cb + lane;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (c <= c1 && it.tile_at(all * (c + 1) / a.ctas) > it.tile_at(all * c / a.ctas))
+        ml = __ldcg(reinterpret_cast<const float2*>(a.ml) + partial_base(a, it, c) + (t - it.tok0) * a.group + g);
+      float mx = ml.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float mn = fmaxf(m, mx);
+      if (mn == -INFINITY) continue;  // nothing with weight here
+      const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+      const float wgt = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
+      float sum = wgt * ml.y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l = fmaf(l, alpha, sum);
+      m = mn;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) acc[i] *= alpha;
+      unsigned live = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+      const float* o0 = a.o + (partial_base(a, it, cb) + (t - it.tok0) * a.group + g) * D + lane * kPer;
+      const int64_t stride = static_cast<int64_t>(it.b < 0 ? a.item_rows_p : a.item_rows_s) * D;
+      while (live) {
+        float v[4][kPer], wv[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int src = live ? __ffs(live) - 1 : 0;
+          wv[u] = live ? 1.f : 0.f;
+          wv[u] *= __shfl_sync(0xffffffffu, wgt, src);
+          const float* p = o0 + src * stride;
+          if (live) {
+            if constexpr (kPer == 4) {
+              const float4 f = __ldcg(reinterpret_cast<const float4*>(p));
+              v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
+            } else {
+              const float2 f = __ldcg(reinterpret_cast<const float2*>(p));
+              v[u][0] = f.x, v[u][1] = f.y;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) v[u][i] = 0.f;
+          }
+          live &= live - 1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) acc[i] = fmaf(v[u][i], wv[u], acc[i]);
+      }
+    }
+  }
+  // l > 0 wherever a key has weight; NaN stays NaN
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* out = a.output + t * a.o_token + static_cast<int64_t>(qh) * a.o_head + lane * kPer;
+  uint32_t packed[kPer / 2];
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i) packed[i] = pack2<QT>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  if (a.o_vec) {
+    if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(packed[0], packed[1]);
+    else *reinterpret_cast<uint32_t*>(out) = packed[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) out[i] = static_cast<uint16_t>(packed[i / 2] >> (16 * (i & 1)));
+  }
+  if (a.lse && lane == 0)
+    a.lse[t * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
+}  // namespace origami
