@@ -17,7 +17,7 @@
 // in equal contiguous shares: no tail, no atomics, a fixed order of summation. A share's piece
 // of an item (a "segment") writes one partial; merge_partials joins each row's partials.
 //
-// A CTA (13 warps): 4 loader warps gather K and V tiles through the block tables with 16-byte
+// A CTA: 4 loader warps gather K and V tiles through the block tables with 16-byte
 // cp.async into a ring of 128-byte-swizzled tiles (any block size; rows past the end become
 // zeros, so garbage there cannot reach the products); one thread issues tcgen05.mma; two
 // softmax warpgroups own one stream each, a stream being one (S, O) accumulator pair in TMEM:
@@ -41,7 +41,11 @@ namespace origami {
 
 namespace spa {
 
-constexpr int kThreadsS = 416;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12: MMA
+constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12: MMA
+// Registers per thread at launch, then of the softmax warpgroups and of the others:
+// 256 * 176 + 256 * 80 = 512 * 128, all that the block was launched with.
+constexpr int kRegsLaunch = 128, kRegsSoftmax = 176, kRegsOther = 80;
+static_assert(256 * (kRegsSoftmax + kRegsOther) <= kThreadsS * kRegsLaunch, "register shares");
 constexpr int kTile = 128;      // keys per tile, rows per row tile
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of a segment.
 constexpr int kCostTile = 8, kCostPair = 8, kCostItem = 4;
@@ -51,10 +55,9 @@ template <int D>
 struct Smem {
   static constexpr int tile = kTile * D * 2;
   static constexpr int stages = D == 128 ? 5 : 10;
-  static constexpr int lag = D == 128 ? 3 : 6;  // stages a loader keeps in flight
   static constexpr int ring = 2 * tile;
   static constexpr int scalars = ring + stages * tile;
-  static constexpr int bytes = scalars + 2 * kTile * 8 + 512;
+  static constexpr int bytes = scalars + 2 * kTile * 8 + 1024;
 };
 
 }  // namespace spa
@@ -189,7 +192,7 @@ struct Deal {
   int64_t start;
 };
 
-// Walks the segments of a CTA's share. Every role runs its own copy.
+// Walks the segments of a CTA's share (one warp of the CTA).
 struct Walk {
   const SharedArgs& a;
   const Deal& d;
@@ -258,9 +261,16 @@ struct Walk {
     }
     return false;
   }
-  // Partial row of the segment's first row.
-  __device__ __forceinline__ int64_t partial_row(int cta) const;
 };
+
+// A segment as the other warps read it from shared memory.
+struct Segment {
+  int64_t prow;       // partial row of its first row
+  int32_t t0, n;      // first tile, tiles; n = 0 ends the share
+  int32_t pair, h, b;  // two row tiles; KV head; request, -1 for the prefix
+  int32_t tok0, ntok, kend, vis0;
+};
+constexpr int kSegments = 4;  // in the ring between the scheduler and the others
 
 // Partial rows: an item's rows begin at its place among all rows of its kind plus its CTA's
 // index times the rows one item may have. Two segments never overlap: a later CTA's segment of
@@ -271,7 +281,6 @@ __device__ __forceinline__ int64_t partial_base(const SharedArgs& a, const Item&
   return static_cast<int64_t>(a.q_heads) * a.tokens + static_cast<int64_t>(a.ctas) * a.item_rows_p + rows +
          static_cast<int64_t>(cta) * a.item_rows_s;
 }
-__device__ __forceinline__ int64_t Walk::partial_row(int cta) const { return partial_base(a, it, cta); }
 
 // ---------------------------------------------------------------------------------------
 // tcgen05 helpers
@@ -311,15 +320,41 @@ __device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
+// 128 columns: four loads in flight, one wait. The empty statements tie every value to the
+// wait, so that none is used before it.
+__device__ __forceinline__ void ld128(uint32_t addr, uint32_t (&r)[128]) {
+#pragma unroll
+  for (int c = 0; c < 128; c += 32)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31}, [%32];\n"
+        : "=r"(r[c]), "=r"(r[c + 1]), "=r"(r[c + 2]), "=r"(r[c + 3]), "=r"(r[c + 4]), "=r"(r[c + 5]), "=r"(r[c + 6]),
+          "=r"(r[c + 7]), "=r"(r[c + 8]), "=r"(r[c + 9]), "=r"(r[c + 10]), "=r"(r[c + 11]), "=r"(r[c + 12]),
+          "=r"(r[c + 13]), "=r"(r[c + 14]), "=r"(r[c + 15]), "=r"(r[c + 16]), "=r"(r[c + 17]), "=r"(r[c + 18]),
+          "=r"(r[c + 19]), "=r"(r[c + 20]), "=r"(r[c + 21]), "=r"(r[c + 22]), "=r"(r[c + 23]), "=r"(r[c + 24]),
+          "=r"(r[c + 25]), "=r"(r[c + 26]), "=r"(r[c + 27]), "=r"(r[c + 28]), "=r"(r[c + 29]), "=r"(r[c + 30]),
+          "=r"(r[c + 31])
+        : "r"(addr + c)
+        : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < 128; ++j) asm volatile("" : "+r"(r[j]));
+}
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31,%32};\n" ::"r"(addr),
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      " tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
@@ -369,7 +404,8 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
 }
 
 struct Bars {
-  uint64_t full[10], empty[10], q_empty[2], s_full[2], p_full[2], pv[2], o_free, xch, done;
+  uint64_t full[10], empty[10], q_empty[2], s_full[2], p_full[2], pv[2], seg_full[kSegments], seg_empty[kSegments];
+  uint64_t o_free, xch, done;
 };
 
 }  // namespace spa
@@ -388,12 +424,13 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + 1);
   int* abort_sm = reinterpret_cast<int*>(tslot + 1);
   Deal* deal_sm = reinterpret_cast<Deal*>(tslot + 2);
-  static_assert(sizeof(Bars) + 8 + sizeof(Deal) <= 512, "scalars fit");
+  Segment* segs = reinterpret_cast<Segment*>(deal_sm + 1);
+  static_assert(sizeof(Bars) + 8 + sizeof(Deal) + kSegments * sizeof(Segment) <= 1024, "scalars fit");
   static_assert(S::bytes <= 227 * 1024, "shared memory of one SM");
   constexpr bool kBf16 = attn::is_bf16<QT>();
   constexpr uint32_t kIdescS = attn::instr_desc(kBf16, kTile);
   constexpr uint32_t kIdescO = attn::instr_desc(kBf16, D) | (1u << 16);  // B (V) is N-major
-  constexpr uint32_t kS[2] = {0, 128}, kO[2] = {256, 384};
+  constexpr uint32_t kO = 256;  // S_s at column 128 s, O_s at 256 + 128 s
   constexpr uint32_t kPCol = 64;  // P lies over the second half of S
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -405,7 +442,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   }
   if (tid == 0) {
     for (int i = 0; i < S::stages; ++i) {
-      mbar_init(&bars->full[i], 4);
+      mbar_init(&bars->full[i], 4 * 32);
       mbar_init(&bars->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -413,6 +450,10 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], kTile);
       mbar_init(&bars->pv[i], 1);
+    }
+    for (int i = 0; i < kSegments; ++i) {
+      mbar_init(&bars->seg_full[i], 1);
+      mbar_init(&bars->seg_empty[i], 8 + 4 + 1);  // softmax and loader warps, the products' thread
     }
     mbar_init(&bars->o_free, 2 * kTile);
     mbar_init(&bars->xch, 2 * kTile);
@@ -503,198 +544,213 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tslot;
-  const Deal deal = *deal_sm;
   volatile int* abort = abort_sm;
-  Walk w(a, deal);
 
   if (warp >= 8 && warp < 12) {
     // ---------------------------------------------------------------- loaders
     // Warp lw fills rows 32 lw .. 32 lw + 31 of every tile; lane l knows row 32 lw + l.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
     constexpr int kChunks = D / 8;          // 16-byte chunks per row
     constexpr int kRowsPer = 32 / kChunks;  // rows a warp copies at once
     const int lw = warp - 8;
     const int sub = lane / kChunks, chunk = lane % kChunks;
+    // this lane's chunk of row 32 lw + sub; kRowsPer rows on, the row's swizzle changes
     const uint32_t base = smem_u32(sm);
-    int ring = 0, signalled = 0;  // stages issued / signalled
-    uint32_t q_uses[2] = {0u, 0u};
-    int q_next = 0;
-    bool ok = true;
-    auto signal_one = [&]() {
-      proxy_fence();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->full[signalled % S::stages]);
-      ++signalled;
-    };
-    auto drain = [&]() {
-      asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-      while (signalled < ring) signal_one();
-    };
-    // cache row of key `key` of this item, -1 past its end, -2 outside the cache
-    auto row_of = [&](int64_t key) -> int {
-      if (key >= w.it.kend) return -1;
-      const uint32_t k = static_cast<uint32_t>(key), page = k / static_cast<uint32_t>(a.block_size);
-      const int32_t* table = w.it.b < 0 ? a.prefix_blocks : a.suffix_blocks + w.it.b * a.suffix_stride;
-      const int pb = __ldg(table + page);
-      if (pb < 0 || pb >= a.num_blocks) return -2;
-      return pb * a.block_rows + static_cast<int>(k - page * static_cast<uint32_t>(a.block_size));
-    };
-    // Waits until stage `ring` may be refilled.
-    auto acquire = [&]() {
-      const int st = ring % S::stages, use = ring / S::stages;
-      if (use == 0) return;
-      const uint32_t parity = static_cast<uint32_t>((use - 1) & 1);
-      bool ready = mbar_wait_bounded(&bars->empty[st], parity, 1);
-      ready = __all_sync(0xffffffffu, ready);
-      if (!ready) {
-        drain();  // whoever frees the stage may need the ones in flight
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->empty[st], parity, abort));
+    uint32_t ring = 0, slot = 0, q_used = 0u, q_phase = 0u, q_next = 0u;
+    bool ok = true, plain_q = false;
+    // Waits until stage `ring` may be refilled, copies this warp's rows of K or V into it. The
+    // stage is full when every loader thread's copies so far have landed (Q's with the first K's).
+    auto emit = [&](int row, const uint16_t* src) {
+      const uint32_t st = ring % S::stages, use = ring / S::stages;
+      if (use > 0) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->empty[st], (use - 1) & 1u, abort));
+        if (!ok) return;
       }
-    };
-    auto emit = [&](int row, int which) {
-      acquire();
-      if (!ok) return;
-      const uint32_t dst = base + S::ring + (ring % S::stages) * S::tile;
-      const uint16_t* src = a.cache + which * a.kv_stride + static_cast<int64_t>(w.it.h) * D + chunk * 8;
-#pragma unroll 8
+      const uint32_t dst = base + S::ring + st * S::tile;
+#pragma unroll 4
       for (int i = 0; i < 32 / kRowsPer; ++i) {
         const int r = i * kRowsPer + sub;
         const int cr = __shfl_sync(0xffffffffu, row, r);
         cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
       }
-      asm volatile("cp.async.commit_group;\n" ::: "memory");
-      ++ring;
-      if (ring - signalled > S::lag) {
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(S::lag) : "memory");
-        signal_one();
+      if (plain_q) {  // Q came through registers: an arrival that releases those stores too
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
+        mbar_arrive(&bars->full[st]);
+        plain_q = false;
+      } else {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&bars->full[st])) : "memory");
       }
+      ++ring;
     };
-    while (ok && w.step()) {
+    for (;; ++slot) {
+      ok = ok && __all_sync(0xffffffffu, wait_or_abort(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u, abort));
+      if (!ok) break;
+      const Segment seg = segs[slot % kSegments];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->seg_empty[slot % kSegments]);
+      if (seg.n == 0) break;
+      const int32_t* table = seg.b < 0 ? a.prefix_blocks : a.suffix_blocks + seg.b * a.suffix_stride;
+      // cache row of key `key`, negative past the end of the item or outside the cache
+      auto row_of = [&](int key) -> int {
+        if (key >= seg.kend) return -1;
+        const uint32_t page = static_cast<uint32_t>(key) / static_cast<uint32_t>(a.block_size);
+        const int pb = __ldg(table + page);
+        return pb < 0 || pb >= a.num_blocks ? -1 : pb * a.block_rows + (key - static_cast<int>(page) * a.block_size);
+      };
+      int key = seg.t0 * kTile + 32 * lw + lane;
+      int row = row_of(key), prev = -1;
       // Q: one row tile, into the buffer after the last one used, or both for a pair
-      const int tiles_q = w.it.pair ? 2 : 1;
-      if (w.it.pair) q_next = 0;
-      for (int q = 0; q < tiles_q && ok; ++q) {
-        const int buf = q_next;
-        q_next ^= 1;
-        if (q_uses[buf] > 0) {
-          const uint32_t parity = (q_uses[buf] - 1) & 1u;
-          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars->q_empty[buf], parity, 1))) {
-            drain();
-            ok = __all_sync(0xffffffffu, wait_or_abort(&bars->q_empty[buf], parity, abort));
-            if (!ok) break;
-          }
+      if (seg.pair) q_next = 0;
+#pragma unroll 1
+      for (int q = 0; q <= seg.pair; ++q) {
+        const uint32_t buf = q_next;
+        q_next ^= 1u;
+        if ((q_used >> buf) & 1u) {
+          ok = __all_sync(0xffffffffu, wait_or_abort(&bars->q_empty[buf], (q_phase >> buf) & 1u, abort));
+          if (!ok) break;
+          q_phase ^= 1u << buf;
         }
-        ++q_uses[buf];
-        const int rows = min(a.tile_tokens, w.it.ntok - q * a.tile_tokens) * a.group;
-        const int64_t tok = w.it.tok0 + q * a.tile_tokens;
+        q_used |= 1u << buf;
+        // lane l finds the query row of tile row 32 lw + l
+        const int tile_row = 32 * lw + lane, tl = tile_row / a.group;
+        const int rows = min(a.tile_tokens, seg.ntok - q * a.tile_tokens) * a.group;
+        const int64_t at = tile_row < rows ? (seg.tok0 + static_cast<int64_t>(q) * a.tile_tokens + tl) * a.q_token +
+                                                 (seg.h * a.group + tile_row - tl * a.group) * a.q_head
+                                           : -1;
         const uint32_t dst = base + buf * S::tile;
-#pragma unroll 4
+#pragma unroll 2
         for (int i = 0; i < 32 / kRowsPer; ++i) {
-          const int r = 32 * lw + i * kRowsPer + sub;
-          const bool valid = r < rows;
-          const int64_t t = tok + (valid ? r / a.group : 0);
-          const int qh = w.it.h * a.group + (valid ? r % a.group : 0);
-          const uint16_t* src = a.query + t * a.q_token + qh * a.q_head + chunk * 8;
+          const int r = i * kRowsPer + sub;
+          const int64_t from = __shfl_sync(0xffffffffu, at, r);
+          const uint16_t* src = a.query + (from < 0 ? 0 : from) + chunk * 8;
           if (a.q_vec) {
-            cp16_or_zero(dst + chunk_off(r, chunk), src, valid);
+            cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src, from >= 0);
           } else {
             uint32_t v[4] = {0u, 0u, 0u, 0u};
-            if (valid) {
+            if (from >= 0) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) v[j] = src[2 * j] | (static_cast<uint32_t>(src[2 * j + 1]) << 16);
             }
-            *reinterpret_cast<uint4*>(sm + buf * S::tile + chunk_off(r, chunk)) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(sm + buf * S::tile + chunk_off(32 * lw + r, chunk)) =
+                make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
       }
       if (!ok) break;
+      plain_q = !a.q_vec;
       // pair: K V K V ..; split: K K V K V .. V, the order in which the products first use them
-      const int n = w.t1 - w.t0;
-      int row = row_of(static_cast<int64_t>(w.t0) * kTile + 32 * lw + lane), prev = -1;
-      for (int i = 0; i <= n && ok; ++i) {
-        const int next_row = i + 1 < n ? row_of(static_cast<int64_t>(w.t0 + i + 1) * kTile + 32 * lw + lane) : -1;
-        if (i < n) emit(row, 0);
-        if (w.it.pair) {
-          if (i < n && ok) emit(row, 1);
-        } else if (i > 0 && ok) {
-          emit(prev, 1);
-        }
+      const uint16_t* k_src = a.cache + static_cast<int64_t>(seg.h) * D + chunk * 8;
+      const uint16_t* v_src = k_src + a.kv_stride;
+#pragma unroll 1
+      for (int i = 0; i <= seg.n && ok; ++i) {
+        key += kTile;
+        const int next_row = i + 1 < seg.n ? row_of(key) : -1;
+        if (i < seg.n) emit(row, k_src);
+        const bool v_now = seg.pair ? i < seg.n : i > 0;
+        if (v_now && ok) emit(seg.pair ? row : prev, v_src);
         prev = row;
         row = next_row;
       }
     }
-    drain();
-  } else if (warp == 12) {
-    // ---------------------------------------------------------------- products
-    if (lane == 0) {
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
+    if (warp == 13 && lane == 0) {
+      // -------------------------------------------------------------- scheduler
+      const Deal deal = *deal_sm;
+      Walk w(a, deal);
+      for (uint32_t slot = 0;; ++slot) {
+        const uint32_t at = slot % kSegments, use = slot / kSegments;
+        const bool more = w.step();
+        if (use > 0 && !wait_or_abort(&bars->seg_empty[at], (use - 1) & 1u, abort)) break;
+        Segment& g = segs[at];
+        g.n = more ? w.t1 - w.t0 : 0;
+        g.t0 = w.t0;
+        g.pair = w.it.pair;
+        g.h = w.it.h;
+        g.b = w.it.b;
+        g.tok0 = static_cast<int32_t>(w.it.tok0);
+        g.ntok = w.it.ntok;
+        g.kend = w.it.kend;
+        g.vis0 = w.it.vis0;
+        g.prow = more ? partial_base(a, w.it, cta) : 0;
+        mbar_arrive(&bars->seg_full[at]);
+        if (!more) break;
+      }
+    } else if (warp == 12 && lane == 0) {
+      // -------------------------------------------------------------- products
       const uint32_t base = smem_u32(sm);
-      int ring = 0;  // stage index at which the segment begins
-      uint32_t p_phase[2] = {0u, 0u}, pv_phase[2] = {0u, 0u}, o_phase = 0u;
-      int q_next = 0;
-      bool pending[2] = {false, false};  // a product of the stream that was not waited for
-      bool first_seg = true, ok = true;
-      while (ok && w.step()) {
-        const int n = w.t1 - w.t0;
-        const bool pair = w.it.pair;
-        const int ns[2] = {pair ? n : (n + 1) / 2, pair ? n : n / 2};
+      uint32_t ring = 0;  // stage index at which the segment begins
+      // phases and pending products (not waited for yet) of the streams, bit s
+      uint32_t p_phase = 0u, pv_phase = 0u, pending = 0u, o_phase = 0u, q_next = 0u;
+      bool ok = true;
+      for (uint32_t slot = 0;; ++slot) {
+        if (!ok || !wait_or_abort(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u, abort)) break;
+        const int n = segs[slot % kSegments].n;
+        const bool pair = segs[slot % kSegments].pair != 0;
+        mbar_arrive(&bars->seg_empty[slot % kSegments]);
+        if (n == 0) break;
+        const int ns0 = pair ? n : (n + 1) / 2, ns1 = pair ? n : n / 2;
         if (pair) q_next = 0;
-        const int qb[2] = {q_next, pair ? 1 : q_next};
-        if (!pair) q_next ^= 1;
-        auto stage_k = [&](int t) { return ring + (pair ? 2 * t : t == 0 ? 0 : 2 * t - 1); };
-        auto stage_v = [&](int t) { return ring + (pair ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1)); };
-        auto wait_full = [&](int st) {
-          return wait_or_abort(&bars->full[st % S::stages], static_cast<uint32_t>((st / S::stages) & 1), abort);
+        const uint32_t qb = q_next;
+        if (!pair) q_next ^= 1u;
+        // the copies are generic-proxy writes: the fence orders the products' reads behind them
+        auto wait_full = [&](uint32_t st) {
+          const bool full = wait_or_abort(&bars->full[st % S::stages], (st / S::stages) & 1u, abort);
+          proxy_fence();
+          return full;
         };
-        auto tile_of = [&](int s, int i) { return pair ? i : 2 * i + s; };
-        auto issue_s = [&](int s, int i) {
-          const int st = stage_k(tile_of(s, i));
+        auto issue_s = [&](uint32_t s, int i) {
+          const int t = pair ? i : 2 * i + static_cast<int>(s);
+          const uint32_t st = ring + (pair ? 2 * t : t == 0 ? 0 : 2 * t - 1);
           if (!wait_full(st)) return false;
           // P lies in S: the product that reads it must have ended before S is written again
-          if (pending[s] && !wait_or_abort(&bars->pv[s], pv_phase[s] ^ 1u, abort)) return false;
-          pending[s] = false;
+          if (((pending >> s) & 1u) && !wait_or_abort(&bars->pv[s], ((pv_phase >> s) & 1u) ^ 1u, abort)) return false;
+          pending &= ~(1u << s);
           tc_fence_after();
-          const uint32_t qa = base + qb[s] * S::tile, ka = base + S::ring + (st % S::stages) * S::tile;
+          const uint64_t qd = desc128(base + (pair ? s : qb) * S::tile, 16);
+          const uint64_t kd = desc128(base + S::ring + (st % S::stages) * S::tile, 16);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-            mma_ss(tmem + kS[s], desc128(qa + off, 16), desc128(ka + off, 16), kIdescS, k > 0 ? 1u : 0u);
+            const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+            mma_ss(tmem + 128 * s, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
           }
           mma_commit(&bars->s_full[s]);
           if (!pair || s == 1) mma_commit(&bars->empty[st % S::stages]);
           // the last product that reads a Q buffer frees it
-          if (i == ns[s] - 1) {
-            if (pair) mma_commit(&bars->q_empty[s]);
-            else if (tile_of(s, i) == n - 1) mma_commit(&bars->q_empty[qb[0]]);
-          }
+          if (pair ? i == n - 1 : t == n - 1) mma_commit(&bars->q_empty[pair ? s : qb]);
           return true;
         };
-        for (int s = 0; s < 2 && ok; ++s)
-          if (ns[s] > 0) ok = issue_s(s, 0);
-        for (int i = 0; i < ns[0] && ok; ++i) {
-          for (int s = 0; s < 2 && ok; ++s) {
-            if (i >= ns[s]) continue;
-            const int st = stage_v(tile_of(s, i));
-            ok = wait_full(st) && wait_or_abort(&bars->p_full[s], p_phase[s], abort);
+        ok = issue_s(0, 0);
+        if (ok && ns1 > 0) ok = issue_s(1, 0);
+#pragma unroll 1
+        for (int i = 0; i < ns0 && ok; ++i) {
+#pragma unroll 1
+          for (uint32_t s = 0; s < 2 && ok; ++s) {
+            if (s == 1 && i >= ns1) break;
+            const int t = pair ? i : 2 * i + static_cast<int>(s);
+            const uint32_t st = ring + (pair ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1));
+            ok = wait_full(st) && wait_or_abort(&bars->p_full[s], (p_phase >> s) & 1u, abort);
             if (!ok) break;
-            p_phase[s] ^= 1u;
-            if (i == 0 && s == 0 && !first_seg) {  // the last segment's O has been read
+            p_phase ^= 1u << s;
+            if (i == 0 && s == 0 && slot > 0) {  // the last segment's O has been read
               ok = wait_or_abort(&bars->o_free, o_phase, abort);
               if (!ok) break;
               o_phase ^= 1u;
             }
             tc_fence_after();
-            const uint32_t va = base + S::ring + (st % S::stages) * S::tile;
+            const uint64_t vd = desc128(base + S::ring + (st % S::stages) * S::tile, kTile * 128);
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              mma_ts(tmem + kO[s], tmem + kS[s] + kPCol + k * 8, desc128(va + k * 2048, kTile * 128), kIdescO,
+              mma_ts(tmem + kO + 128 * s, tmem + 128 * s + kPCol + k * 8, vd + k * (2048 >> 4), kIdescO,
                      (i > 0 || k > 0) ? 1u : 0u);
             mma_commit(&bars->pv[s]);
             if (!pair || s == 1) mma_commit(&bars->empty[st % S::stages]);
-            pending[s] = true;
-            pv_phase[s] ^= 1u;
-            if (i + 1 < ns[s]) ok = issue_s(s, i + 1);
+            pending |= 1u << s;
+            pv_phase ^= 1u << s;
+            if (i + 1 < (s == 0 ? ns0 : ns1)) ok = issue_s(s, i + 1);
           }
         }
-        first_seg = false;
         ring += 2 * n;
       }
       // nothing may be in flight when the columns are released
@@ -704,102 +760,101 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax of stream s
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax));
     const int s = warp >> 2;
     const int row = tid & (kTile - 1);
-    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lane_base + (s == 0 ? kS[0] : kS[1]);
-    const uint32_t to = tmem + lane_base + (s == 0 ? kO[0] : kO[1]);
-    uint32_t s_phase = 0u, pv_parity = 0u, x_phase = 0u;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t ts = lane_base + 128 * s, to = lane_base + kO + 128 * s;
+    const int token_in_tile = row / a.group;
+    uint32_t s_phase = 0u, pv_phase = 0u, x_phase = 0u;
     bool ok = true;
-    while (ok && w.step()) {
-      const int n = w.t1 - w.t0;
-      const bool pair = w.it.pair;
-      const int steps = pair ? n : s == 0 ? (n + 1) / 2 : n / 2;
+    for (uint32_t slot = 0;; ++slot) {
+      ok = ok && __all_sync(0xffffffffu, wait_or_abort(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u, abort));
+      if (!ok) break;
+      const Segment seg = segs[slot % kSegments];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->seg_empty[slot % kSegments]);
+      if (seg.n == 0) break;
+      const bool pair = seg.pair != 0;
+      const int steps = pair ? seg.n : s == 0 ? (seg.n + 1) / 2 : seg.n / 2;
       const int first_tok = pair ? s * a.tile_tokens : 0;
-      const int rows = min(a.tile_tokens, w.it.ntok - first_tok) * a.group;
+      const int rows = min(a.tile_tokens, seg.ntok - first_tok) * a.group;
       const bool warp_live = (warp & 3) * 32 < rows;
-      // keys of the item this row sees
-      int visible = 0;
-      if (row < rows)
-        visible = w.it.b < 0 ? w.it.kend : clampi(static_cast<int64_t>(w.it.vis0) + row / a.group, 0, w.it.kend);
+      // keys of the item this row sees, less those before the current tile
+      int lim = 0;
+      if (row < rows) lim = seg.b < 0 ? seg.kend : clampi(static_cast<int64_t>(seg.vis0) + token_in_tile, 0, seg.kend);
+      lim -= (seg.t0 + (pair ? 0 : s)) * kTile;
       float m = -INFINITY, l = 0.f;
+#pragma unroll 1
       for (int i = 0; i < steps; ++i) {
-        const int t = w.t0 + (pair ? i : 2 * i + s);
         ok = __all_sync(0xffffffffu, wait_or_abort(&bars->s_full[s], s_phase, abort));
         if (!ok) break;
         s_phase ^= 1u;
         tc_fence_after();
         if (warp_live) {
-          const int lim = visible - t * kTile;  // columns below lim are seen
-          const bool all_seen = __all_sync(0xffffffffu, lim >= kTile || row >= rows);
-          uint32_t x[4][32];  // the last 64 columns stay; P goes where they were
-          float mt = -INFINITY;
+          uint32_t x[128];  // P goes over the second half of S, so all of S is read first
+          ld128(ts, x);
+          if (!__all_sync(0xffffffffu, lim >= kTile || row >= rows)) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            ld32(ts + 32 * c, x[c]);
-            if (all_seen) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) mt = fmaxf(mt, __uint_as_float(x[c][j]));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (32 * c + j < lim) mt = fmaxf(mt, __uint_as_float(x[c][j]));
-            }
+            for (int j = 0; j < kTile; ++j)
+              if (j >= lim) x[j] = 0xFF800000u;  // -inf: not seen
           }
-          mt *= a.scale_log2;
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < kTile; j += 8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(x[j + 2 * k]), __uint_as_float(x[j + 2 * k + 1])));
+          }
+          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
           const bool grow = mt > m + 8.f || (m == -INFINITY && mt > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
-            const float mn = grow ? mt : m;
-            const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mn)) : 1.f;
+            const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mt)) : 1.f;
             if (i > 0) {
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                ld16(to + c, o);
 #pragma unroll
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                ld32(to + 32 * c, o);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                st32(to + 32 * c, o);
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                st16(to + c, o);
               }
             }
             l *= alpha;
-            m = mn;
+            m = grow ? mt : m;
           }
           const float neg = m == -INFINITY ? 0.f : -m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t p[32];
+          for (int q = 0; q < 4; ++q) {
+            uint32_t p[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int c = 2 * half + (j >> 4), e = (2 * j) & 31;
-              float p0 = ex2(fmaf(__uint_as_float(x[c][e]), a.scale_log2, neg));
-              float p1 = ex2(fmaf(__uint_as_float(x[c][e + 1]), a.scale_log2, neg));
-              if (!all_seen) {
-                if (64 * half + 2 * j >= lim) p0 = 0.f;
-                if (64 * half + 2 * j + 1 >= lim) p1 = 0.f;
-              }
+            for (int j = 0; j < 16; ++j) {
+              const float p0 = ex2(fmaf(__uint_as_float(x[32 * q + 2 * j]), a.scale_log2, neg));
+              const float p1 = ex2(fmaf(__uint_as_float(x[32 * q + 2 * j + 1]), a.scale_log2, neg));
               sum[j & 1] += p0;
               sum[2 + (j & 1)] += p1;
               p[j] = pack2<QT>(p0, p1);
             }
-            st32(ts + kPCol + 32 * half, p);
+            st16(ts + kPCol + 16 * q, p);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           st_wait();
         }
         tc_fence_before();
         mbar_arrive(&bars->p_full[s]);
-        if (i == steps - 1) break;
-        pv_parity ^= 1u;
+        lim -= pair ? kTile : 2 * kTile;
       }
       if (!ok) break;
       // ------------------------------------------------------------ the segment's partial
       // scores that are all NaN leave no maximum: any reference carries their NaN on
       if (l != l && m == -INFINITY) m = 0.f;
       if (steps > 0) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->pv[s], pv_parity, abort));
+        // one phase per step: the last one's parity
+        pv_phase ^= static_cast<uint32_t>(steps - 1) & 1u;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->pv[s], pv_phase, abort));
         if (!ok) break;
-        pv_parity ^= 1u;
+        pv_phase ^= 1u;
       }
       if (!pair) {
         // Both streams' sums belong to the same rows: exchange (m, l), then each stream joins
@@ -815,26 +870,27 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       }
       tc_fence_after();
       if (warp_live) {
-        const int64_t prow = w.partial_row(cta) + first_tok * a.group + row;
+        const int64_t prow = seg.prow + first_tok * a.group + row;
         if (pair) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
-            ld32(to + 32 * c, o);
-            if (row < rows) store_o(a.o + prow * D + 32 * c, o);
+            ld32(to + c, o);
+            if (row < rows) store_o(a.o + prow * D + c, o);
           }
           if (row < rows) reinterpret_cast<float2*>(a.ml)[prow] = make_float2(m, l);
         } else {
-          const float2 ml0 = ml_sm[row], ml1 = n > 1 ? ml_sm[kTile + row] : make_float2(-INFINITY, 0.f);
+          const bool two = seg.n > 1;
+          const float2 ml0 = ml_sm[row], ml1 = two ? ml_sm[kTile + row] : make_float2(-INFINITY, 0.f);
           const float mm = fmaxf(ml0.x, ml1.x);
           const float w0 = ml0.x == -INFINITY ? 0.f : ex2(ml0.x - mm), w1 = ml1.x == -INFINITY ? 0.f : ex2(ml1.x - mm);
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            const int col = s * (D / 2) + 32 * c;
+#pragma unroll 1
+          for (int c = 0; c < D / 2; c += 32) {
+            const int col = s * (D / 2) + c;
             uint32_t o0[32], o1[32];
-            ld32(tmem + lane_base + kO[0] + col, o0);
-            if (n > 1) {
-              ld32(tmem + lane_base + kO[1] + col, o1);
+            ld32(lane_base + kO + col, o0);
+            if (two) {
+              ld32(lane_base + kO + 128 + col, o1);
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 o0[j] = __float_as_uint(fmaf(__uint_as_float(o0[j]), w0, __uint_as_float(o1[j]) * w1));
@@ -842,7 +898,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             if (row < rows) store_o(a.o + prow * D + col, o0);
           }
           if (row < rows && s == 0)
-            reinterpret_cast<float2*>(a.ml)[prow] = n > 1 ? make_float2(mm, fmaf(ml0.y, w0, ml1.y * w1)) : ml0;
+            reinterpret_cast<float2*>(a.ml)[prow] = two ? make_float2(mm, fmaf(ml0.y, w0, ml1.y * w1)) : ml0;
         }
       }
       tc_fence_before();
