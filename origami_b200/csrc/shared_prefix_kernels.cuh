@@ -91,7 +91,6 @@ struct SharedArgs {
 
 namespace spa {
 
-using attn::mma_commit;
 using attn::pack2;
 using attn::proxy_fence;
 using attn::tc_fence_after;
@@ -292,18 +291,32 @@ __device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lbo) {
   return (static_cast<uint64_t>(addr >> 4) & 0x3FFFull) | (static_cast<uint64_t>(lbo >> 4) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+// The warp that issues products runs as one, so that descriptors stay in uniform registers;
+// `lead` is 1 in the elected thread, whose products and commits these are.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t lead;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
+  return lead;
+}
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(da), "l"(db), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(ta), "l"(db), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(ta), "l"(db), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
       : "memory");
 }
 
@@ -677,64 +690,48 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         mbar_arrive(&bars->seg_full[at]);
         if (!more) break;
       }
-    } else if (warp == 12 && lane == 0) {
+    } else if (warp == 12) {
       // -------------------------------------------------------------- products
-      const uint32_t base = smem_u32(sm);
+      const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t lead = elect_one();
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort)) != 0;
+      };
+      // the copies are generic-proxy writes: the fence orders the products' reads behind them
+      auto wait_full = [&](uint32_t st) {
+        const bool full = wait(&bars->full[st % S::stages], (st / S::stages) & 1u);
+        proxy_fence();
+        return full;
+      };
       uint32_t ring = 0;  // stage index at which the segment begins
       // phases and pending products (not waited for yet) of the streams, bit s
       uint32_t p_phase = 0u, pv_phase = 0u, pending = 0u, o_phase = 0u, q_next = 0u;
       bool ok = true;
+#pragma unroll 1
       for (uint32_t slot = 0;; ++slot) {
-        if (!ok || !wait_or_abort(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u, abort)) break;
-        const int n = segs[slot % kSegments].n;
-        const bool pair = segs[slot % kSegments].pair != 0;
-        mbar_arrive(&bars->seg_empty[slot % kSegments]);
+        if (!ok || !wait(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u)) break;
+        const int n = __shfl_sync(0xffffffffu, segs[slot % kSegments].n, 0);
+        const bool pair = __shfl_sync(0xffffffffu, segs[slot % kSegments].pair, 0) != 0;
+        if (lead) mbar_arrive(&bars->seg_empty[slot % kSegments]);
         if (n == 0) break;
         const int ns0 = pair ? n : (n + 1) / 2, ns1 = pair ? n : n / 2;
         if (pair) q_next = 0;
         const uint32_t qb = q_next;
         if (!pair) q_next ^= 1u;
-        // the copies are generic-proxy writes: the fence orders the products' reads behind them
-        auto wait_full = [&](uint32_t st) {
-          const bool full = wait_or_abort(&bars->full[st % S::stages], (st / S::stages) & 1u, abort);
-          proxy_fence();
-          return full;
-        };
-        auto issue_s = [&](uint32_t s, int i) {
-          const int t = pair ? i : 2 * i + static_cast<int>(s);
-          const uint32_t st = ring + (pair ? 2 * t : t == 0 ? 0 : 2 * t - 1);
-          if (!wait_full(st)) return false;
-          // P lies in S: the product that reads it must have ended before S is written again
-          if (((pending >> s) & 1u) && !wait_or_abort(&bars->pv[s], ((pv_phase >> s) & 1u) ^ 1u, abort)) return false;
-          pending &= ~(1u << s);
-          tc_fence_after();
-          const uint64_t qd = desc128(base + (pair ? s : qb) * S::tile, 16);
-          const uint64_t kd = desc128(base + S::ring + (st % S::stages) * S::tile, 16);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-            mma_ss(tmem + 128 * s, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
-          }
-          mma_commit(&bars->s_full[s]);
-          if (!pair || s == 1) mma_commit(&bars->empty[st % S::stages]);
-          // the last product that reads a Q buffer frees it
-          if (pair ? i == n - 1 : t == n - 1) mma_commit(&bars->q_empty[pair ? s : qb]);
-          return true;
-        };
-        ok = issue_s(0, 0);
-        if (ok && ns1 > 0) ok = issue_s(1, 0);
+        // Step j of the segment: stream j & 1's product i = j >> 1. Each turn adds P V of a
+        // step, then begins S of the stream's next step; the first two turns only begin S.
 #pragma unroll 1
-        for (int i = 0; i < ns0 && ok; ++i) {
-#pragma unroll 1
-          for (uint32_t s = 0; s < 2 && ok; ++s) {
-            if (s == 1 && i >= ns1) break;
+        for (int j = -2; j < 2 * ns0 && ok; ++j) {
+          const uint32_t s = static_cast<uint32_t>(j) & 1u;
+          const int i = j >> 1, ns = s == 0 ? ns0 : ns1;
+          if (i >= 0 && i < ns) {
             const int t = pair ? i : 2 * i + static_cast<int>(s);
             const uint32_t st = ring + (pair ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1));
-            ok = wait_full(st) && wait_or_abort(&bars->p_full[s], (p_phase >> s) & 1u, abort);
+            ok = wait_full(st) && wait(&bars->p_full[s], (p_phase >> s) & 1u);
             if (!ok) break;
             p_phase ^= 1u << s;
-            if (i == 0 && s == 0 && slot > 0) {  // the last segment's O has been read
-              ok = wait_or_abort(&bars->o_free, o_phase, abort);
+            if (j == 0 && slot > 0) {  // the last segment's O has been read
+              ok = wait(&bars->o_free, o_phase);
               if (!ok) break;
               o_phase ^= 1u;
             }
@@ -742,20 +739,40 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             const uint64_t vd = desc128(base + S::ring + (st % S::stages) * S::tile, kTile * 128);
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              mma_ts(tmem + kO + 128 * s, tmem + 128 * s + kPCol + k * 8, vd + k * (2048 >> 4), kIdescO,
+              mma_ts(lead, tm + kO + 128 * s, tm + 128 * s + kPCol + k * 8, vd + k * (2048 >> 4), kIdescO,
                      (i > 0 || k > 0) ? 1u : 0u);
-            mma_commit(&bars->pv[s]);
-            if (!pair || s == 1) mma_commit(&bars->empty[st % S::stages]);
+            commit(lead, &bars->pv[s]);
+            if (!pair || s == 1) commit(lead, &bars->empty[st % S::stages]);
             pending |= 1u << s;
             pv_phase ^= 1u << s;
-            if (i + 1 < (s == 0 ? ns0 : ns1)) ok = issue_s(s, i + 1);
+          }
+          if (i + 1 < ns) {
+            const int t = pair ? i + 1 : 2 * (i + 1) + static_cast<int>(s);
+            const uint32_t st = ring + (pair ? 2 * t : t == 0 ? 0 : 2 * t - 1);
+            ok = wait_full(st);
+            // P lies in S: the product that reads it must have ended before S is written again
+            if (ok && ((pending >> s) & 1u)) ok = wait(&bars->pv[s], ((pv_phase >> s) & 1u) ^ 1u);
+            if (!ok) break;
+            pending &= ~(1u << s);
+            tc_fence_after();
+            const uint64_t qd = desc128(base + (pair ? s : qb) * S::tile, 16);
+            const uint64_t kd = desc128(base + S::ring + (st % S::stages) * S::tile, 16);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+              mma_ss(lead, tm + 128 * s, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
+            }
+            commit(lead, &bars->s_full[s]);
+            if (!pair || s == 1) commit(lead, &bars->empty[st % S::stages]);
+            // the last product that reads a Q buffer frees it
+            if (t == n - 1) commit(lead, &bars->q_empty[pair ? s : qb]);
           }
         }
         ring += 2 * n;
       }
       // nothing may be in flight when the columns are released
-      mma_commit(&bars->done);
-      wait_or_abort(&bars->done, 0u, abort);
+      commit(lead, &bars->done);
+      wait(&bars->done, 0u);
     }
     __syncwarp();
   } else {
