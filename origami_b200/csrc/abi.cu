@@ -109,6 +109,19 @@ int32_t persistent_slots(const void* fn, int smem, int& resident) {
   return ORIGAMI_OK;
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
 }  // namespace origami_host
 
 
@@ -393,19 +406,6 @@ int32_t canonical_common(bool restore, const uint8_t* d_packed, int64_t packed_b
 // ---------------------------------------------------------------------------------------
 // TMA path for the aligned plane format (see tma_kernels.cuh).
 // ---------------------------------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
-
 // True when every (kv, plane) component is a dense [H*D runs][T*bits/8] byte array in
 // canonical order with 16-byte aligned rows, and the tile boxes are 16-byte multiples.
 bool tma_eligible(int mode, const std::vector<Spec>& specs, const int64_t* off, const origami_planes* pl,

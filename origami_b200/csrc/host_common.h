@@ -5,6 +5,7 @@
 
 #include <cstdint>
 
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include "../../include/origami_b200.h"
@@ -30,5 +31,8 @@ int32_t validate_cache(const origami_paged_kv* kv, PagedGeom& g);
 // Raises the kernel's dynamic shared-memory limit to `smem` (once per kernel and device)
 // and returns the CTAs of kThreads threads resident on the whole device.
 int32_t persistent_slots(const void* fn, int smem, int& resident);
+
+// The driver's cuTensorMapEncodeTiled, null where the driver has none.
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
 }  // namespace origami_host

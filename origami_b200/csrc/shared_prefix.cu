@@ -81,13 +81,6 @@ int32_t launch(const origami::SharedArgs& a, cudaStream_t st) {
   int resident = 0;
   int32_t rc = persistent_slots(reinterpret_cast<const void*>(fn), smem, resident);  // raises the shared-memory limit
   if (rc) return rc;
-  // the kernel's warpgroups share out exactly the registers of this launch
-  static const int regs = [fn] {
-    cudaFuncAttributes at{};
-    return cudaFuncGetAttributes(&at, fn) == cudaSuccess ? at.numRegs : 0;
-  }();
-  if (regs != origami::spa::kRegsLaunch)
-    return fail(ORIGAMI_ERR_CUDA, "shared_prefix_attention was built with %d registers", regs);
   rc = launch_dependent(fn, dim3(static_cast<unsigned>(a.ctas)), origami::spa::kThreadsS, smem, st,
                         "shared_prefix_attention launch", a);
   if (rc) return rc;
@@ -203,6 +196,25 @@ int32_t origami_shared_prefix_attention(
   a.tile_tokens = origami::spa::kTile / a.group;
   a.item_rows_p = w.item_rows_p;
   a.item_rows_s = w.item_rows_s;
+  a.all_rows = static_cast<int32_t>(2 * cache->num_blocks * cache->block_size);
+  a.v_rows = static_cast<int32_t>(g.kv_stride / g.token_stride);
+  a.inv_ctas = sms > 1 ? ~0ull / static_cast<uint64_t>(sms) : ~0ull;
+  // TMA boxes of at least one swizzle atom (8 rows) that lie inside one block and one warp's 32 rows
+  a.tma_rows = 32;
+  while (a.tma_rows >= 8 && cache->block_size % a.tma_rows != 0) a.tma_rows /= 2;
+  if (a.tma_rows < 8) a.tma_rows = 0;
+  if (a.tma_rows > 0) {
+    auto encode = tensor_map_encoder();
+    if (encode == nullptr) return fail(ORIGAMI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(cache->num_heads),
+                                static_cast<cuuint64_t>(a.all_rows)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim * 2), static_cast<cuuint64_t>(g.token_stride * 2)};
+    const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(a.tma_rows)}, estr[3] = {1, 1, 1};
+    const CUresult r = encode(&a.map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, cache->d_data, dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ORIGAMI_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  }
   a.q_vec = rows_vec(query);
   a.o_vec = rows_vec(output);
   a.ctas = sms;

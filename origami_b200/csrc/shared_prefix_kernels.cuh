@@ -17,20 +17,22 @@
 // in equal contiguous shares: no tail, no atomics, a fixed order of summation. A share's piece
 // of an item (a "segment") writes one partial; merge_partials joins each row's partials.
 //
-// A CTA: 4 loader warps gather K and V tiles through the block tables with 16-byte
-// cp.async into a ring of 128-byte-swizzled tiles (any block size; rows past the end become
-// zeros, so garbage there cannot reach the products); one thread issues tcgen05.mma; two
-// softmax warpgroups own one stream each, a stream being one (S, O) accumulator pair in TMEM:
-//   S_s [128 rows x 128 keys] = Q K^T (shared memory operands),
-//   O_s [128 rows x D]       += P V   (P in TMEM over S's second half, V as the N-major B operand).
-// One thread owns one row, so the softmax needs no exchange. O is rescaled only when the
+// A CTA: 4 loader warps gather K and V tiles through the block tables into a ring of
+// 128-byte-swizzled tiles, by TMA where a block's rows come in eights (a box per block), else
+// and where a tile ends inside with 16-byte cp.async (rows past the end become zeros, so
+// garbage there cannot reach the products); one warp issues tcgen05.mma; two softmax
+// warpgroups own one stream each, a stream being, in TMEM, two score buffers of 64 keys and O:
+//   S_s [128 rows x 64 keys] = Q K^T (shared memory operands),
+//   O_s [128 rows x D]      += P V   (P over the second half of its S, V the N-major B operand).
+// The next 64 scores are ready when a softmax step ends, so a stream's chain is its softmax
+// alone. One thread owns one row: the softmax needs no exchange. O is rescaled only when the
 // maximum grew by more than 2^8 (P stays below 2^8, exact in the same relative precision).
 // With more than 128 rows an item has two row tiles, one per stream, that share each K and V
-// tile ("pair"); with fewer, the streams take alternate key tiles of one row tile and join at
-// the end of the segment ("split"). Either way one stream's softmax runs under the other's
-// products.
+// tile ("pair"); with fewer, the streams take one half of each key tile for one row tile and
+// join at the end of the segment ("split").
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -41,12 +43,9 @@ namespace origami {
 
 namespace spa {
 
-constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12: MMA
-// Registers per thread at launch, then of the softmax warpgroups and of the others:
-// 256 * 176 + 256 * 80 = 512 * 128, all that the block was launched with.
-constexpr int kRegsLaunch = 128, kRegsSoftmax = 176, kRegsOther = 80;
-static_assert(256 * (kRegsSoftmax + kRegsOther) <= kThreadsS * kRegsLaunch, "register shares");
+constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12: products; 13: scheduler
 constexpr int kTile = 128;      // keys per tile, rows per row tile
+constexpr int kHalf = 64;       // keys per softmax step
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of a segment.
 constexpr int kCostTile = 8, kCostPair = 8, kCostItem = 4;
 
@@ -63,6 +62,7 @@ struct Smem {
 }  // namespace spa
 
 struct SharedArgs {
+  CUtensorMap map;  // the cache as [token rows, heads, D], boxes of tma_rows x 1 x 64; see tma_rows
   const uint16_t* query;
   uint16_t* output;
   float* lse;
@@ -80,6 +80,9 @@ struct SharedArgs {
   int32_t q_heads, kv_heads, group, tile_tokens;  // tokens per row tile
   int32_t item_rows_p, item_rows_s;               // partial rows a CTA may need for a prefix / suffix item
   int32_t q_vec, o_vec, ctas;
+  int32_t tma_rows;   // token rows per TMA box (divides the block size), 0: no TMA
+  int32_t all_rows, v_rows;  // token rows of the cache; rows from a token's K to its V
+  uint64_t inv_ctas;  // floor(2^64 / ctas)
   float scale_log2;
   // workspace
   int64_t* head;      // {prefix cost per head, suffix cost per head}
@@ -119,11 +122,15 @@ struct Item {
   __device__ __forceinline__ int tile_at(int64_t w) const {
     const int64_t x = w - start - kCostItem;
     if (x <= 0) return 0;
-    const int64_t t = (x + tile_cost - 1) / tile_cost;
+    const int64_t t = pair ? (x + kCostPair - 1) / kCostPair : (x + kCostTile - 1) / kCostTile;
     return t > tiles() ? tiles() : static_cast<int>(t);
   }
 };
 
+// Where CTA c's share begins: monotone in c, 0 and `all` at the ends.
+__device__ __forceinline__ int64_t share_begin(const SharedArgs& a, int64_t all, int c) {
+  return c >= a.ctas ? all : static_cast<int64_t>(__umul64hi(static_cast<uint64_t>(all) * c, a.inv_ctas));
+}
 __device__ __forceinline__ int used_tokens(const SharedArgs& a) {
   return clampi(__ldg(a.query_start + a.requests), 0, a.tokens);
 }
@@ -214,10 +221,10 @@ struct Walk {
     ptok = 0;
     if (in_prefix) {
       const int per = prefix_item_tokens(a, d.used);
-      ph = static_cast<int>(d.w0 / d.wp);
-      const int64_t in_head = d.w0 - ph * d.wp;
+      int64_t in_head = d.w0;
+      for (; in_head >= d.wp; in_head -= d.wp) ++ph;
       const int64_t first = prefix_item(a, d.used, 0, 0, 0).cost();
-      const int64_t i = min64(in_head / first, (d.used + per - 1) / per - 1);
+      const int64_t i = in_head < first ? 0 : min64(in_head / first, (d.used + per - 1) / per - 1);
       ptok = i * per;
       next = ph * d.wp + i * first;
     }
@@ -266,6 +273,7 @@ struct Walk {
 struct Segment {
   int64_t prow;       // partial row of its first row
   int32_t t0, n;      // first tile, tiles; n = 0 ends the share
+  int32_t halves;     // 64-key halves of its tiles that hold keys
   int32_t pair, h, b;  // two row tiles; KV head; request, -1 for the prefix
   int32_t tok0, ntok, kend, vis0;
 };
@@ -333,11 +341,11 @@ __device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
-// 128 columns: four loads in flight, one wait. The empty statements tie every value to the
+// 64 columns: two loads in flight, one wait. The empty statements tie every value to the
 // wait, so that none is used before it.
-__device__ __forceinline__ void ld128(uint32_t addr, uint32_t (&r)[128]) {
+__device__ __forceinline__ void ld64(uint32_t addr, uint32_t (&r)[64]) {
 #pragma unroll
-  for (int c = 0; c < 128; c += 32)
+  for (int c = 0; c < 64; c += 32)
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
@@ -352,7 +360,7 @@ __device__ __forceinline__ void ld128(uint32_t addr, uint32_t (&r)[128]) {
         : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-  for (int j = 0; j < 128; ++j) asm volatile("" : "+r"(r[j]));
+  for (int j = 0; j < 64; ++j) asm volatile("" : "+r"(r[j]));
 }
 __device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
@@ -416,8 +424,42 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
   return static_cast<uint32_t>((c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// TMA: a box of the cache's token rows from row z, one head, 64 dims from x.
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// Two floats at a time.
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Barriers of products have one entry per stream and score buffer: the step that uses a buffer
+// next begins only after the last use's phase was seen, so a parity is never ambiguous.
 struct Bars {
-  uint64_t full[10], empty[10], q_empty[2], s_full[2], p_full[2], pv[2], seg_full[kSegments], seg_empty[kSegments];
+  uint64_t full[10], empty[10], q_empty[2], s_full[4], p_full[4], pv[4], seg_full[kSegments], seg_empty[kSegments];
   uint64_t o_free, xch, done;
 };
 
@@ -441,10 +483,10 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   static_assert(sizeof(Bars) + 8 + sizeof(Deal) + kSegments * sizeof(Segment) <= 1024, "scalars fit");
   static_assert(S::bytes <= 227 * 1024, "shared memory of one SM");
   constexpr bool kBf16 = attn::is_bf16<QT>();
-  constexpr uint32_t kIdescS = attn::instr_desc(kBf16, kTile);
+  constexpr uint32_t kIdescS = attn::instr_desc(kBf16, kHalf);
   constexpr uint32_t kIdescO = attn::instr_desc(kBf16, D) | (1u << 16);  // B (V) is N-major
-  constexpr uint32_t kO = 256;  // S_s at column 128 s, O_s at 256 + 128 s
-  constexpr uint32_t kPCol = 64;  // P lies over the second half of S
+  constexpr uint32_t kO = 256;  // buffer b of S_s at column 128 s + 64 b, O_s at 256 + 128 s
+  constexpr uint32_t kPCol = 32;  // P lies over the second half of its S
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = static_cast<int>(blockIdx.x);
@@ -458,11 +500,11 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       mbar_init(&bars->full[i], 4 * 32);
       mbar_init(&bars->empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->q_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->q_empty[i], 1);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->p_full[i], kTile);
       mbar_init(&bars->pv[i], 1);
+      mbar_init(&bars->p_full[i], kTile);
     }
     for (int i = 0; i < kSegments; ++i) {
       mbar_init(&bars->seg_full[i], 1);
@@ -505,10 +547,12 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     const int64_t excl = before + incl - sum;
     const int used = used_tokens(a);
     const int64_t wp = prefix_cost(a, used), all_p = wp * a.kv_heads, all = all_p + total * a.kv_heads;
-    const int64_t w0 = all * cta / a.ctas, w1 = all * (cta + 1) / a.ctas;
+    const int64_t w0 = share_begin(a, all, cta), w1 = share_begin(a, all, cta + 1);
     // the share's first suffix item: in the run of requests that holds its cost
     const int64_t y = w0 <= all_p ? 0 : w0 - all_p;
-    const int64_t fh = total > 0 ? y / total : 0, rem = y - fh * total;
+    int fh = 0;
+    int64_t rem = y;
+    for (; total > 0 && rem >= total; rem -= total) ++fh;
     if (tid == 0) {
       deal_sm->wp = wp;
       deal_sm->ws = total;
@@ -540,7 +584,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         if (rem < at + c) break;
         at += c;
       }
-      deal_sm->h = static_cast<int>(fh);
+      deal_sm->h = fh;
       deal_sm->b = b;
       deal_sm->tile = t;
       deal_sm->start = all_p + fh * total + at;
@@ -562,7 +606,6 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   if (warp >= 8 && warp < 12) {
     // ---------------------------------------------------------------- loaders
     // Warp lw fills rows 32 lw .. 32 lw + 31 of every tile; lane l knows row 32 lw + l.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
     constexpr int kChunks = D / 8;          // 16-byte chunks per row
     constexpr int kRowsPer = 32 / kChunks;  // rows a warp copies at once
     const int lw = warp - 8;
@@ -571,20 +614,33 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     const uint32_t base = smem_u32(sm);
     uint32_t ring = 0, slot = 0, q_used = 0u, q_phase = 0u, q_next = 0u;
     bool ok = true, plain_q = false;
-    // Waits until stage `ring` may be refilled, copies this warp's rows of K or V into it. The
-    // stage is full when every loader thread's copies so far have landed (Q's with the first K's).
-    auto emit = [&](int row, const uint16_t* src) {
+    // Waits until stage `ring` may be refilled, copies this warp's rows of K (which = 0) or V
+    // into it: all inside the item (`whole`) by TMA, else row by row. The stage is full when
+    // every loader thread's copies so far have landed (Q's with the first K's).
+    auto emit = [&](int row, int which, bool whole, int head) {
       const uint32_t st = ring % S::stages, use = ring / S::stages;
       if (use > 0) {
         ok = __all_sync(0xffffffffu, wait_or_abort(&bars->empty[st], (use - 1) & 1u, abort));
         if (!ok) return;
       }
       const uint32_t dst = base + S::ring + st * S::tile;
+      if (whole && a.tma_rows > 0) {
+        if (lane == 0) expect_tx(&bars->full[st], 32 * D * 2);
+        __syncwarp();
+        if ((lane & (a.tma_rows - 1)) == 0) {
+          const int z = row < 0 ? a.all_rows : row + which * a.v_rows;  // past the last row: zeros
+#pragma unroll
+          for (int x = 0; x < D; x += 64)
+            tma_rows(dst + (x >> 6) * (kTile * 128) + (32 * lw + lane) * 128, &a.map, x, head, z, &bars->full[st]);
+        }
+      } else {
+        const uint16_t* src = a.cache + which * a.kv_stride + static_cast<int64_t>(head) * D + chunk * 8;
 #pragma unroll 4
-      for (int i = 0; i < 32 / kRowsPer; ++i) {
-        const int r = i * kRowsPer + sub;
-        const int cr = __shfl_sync(0xffffffffu, row, r);
-        cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
+        for (int i = 0; i < 32 / kRowsPer; ++i) {
+          const int r = i * kRowsPer + sub;
+          const int cr = __shfl_sync(0xffffffffu, row, r);
+          cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
+        }
       }
       if (plain_q) {  // Q came through registers: an arrival that releases those stores too
         asm volatile("cp.async.wait_all;\n" ::: "memory");
@@ -611,7 +667,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         return pb < 0 || pb >= a.num_blocks ? -1 : pb * a.block_rows + (key - static_cast<int>(page) * a.block_size);
       };
       int key = seg.t0 * kTile + 32 * lw + lane;
-      int row = row_of(key), prev = -1;
+      int row = row_of(key);
       // Q: one row tile, into the buffer after the last one used, or both for a pair
       if (seg.pair) q_next = 0;
 #pragma unroll 1
@@ -651,23 +707,22 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       }
       if (!ok) break;
       plain_q = !a.q_vec;
-      // pair: K V K V ..; split: K K V K V .. V, the order in which the products first use them
-      const uint16_t* k_src = a.cache + static_cast<int64_t>(seg.h) * D + chunk * 8;
-      const uint16_t* v_src = k_src + a.kv_stride;
 #pragma unroll 1
-      for (int i = 0; i <= seg.n && ok; ++i) {
+      for (int i = 0; i < seg.n && ok; ++i) {
+        const bool whole = __all_sync(0xffffffffu, key < seg.kend);
         key += kTile;
         const int next_row = i + 1 < seg.n ? row_of(key) : -1;
-        if (i < seg.n) emit(row, k_src);
-        const bool v_now = seg.pair ? i < seg.n : i > 0;
-        if (v_now && ok) emit(seg.pair ? row : prev, v_src);
-        prev = row;
+        emit(row, 0, whole, seg.h);
+        if (ok) emit(row, 1, whole, seg.h);
         row = next_row;
       }
     }
+    // every stage was waited for by the products; after a timeout, wait (bounded) for what is in flight
+    if (*abort)
+      for (uint32_t i = ring > S::stages ? ring - S::stages : 0; i < ring; ++i)
+        mbar_wait_bounded(&bars->full[i % S::stages], (i / S::stages) & 1u, 1u << 16);
     asm volatile("cp.async.wait_all;\n" ::: "memory");
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
     if (warp == 13 && lane == 0) {
       // -------------------------------------------------------------- scheduler
       const Deal deal = *deal_sm;
@@ -679,6 +734,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         Segment& g = segs[at];
         g.n = more ? w.t1 - w.t0 : 0;
         g.t0 = w.t0;
+        g.halves = (min(w.it.kend - w.t0 * kTile, g.n * kTile) + kHalf - 1) / kHalf;
         g.pair = w.it.pair;
         g.h = w.it.h;
         g.b = w.it.b;
@@ -704,69 +760,74 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         return full;
       };
       uint32_t ring = 0;  // stage index at which the segment begins
-      // phases and pending products (not waited for yet) of the streams, bit s
-      uint32_t p_phase = 0u, pv_phase = 0u, pending = 0u, o_phase = 0u, q_next = 0u;
+      // of each stream: S products and P V products begun, the latter waited for
+      uint32_t n_s[2] = {0u, 0u}, n_pv[2] = {0u, 0u}, n_done[2] = {0u, 0u};
+      uint32_t o_phase = 0u, q_next = 0u;
       bool ok = true;
 #pragma unroll 1
       for (uint32_t slot = 0;; ++slot) {
         if (!ok || !wait(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u)) break;
         const int n = __shfl_sync(0xffffffffu, segs[slot % kSegments].n, 0);
         const bool pair = __shfl_sync(0xffffffffu, segs[slot % kSegments].pair, 0) != 0;
+        const int halves = __shfl_sync(0xffffffffu, segs[slot % kSegments].halves, 0);
         if (lead) mbar_arrive(&bars->seg_empty[slot % kSegments]);
         if (n == 0) break;
-        const int ns0 = pair ? n : (n + 1) / 2, ns1 = pair ? n : n / 2;
+        const int g0 = pair ? halves : (halves + 1) / 2, g1 = pair ? halves : halves / 2;
         if (pair) q_next = 0;
         const uint32_t qb = q_next;
         if (!pair) q_next ^= 1u;
-        // Step j of the segment: stream j & 1's product i = j >> 1. Each turn adds P V of a
-        // step, then begins S of the stream's next step; the first two turns only begin S.
-#pragma unroll 1
-        for (int j = -2; j < 2 * ns0 && ok; ++j) {
-          const uint32_t s = static_cast<uint32_t>(j) & 1u;
-          const int i = j >> 1, ns = s == 0 ? ns0 : ns1;
-          if (i >= 0 && i < ns) {
-            const int t = pair ? i : 2 * i + static_cast<int>(s);
-            const uint32_t st = ring + (pair ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1));
-            ok = wait_full(st) && wait(&bars->p_full[s], (p_phase >> s) & 1u);
-            if (!ok) break;
-            p_phase ^= 1u << s;
-            if (j == 0 && slot > 0) {  // the last segment's O has been read
-              ok = wait(&bars->o_free, o_phase);
-              if (!ok) break;
-              o_phase ^= 1u;
+        // A turn of stream s begins S of its step g + 1, then adds P V of step g. Step g is half
+        // g & 1 of tile g >> 1 (pair) or half s of tile g (split). The last product that reads a
+        // tile frees its stage.
+        auto turn = [&](auto stream, int g) {
+          constexpr uint32_t s = decltype(stream)::value;
+          const int gs = s == 0 ? g0 : g1;
+          auto last_of_tile = [&](int x) { return s == 1 ? !pair || (x & 1) || x == g1 - 1 : !pair && x >= g1; };
+          if (g + 1 < gs) {
+            const int x = g + 1;
+            const uint32_t st = ring + 2 * (pair ? x >> 1 : x), half = pair ? x & 1 : s, buf = n_s[s] & 1u;
+            if (!wait_full(st)) return false;
+            // P of two steps before lies in this S: the last product begun must have ended
+            if (n_done[s] != n_pv[s]) {
+              if (!wait(&bars->pv[2 * s + ((n_pv[s] - 1) & 1u)], ((n_pv[s] - 1) >> 1) & 1u)) return false;
+              n_done[s] = n_pv[s];
             }
             tc_fence_after();
-            const uint64_t vd = desc128(base + S::ring + (st % S::stages) * S::tile, kTile * 128);
-#pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              mma_ts(lead, tm + kO + 128 * s, tm + 128 * s + kPCol + k * 8, vd + k * (2048 >> 4), kIdescO,
-                     (i > 0 || k > 0) ? 1u : 0u);
-            commit(lead, &bars->pv[s]);
-            if (!pair || s == 1) commit(lead, &bars->empty[st % S::stages]);
-            pending |= 1u << s;
-            pv_phase ^= 1u << s;
-          }
-          if (i + 1 < ns) {
-            const int t = pair ? i + 1 : 2 * (i + 1) + static_cast<int>(s);
-            const uint32_t st = ring + (pair ? 2 * t : t == 0 ? 0 : 2 * t - 1);
-            ok = wait_full(st);
-            // P lies in S: the product that reads it must have ended before S is written again
-            if (ok && ((pending >> s) & 1u)) ok = wait(&bars->pv[s], ((pv_phase >> s) & 1u) ^ 1u);
-            if (!ok) break;
-            pending &= ~(1u << s);
-            tc_fence_after();
             const uint64_t qd = desc128(base + (pair ? s : qb) * S::tile, 16);
-            const uint64_t kd = desc128(base + S::ring + (st % S::stages) * S::tile, 16);
+            const uint64_t kd = desc128(base + S::ring + (st % S::stages) * S::tile + half * (kHalf * 128), 16);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-              mma_ss(lead, tm + 128 * s, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
+              mma_ss(lead, tm + 128 * s + 64 * buf, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
             }
-            commit(lead, &bars->s_full[s]);
-            if (!pair || s == 1) commit(lead, &bars->empty[st % S::stages]);
-            // the last product that reads a Q buffer frees it
-            if (t == n - 1) commit(lead, &bars->q_empty[pair ? s : qb]);
+            commit(lead, &bars->s_full[2 * s + buf]);
+            if (last_of_tile(x)) commit(lead, &bars->empty[st % S::stages]);
+            if (pair ? x == gs - 1 : x == g0 - 1 && last_of_tile(x)) commit(lead, &bars->q_empty[pair ? s : qb]);
+            ++n_s[s];
           }
+          if (g >= 0 && g < gs) {
+            const uint32_t st = ring + 2 * (pair ? g >> 1 : g) + 1, half = pair ? g & 1 : s, buf = n_pv[s] & 1u;
+            if (!wait_full(st) || !wait(&bars->p_full[2 * s + buf], (n_pv[s] >> 1) & 1u)) return false;
+            if (g == 0 && s == 0 && slot > 0) {  // the last segment's O has been read
+              if (!wait(&bars->o_free, o_phase)) return false;
+              o_phase ^= 1u;
+            }
+            tc_fence_after();
+            const uint64_t vd = desc128(base + S::ring + (st % S::stages) * S::tile + half * (kHalf * 128), kTile * 128);
+#pragma unroll
+            for (int k = 0; k < kHalf / 16; ++k)
+              mma_ts(lead, tm + kO + 128 * s, tm + 128 * s + 64 * buf + kPCol + k * 8, vd + k * (2048 >> 4), kIdescO,
+                     (g > 0 || k > 0) ? 1u : 0u);
+            commit(lead, &bars->pv[2 * s + buf]);
+            if (last_of_tile(g)) commit(lead, &bars->empty[st % S::stages]);
+            ++n_pv[s];
+          }
+          return true;
+        };
+#pragma unroll 1
+        for (int g = -1; g < g0 && ok; ++g) {
+          ok = turn(std::integral_constant<uint32_t, 0>{}, g);
+          if (ok) ok = turn(std::integral_constant<uint32_t, 1>{}, g);
         }
         ring += 2 * n;
       }
@@ -777,13 +838,12 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax of stream s
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax));
     const int s = warp >> 2;
     const int row = tid & (kTile - 1);
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t ts = lane_base + 128 * s, to = lane_base + kO + 128 * s;
     const int token_in_tile = row / a.group;
-    uint32_t s_phase = 0u, pv_phase = 0u, x_phase = 0u;
+    uint32_t count = 0u, x_phase = 0u;  // steps so far
     bool ok = true;
     for (uint32_t slot = 0;; ++slot) {
       ok = ok && __all_sync(0xffffffffu, wait_or_abort(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u, abort));
@@ -793,32 +853,32 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       if (lane == 0) mbar_arrive(&bars->seg_empty[slot % kSegments]);
       if (seg.n == 0) break;
       const bool pair = seg.pair != 0;
-      const int steps = pair ? seg.n : s == 0 ? (seg.n + 1) / 2 : seg.n / 2;
+      const int steps = pair ? seg.halves : s == 0 ? (seg.halves + 1) / 2 : seg.halves / 2;
       const int first_tok = pair ? s * a.tile_tokens : 0;
       const int rows = min(a.tile_tokens, seg.ntok - first_tok) * a.group;
       const bool warp_live = (warp & 3) * 32 < rows;
-      // keys of the item this row sees, less those before the current tile
+      // keys of the item this row sees, less those before the current step's
       int lim = 0;
       if (row < rows) lim = seg.b < 0 ? seg.kend : clampi(static_cast<int64_t>(seg.vis0) + token_in_tile, 0, seg.kend);
-      lim -= (seg.t0 + (pair ? 0 : s)) * kTile;
+      lim -= seg.t0 * kTile + (pair ? 0 : s * kHalf);
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int i = 0; i < steps; ++i) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->s_full[s], s_phase, abort));
+        const uint32_t buf = count & 1u;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->s_full[2 * s + buf], (count >> 1) & 1u, abort));
         if (!ok) break;
-        s_phase ^= 1u;
         tc_fence_after();
         if (warp_live) {
-          uint32_t x[128];  // P goes over the second half of S, so all of S is read first
-          ld128(ts, x);
-          if (!__all_sync(0xffffffffu, lim >= kTile || row >= rows)) {
+          uint32_t x[kHalf];  // P goes over the second half of S, so all of S is read first
+          ld64(ts + 64 * buf, x);
+          if (!__all_sync(0xffffffffu, lim >= kHalf || row >= rows)) {
 #pragma unroll
-            for (int j = 0; j < kTile; ++j)
+            for (int j = 0; j < kHalf; ++j)
               if (j >= lim) x[j] = 0xFF800000u;  // -inf: not seen
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < kTile; j += 8) {
+          for (int j = 0; j < kHalf; j += 8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(x[j + 2 * k]), __uint_as_float(x[j + 2 * k + 1])));
@@ -827,7 +887,11 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           const bool grow = mt > m + 8.f || (m == -INFINITY && mt > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
             const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mt)) : 1.f;
-            if (i > 0) {
+            if (i > 0) {  // O is at rest once the product of the step before has ended
+              const uint32_t last = count - 1;
+              ok = __all_sync(0xffffffffu, wait_or_abort(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort));
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D; c += 16) {
                 uint32_t o[16];
@@ -841,37 +905,41 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             m = grow ? mt : m;
           }
           const float neg = m == -INFINITY ? 0.f : -m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), neg2 = pair2(neg, neg);
+          uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             uint32_t p[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float p0 = ex2(fmaf(__uint_as_float(x[32 * q + 2 * j]), a.scale_log2, neg));
-              const float p1 = ex2(fmaf(__uint_as_float(x[32 * q + 2 * j + 1]), a.scale_log2, neg));
-              sum[j & 1] += p0;
-              sum[2 + (j & 1)] += p1;
+              float p0, p1;
+              split2(fma2(pair2(__uint_as_float(x[32 * q + 2 * j]), __uint_as_float(x[32 * q + 2 * j + 1])), scale2, neg2),
+                     p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              sum[j & 3] = add2(sum[j & 3], pair2(p0, p1));
               p[j] = pack2<QT>(p0, p1);
             }
-            st16(ts + kPCol + 16 * q, p);
+            st16(ts + 64 * buf + kPCol + 16 * q, p);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float l0, l1;
+          split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
+          l += l0 + l1;
           st_wait();
         }
         tc_fence_before();
-        mbar_arrive(&bars->p_full[s]);
-        lim -= pair ? kTile : 2 * kTile;
+        mbar_arrive(&bars->p_full[2 * s + buf]);
+        lim -= pair ? kHalf : kTile;
+        ++count;
       }
       if (!ok) break;
       // ------------------------------------------------------------ the segment's partial
       // scores that are all NaN leave no maximum: any reference carries their NaN on
       if (l != l && m == -INFINITY) m = 0.f;
       if (steps > 0) {
-        // one phase per step: the last one's parity
-        pv_phase ^= static_cast<uint32_t>(steps - 1) & 1u;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->pv[s], pv_phase, abort));
+        const uint32_t last = count - 1;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort));
         if (!ok) break;
-        pv_phase ^= 1u;
       }
       if (!pair) {
         // Both streams' sums belong to the same rows: exchange (m, l), then each stream joins
@@ -897,7 +965,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           }
           if (row < rows) reinterpret_cast<float2*>(a.ml)[prow] = make_float2(m, l);
         } else {
-          const bool two = seg.n > 1;
+          const bool two = seg.halves > 1;
           const float2 ml0 = ml_sm[row], ml1 = two ? ml_sm[kTile + row] : make_float2(-INFINITY, 0.f);
           const float mm = fmaxf(ml0.x, ml1.x);
           const float w0 = ml0.x == -INFINITY ? 0.f : ex2(ml0.x - mm), w1 = ml1.x == -INFINITY ? 0.f : ex2(ml1.x - mm);
@@ -977,13 +1045,13 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
     const Item& it = its[k];
     if (it.kend <= 0) continue;
     // shares that can hold a tile of the item
-    int c0 = static_cast<int>(it.start * a.ctas / all), c1 = static_cast<int>((it.start + it.cost()) * a.ctas / all);
-    c0 = max(c0 - 1, 0);
-    c1 = min(c1 + 1, a.ctas - 1);
+    const float per = static_cast<float>(a.ctas) / static_cast<float>(all);  // off by less than one share
+    const int c0 = max(static_cast<int>(static_cast<float>(it.start) * per) - 2, 0);
+    const int c1 = min(static_cast<int>(static_cast<float>(it.start + it.cost()) * per) + 2, a.ctas - 1);
     for (int cb = c0; cb <= c1; cb += 32) {
       const int c = cb + lane;
       float2 ml = make_float2(-INFINITY, 0.f);
-      if (c <= c1 && it.tile_at(all * (c + 1) / a.ctas) > it.tile_at(all * c / a.ctas))
+      if (c <= c1 && it.tile_at(share_begin(a, all, c + 1)) > it.tile_at(share_begin(a, all, c)))
         ml = __ldcg(reinterpret_cast<const float2*>(a.ml) + partial_base(a, it, c) + (t - it.tok0) * a.group + g);
       float mx = ml.x;
 #pragma unroll
