@@ -54,6 +54,7 @@ template <int D>
 struct Smem {
   static constexpr int tile = kTile * D * 2;
   static constexpr int stages = D == 128 ? 5 : 10;
+  static constexpr int lag = 2;  // stages of a warp's own copies in flight before the oldest is signalled
   static constexpr int ring = 2 * tile;
   static constexpr int scalars = ring + stages * tile;
   static constexpr int bytes = scalars + 2 * kTile * 8 + 1024;
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   }
   if (tid == 0) {
     for (int i = 0; i < S::stages; ++i) {
-      mbar_init(&bars->full[i], 4 * 32);
+      mbar_init(&bars->full[i], 4);
       mbar_init(&bars->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&bars->q_empty[i], 1);
@@ -612,19 +613,43 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     const int sub = lane / kChunks, chunk = lane % kChunks;
     // this lane's chunk of row 32 lw + sub; kRowsPer rows on, the row's swizzle changes
     const uint32_t base = smem_u32(sm);
-    uint32_t ring = 0, slot = 0, q_used = 0u, q_phase = 0u, q_next = 0u;
-    bool ok = true, plain_q = false;
+    uint32_t ring = 0, signalled = 0;  // stages begun, stages whose arrival this warp has made
+    uint32_t slot = 0, q_used = 0u, q_phase = 0u, q_next = 0u;
+    bool ok = true, q_pending = false;
+    // Copies of this warp's own threads are generic-proxy writes: the fence that orders the
+    // products' reads behind them is made here, once they have landed (in the products' warp it
+    // would wait for the products under way). TMA stages need none and arrive at once unless an
+    // older stage is still to be signalled.
+    auto signal = [&](uint32_t upto) {
+      if (signalled == upto) return;
+      proxy_fence();
+      __syncwarp();
+      if (lane == 0)
+        for (uint32_t i = signalled; i < upto; ++i) mbar_arrive(&bars->full[i % S::stages]);
+      signalled = upto;
+    };
+    auto drain = [&]() {
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
+      signal(ring);
+    };
+    // Waits with nothing unsignalled behind: whoever makes the arrival may need it.
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, 1))) return true;
+      drain();
+      return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort)) != 0;
+    };
     // Waits until stage `ring` may be refilled, copies this warp's rows of K (which = 0) or V
     // into it: all inside the item (`whole`) by TMA, else row by row. The stage is full when
-    // every loader thread's copies so far have landed (Q's with the first K's).
+    // every loader warp's rows have landed (Q's with the first K's).
     auto emit = [&](int row, int which, bool whole, int head) {
       const uint32_t st = ring % S::stages, use = ring / S::stages;
       if (use > 0) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->empty[st], (use - 1) & 1u, abort));
+        ok = wait(&bars->empty[st], (use - 1) & 1u);
         if (!ok) return;
       }
       const uint32_t dst = base + S::ring + st * S::tile;
-      if (whole && a.tma_rows > 0) {
+      const bool tma = whole && a.tma_rows > 0;
+      if (tma) {
         if (lane == 0) expect_tx(&bars->full[st], 32 * D * 2);
         __syncwarp();
         if ((lane & (a.tma_rows - 1)) == 0) {
@@ -633,6 +658,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           for (int x = 0; x < D; x += 64)
             tma_rows(dst + (x >> 6) * (kTile * 128) + (32 * lw + lane) * 128, &a.map, x, head, z, &bars->full[st]);
         }
+        __syncwarp();
       } else {
         const uint16_t* src = a.cache + which * a.kv_stride + static_cast<int64_t>(head) * D + chunk * 8;
 #pragma unroll 4
@@ -642,17 +668,19 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
         }
       }
-      if (plain_q) {  // Q came through registers: an arrival that releases those stores too
-        asm volatile("cp.async.wait_all;\n" ::: "memory");
-        mbar_arrive(&bars->full[st]);
-        plain_q = false;
-      } else {
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&bars->full[st])) : "memory");
-      }
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
       ++ring;
+      if (tma && !q_pending && signalled + 1 == ring) {
+        if (lane == 0) mbar_arrive(&bars->full[st]);
+        signalled = ring;
+      } else if (ring - signalled > S::lag) {
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(S::lag) : "memory");
+        signal(ring - S::lag);
+      }
+      q_pending = false;
     };
     for (;; ++slot) {
-      ok = ok && __all_sync(0xffffffffu, wait_or_abort(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u, abort));
+      ok = ok && wait(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u);
       if (!ok) break;
       const Segment seg = segs[slot % kSegments];
       __syncwarp();
@@ -675,7 +703,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         const uint32_t buf = q_next;
         q_next ^= 1u;
         if ((q_used >> buf) & 1u) {
-          ok = __all_sync(0xffffffffu, wait_or_abort(&bars->q_empty[buf], (q_phase >> buf) & 1u, abort));
+          ok = wait(&bars->q_empty[buf], (q_phase >> buf) & 1u);
           if (!ok) break;
           q_phase ^= 1u << buf;
         }
@@ -706,7 +734,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         }
       }
       if (!ok) break;
-      plain_q = !a.q_vec;
+      q_pending = true;
 #pragma unroll 1
       for (int i = 0; i < seg.n && ok; ++i) {
         const bool whole = __all_sync(0xffffffffu, key < seg.kend);
@@ -717,11 +745,11 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         row = next_row;
       }
     }
+    drain();
     // every stage was waited for by the products; after a timeout, wait (bounded) for what is in flight
     if (*abort)
       for (uint32_t i = ring > S::stages ? ring - S::stages : 0; i < ring; ++i)
         mbar_wait_bounded(&bars->full[i % S::stages], (i / S::stages) & 1u, 1u << 16);
-    asm volatile("cp.async.wait_all;\n" ::: "memory");
   } else if (warp >= 12) {
     if (warp == 13 && lane == 0) {
       // -------------------------------------------------------------- scheduler
@@ -753,12 +781,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort)) != 0;
       };
-      // the copies are generic-proxy writes: the fence orders the products' reads behind them
-      auto wait_full = [&](uint32_t st) {
-        const bool full = wait(&bars->full[st % S::stages], (st / S::stages) & 1u);
-        proxy_fence();
-        return full;
-      };
+      auto wait_full = [&](uint32_t st) { return wait(&bars->full[st % S::stages], (st / S::stages) & 1u); };
       uint32_t ring = 0;  // stage index at which the segment begins
       // of each stream: S products and P V products begun, the latter waited for
       uint32_t n_s[2] = {0u, 0u}, n_pv[2] = {0u, 0u}, n_done[2] = {0u, 0u};
