@@ -387,24 +387,39 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Bounded wait that gives up early when another role has: 2 s, far beyond any copy or product.
+// A warp's bounded wait, agreed by its lanes, that gives up early when another role has: 2 s,
+// far beyond any copy or product. The ready barrier costs one poll and one vote.
 constexpr uint64_t kWaitNs = 2000000000ull;
 __device__ __forceinline__ uint64_t now_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
   return t;
 }
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (mbar_wait_bounded(bar, parity, 64)) return true;
+__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __all_sync(0xffffffffu, done != 0) != 0;
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (poll(bar, parity)) return true;
   const uint64_t begin = now_ns();
-  while (!mbar_wait_bounded(bar, parity, 64)) {
-    if (*abort) return false;
-    if (now_ns() - begin > kWaitNs) {
+  for (uint32_t i = 1;; ++i) {
+    if (poll(bar, parity)) return true;
+    if ((i & 63u) == 0 && __any_sync(0xffffffffu, *abort != 0 || now_ns() - begin > kWaitNs)) {
       *abort = 1;
       return false;
     }
   }
-  return true;
+}
+
+// One arrival for a warp (arrivals of single lanes on one barrier would queue up).
+__device__ __forceinline__ void arrive_warp(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // Copy of 16 bytes, or 16 zero bytes where `valid` is false (the source is then not read).
@@ -505,14 +520,14 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     for (int i = 0; i < 4; ++i) {
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->pv[i], 1);
-      mbar_init(&bars->p_full[i], kTile);
+      mbar_init(&bars->p_full[i], 4);
     }
     for (int i = 0; i < kSegments; ++i) {
       mbar_init(&bars->seg_full[i], 1);
       mbar_init(&bars->seg_empty[i], 8 + 4 + 1);  // softmax and loader warps, the products' thread
     }
-    mbar_init(&bars->o_free, 2 * kTile);
-    mbar_init(&bars->xch, 2 * kTile);
+    mbar_init(&bars->o_free, 8);
+    mbar_init(&bars->xch, 8);
     mbar_init(&bars->done, 1);
     *abort_sm = 0;
     fence_mbar_init();
@@ -634,9 +649,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     };
     // Waits with nothing unsignalled behind: whoever makes the arrival may need it.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, 1))) return true;
+      if (poll(bar, parity)) return true;
       drain();
-      return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort)) != 0;
+      return wait_warp(bar, parity, abort);
     };
     // Waits until stage `ring` may be refilled, copies this warp's rows of K (which = 0) or V
     // into it: all inside the item (`whole`) by TMA, else row by row. The stage is full when
@@ -751,14 +766,15 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       for (uint32_t i = ring > S::stages ? ring - S::stages : 0; i < ring; ++i)
         mbar_wait_bounded(&bars->full[i % S::stages], (i / S::stages) & 1u, 1u << 16);
   } else if (warp >= 12) {
-    if (warp == 13 && lane == 0) {
+    if (warp == 13) {
       // -------------------------------------------------------------- scheduler
       const Deal deal = *deal_sm;
       Walk w(a, deal);
       for (uint32_t slot = 0;; ++slot) {
         const uint32_t at = slot % kSegments, use = slot / kSegments;
         const bool more = w.step();
-        if (use > 0 && !wait_or_abort(&bars->seg_empty[at], (use - 1) & 1u, abort)) break;
+        if (use > 0 && !wait_warp(&bars->seg_empty[at], (use - 1) & 1u, abort)) break;
+        if (lane == 0) {
         Segment& g = segs[at];
         g.n = more ? w.t1 - w.t0 : 0;
         g.t0 = w.t0;
@@ -772,17 +788,16 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         g.vis0 = w.it.vis0;
         g.prow = more ? partial_base(a, w.it, cta) : 0;
         mbar_arrive(&bars->seg_full[at]);
+        }
         if (!more) break;
       }
     } else if (warp == 12) {
       // -------------------------------------------------------------- products
       const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t lead = elect_one();
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort)) != 0;
-      };
-      auto wait_full = [&](uint32_t st) { return wait(&bars->full[st % S::stages], (st / S::stages) & 1u); };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_warp(bar, parity, abort); };
       uint32_t ring = 0;  // stage index at which the segment begins
+      uint32_t k_stage = 0u, v_stage = 0u;  // stages of the tiles in use by S and by P V
       // of each stream: S products and P V products begun, the latter waited for
       uint32_t n_s[2] = {0u, 0u}, n_pv[2] = {0u, 0u}, n_done[2] = {0u, 0u};
       uint32_t o_phase = 0u, q_next = 0u;
@@ -808,8 +823,12 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           auto last_of_tile = [&](int x) { return s == 1 ? !pair || (x & 1) || x == g1 - 1 : !pair && x >= g1; };
           if (g + 1 < gs) {
             const int x = g + 1;
-            const uint32_t st = ring + 2 * (pair ? x >> 1 : x), half = pair ? x & 1 : s, buf = n_s[s] & 1u;
-            if (!wait_full(st)) return false;
+            const uint32_t half = pair ? x & 1 : s, buf = n_s[s] & 1u;
+            if (s == 0 && (!pair || half == 0)) {  // stream 1 follows in the same tile
+              const uint32_t at = ring + 2 * (pair ? x >> 1 : x);
+              k_stage = at % S::stages;
+              if (!wait(&bars->full[k_stage], (at / S::stages) & 1u)) return false;
+            }
             // P of two steps before lies in this S: the last product begun must have ended
             if (n_done[s] != n_pv[s]) {
               if (!wait(&bars->pv[2 * s + ((n_pv[s] - 1) & 1u)], ((n_pv[s] - 1) >> 1) & 1u)) return false;
@@ -817,32 +836,37 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             }
             tc_fence_after();
             const uint64_t qd = desc128(base + (pair ? s : qb) * S::tile, 16);
-            const uint64_t kd = desc128(base + S::ring + (st % S::stages) * S::tile + half * (kHalf * 128), 16);
+            const uint64_t kd = desc128(base + S::ring + k_stage * S::tile + half * (kHalf * 128), 16);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
               mma_ss(lead, tm + 128 * s + 64 * buf, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
             }
             commit(lead, &bars->s_full[2 * s + buf]);
-            if (last_of_tile(x)) commit(lead, &bars->empty[st % S::stages]);
+            if (last_of_tile(x)) commit(lead, &bars->empty[k_stage]);
             if (pair ? x == gs - 1 : x == g0 - 1 && last_of_tile(x)) commit(lead, &bars->q_empty[pair ? s : qb]);
             ++n_s[s];
           }
           if (g >= 0 && g < gs) {
-            const uint32_t st = ring + 2 * (pair ? g >> 1 : g) + 1, half = pair ? g & 1 : s, buf = n_pv[s] & 1u;
-            if (!wait_full(st) || !wait(&bars->p_full[2 * s + buf], (n_pv[s] >> 1) & 1u)) return false;
+            const uint32_t half = pair ? g & 1 : s, buf = n_pv[s] & 1u;
+            if (s == 0 && (!pair || half == 0)) {
+              const uint32_t at = ring + 2 * (pair ? g >> 1 : g) + 1;
+              v_stage = at % S::stages;
+              if (!wait(&bars->full[v_stage], (at / S::stages) & 1u)) return false;
+            }
+            if (!wait(&bars->p_full[2 * s + buf], (n_pv[s] >> 1) & 1u)) return false;
             if (g == 0 && s == 0 && slot > 0) {  // the last segment's O has been read
               if (!wait(&bars->o_free, o_phase)) return false;
               o_phase ^= 1u;
             }
             tc_fence_after();
-            const uint64_t vd = desc128(base + S::ring + (st % S::stages) * S::tile + half * (kHalf * 128), kTile * 128);
+            const uint64_t vd = desc128(base + S::ring + v_stage * S::tile + half * (kHalf * 128), kTile * 128);
 #pragma unroll
             for (int k = 0; k < kHalf / 16; ++k)
               mma_ts(lead, tm + kO + 128 * s, tm + 128 * s + 64 * buf + kPCol + k * 8, vd + k * (2048 >> 4), kIdescO,
                      (g > 0 || k > 0) ? 1u : 0u);
             commit(lead, &bars->pv[2 * s + buf]);
-            if (last_of_tile(g)) commit(lead, &bars->empty[st % S::stages]);
+            if (last_of_tile(g)) commit(lead, &bars->empty[v_stage]);
             ++n_pv[s];
           }
           return true;
@@ -869,7 +893,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     uint32_t count = 0u, x_phase = 0u;  // steps so far
     bool ok = true;
     for (uint32_t slot = 0;; ++slot) {
-      ok = ok && __all_sync(0xffffffffu, wait_or_abort(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u, abort));
+      ok = ok && wait_warp(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u, abort);
       if (!ok) break;
       const Segment seg = segs[slot % kSegments];
       __syncwarp();
@@ -888,7 +912,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
 #pragma unroll 1
       for (int i = 0; i < steps; ++i) {
         const uint32_t buf = count & 1u;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->s_full[2 * s + buf], (count >> 1) & 1u, abort));
+        ok = wait_warp(&bars->s_full[2 * s + buf], (count >> 1) & 1u, abort);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
@@ -912,7 +936,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mt)) : 1.f;
             if (i > 0) {  // O is at rest once the product of the step before has ended
               const uint32_t last = count - 1;
-              ok = __all_sync(0xffffffffu, wait_or_abort(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort));
+              ok = wait_warp(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
@@ -951,7 +975,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           st_wait();
         }
         tc_fence_before();
-        mbar_arrive(&bars->p_full[2 * s + buf]);
+        arrive_warp(&bars->p_full[2 * s + buf]);
         lim -= pair ? kHalf : kTile;
         ++count;
       }
@@ -961,7 +985,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       if (l != l && m == -INFINITY) m = 0.f;
       if (steps > 0) {
         const uint32_t last = count - 1;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort));
+        ok = wait_warp(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort);
         if (!ok) break;
       }
       if (!pair) {
@@ -971,8 +995,8 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         // before this segment's first product could begin.
         if (steps > 0) ml_sm[s * kTile + row] = make_float2(m, l);
         tc_fence_before();
-        mbar_arrive(&bars->xch);
-        ok = __all_sync(0xffffffffu, wait_or_abort(&bars->xch, x_phase, abort));
+        arrive_warp(&bars->xch);
+        ok = wait_warp(&bars->xch, x_phase, abort);
         if (!ok) break;
         x_phase ^= 1u;
       }
@@ -1010,7 +1034,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         }
       }
       tc_fence_before();
-      mbar_arrive(&bars->o_free);
+      arrive_warp(&bars->o_free);
     }
   }
   tc_fence_before();
