@@ -20,7 +20,7 @@
 // A CTA: 4 loader warps gather K and V tiles through the block tables into a ring of
 // 128-byte-swizzled tiles, by TMA where a block's rows come in eights (a box per block), else
 // and where a tile ends inside with 16-byte cp.async (rows past the end become zeros, so
-// garbage there cannot reach the products); one warp issues tcgen05.mma; two softmax
+// garbage there cannot reach the products); one warp per stream issues its tcgen05.mma; two softmax
 // warpgroups own one stream each, a stream being, in TMEM, two score buffers of 64 keys and O:
 //   S_s [128 rows x 64 keys] = Q K^T (shared memory operands),
 //   O_s [128 rows x D]      += P V   (P over the second half of its S, V the N-major B operand).
@@ -43,7 +43,8 @@ namespace origami {
 
 namespace spa {
 
-constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12: products; 13: scheduler
+constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12 / 14: products of
+                                // stream 0 / 1; 13: scheduler
 constexpr int kTile = 128;      // keys per tile, rows per row tile
 constexpr int kHalf = 64;       // keys per softmax step
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of a segment.
@@ -514,9 +515,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   if (tid == 0) {
     for (int i = 0; i < S::stages; ++i) {
       mbar_init(&bars->full[i], 4);
-      mbar_init(&bars->empty[i], 1);
+      mbar_init(&bars->empty[i], 2);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&bars->q_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->q_empty[i], 2);
     for (int i = 0; i < 4; ++i) {
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->pv[i], 1);
@@ -524,11 +525,11 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     }
     for (int i = 0; i < kSegments; ++i) {
       mbar_init(&bars->seg_full[i], 1);
-      mbar_init(&bars->seg_empty[i], 8 + 4 + 1);  // softmax and loader warps, the products' thread
+      mbar_init(&bars->seg_empty[i], 8 + 4 + 2);  // softmax, loader and product warps
     }
     mbar_init(&bars->o_free, 8);
     mbar_init(&bars->xch, 8);
-    mbar_init(&bars->done, 1);
+    mbar_init(&bars->done, 2);
     *abort_sm = 0;
     fence_mbar_init();
   }
@@ -775,32 +776,38 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         const bool more = w.step();
         if (use > 0 && !wait_warp(&bars->seg_empty[at], (use - 1) & 1u, abort)) break;
         if (lane == 0) {
-        Segment& g = segs[at];
-        g.n = more ? w.t1 - w.t0 : 0;
-        g.t0 = w.t0;
-        g.halves = (min(w.it.kend - w.t0 * kTile, g.n * kTile) + kHalf - 1) / kHalf;
-        g.pair = w.it.pair;
-        g.h = w.it.h;
-        g.b = w.it.b;
-        g.tok0 = static_cast<int32_t>(w.it.tok0);
-        g.ntok = w.it.ntok;
-        g.kend = w.it.kend;
-        g.vis0 = w.it.vis0;
-        g.prow = more ? partial_base(a, w.it, cta) : 0;
-        mbar_arrive(&bars->seg_full[at]);
+          Segment& g = segs[at];
+          g.n = more ? w.t1 - w.t0 : 0;
+          g.t0 = w.t0;
+          g.halves = (min(w.it.kend - w.t0 * kTile, g.n * kTile) + kHalf - 1) / kHalf;
+          g.pair = w.it.pair;
+          g.h = w.it.h;
+          g.b = w.it.b;
+          g.tok0 = static_cast<int32_t>(w.it.tok0);
+          g.ntok = w.it.ntok;
+          g.kend = w.it.kend;
+          g.vis0 = w.it.vis0;
+          g.prow = more ? partial_base(a, w.it, cta) : 0;
+          mbar_arrive(&bars->seg_full[at]);
         }
         if (!more) break;
       }
-    } else if (warp == 12) {
-      // -------------------------------------------------------------- products
+    } else if (warp == 12 || warp == 14) {
+      // -------------------------------------------------------------- products of stream s
+      const uint32_t s = warp == 12 ? 0u : 1u;
       const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t lead = elect_one();
       auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_warp(bar, parity, abort); };
-      uint32_t ring = 0;  // stage index at which the segment begins
-      uint32_t k_stage = 0u, v_stage = 0u;  // stages of the tiles in use by S and by P V
-      // of each stream: S products and P V products begun, the latter waited for
-      uint32_t n_s[2] = {0u, 0u}, n_pv[2] = {0u, 0u}, n_done[2] = {0u, 0u};
-      uint32_t o_phase = 0u, q_next = 0u;
+      // stages and phases of the tiles that S and P V use next (K and V alternate in the ring)
+      uint32_t k_stage = 0u, k_phase = 0u, v_stage = 1u, v_phase = 0u;
+      auto next_tile = [](uint32_t& stage, uint32_t& phase) {
+        stage += 2;
+        if (stage >= S::stages) {
+          stage -= S::stages;
+          phase ^= 1u;
+        }
+      };
+      uint32_t n_s = 0u, n_pv = 0u, q_next = 0u;  // S and P V products begun
       bool ok = true;
 #pragma unroll 1
       for (uint32_t slot = 0;; ++slot) {
@@ -810,73 +817,84 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         const int halves = __shfl_sync(0xffffffffu, segs[slot % kSegments].halves, 0);
         if (lead) mbar_arrive(&bars->seg_empty[slot % kSegments]);
         if (n == 0) break;
-        const int g0 = pair ? halves : (halves + 1) / 2, g1 = pair ? halves : halves / 2;
         if (pair) q_next = 0;
-        const uint32_t qb = q_next;
+        const uint32_t qb = pair ? s : q_next;
         if (!pair) q_next ^= 1u;
-        // A turn of stream s begins S of its step g + 1, then adds P V of step g. Step g is half
-        // g & 1 of tile g >> 1 (pair) or half s of tile g (split). The last product that reads a
-        // tile frees its stage.
-        auto turn = [&](auto stream, int g) {
-          constexpr uint32_t s = decltype(stream)::value;
-          const int gs = s == 0 ? g0 : g1;
-          auto last_of_tile = [&](int x) { return s == 1 ? !pair || (x & 1) || x == g1 - 1 : !pair && x >= g1; };
-          if (g + 1 < gs) {
+        // Step g of the stream is half g & 1 of tile g >> 1 (pair) or half s of tile g (split).
+        const int steps = pair ? halves : (halves + 1 - static_cast<int>(s)) / 2;
+        const int odd = pair ? 1 : 0;  // a tile's first step has (g & odd) == 0, its last odd, or ends the segment
+        const uint32_t half0 = pair ? 0u : s * (kHalf * 128);
+        const uint64_t qd = desc128(base + qb * S::tile, 16);
+        // both streams free a Q buffer, for the other one too where it does not read it
+        auto free_q = [&]() {
+          commit(lead, &bars->q_empty[qb]);
+          if (pair) commit(lead, &bars->q_empty[qb]);
+        };
+        // S of step g + 1 is begun before P V of step g
+#pragma unroll 1
+        for (int g = -1; g < steps; ++g) {
+          if (g + 1 < steps) {
             const int x = g + 1;
-            const uint32_t half = pair ? x & 1 : s, buf = n_s[s] & 1u;
-            if (s == 0 && (!pair || half == 0)) {  // stream 1 follows in the same tile
-              const uint32_t at = ring + 2 * (pair ? x >> 1 : x);
-              k_stage = at % S::stages;
-              if (!wait(&bars->full[k_stage], (at / S::stages) & 1u)) return false;
+            if ((x & odd) == 0 && !wait(&bars->full[k_stage], k_phase)) {
+              ok = false;
+              break;
             }
             // P of two steps before lies in this S: the last product begun must have ended
-            if (n_done[s] != n_pv[s]) {
-              if (!wait(&bars->pv[2 * s + ((n_pv[s] - 1) & 1u)], ((n_pv[s] - 1) >> 1) & 1u)) return false;
-              n_done[s] = n_pv[s];
+            if (n_pv > 0 && !wait(&bars->pv[2 * s + ((n_pv - 1) & 1u)], ((n_pv - 1) >> 1) & 1u)) {
+              ok = false;
+              break;
             }
             tc_fence_after();
-            const uint64_t qd = desc128(base + (pair ? s : qb) * S::tile, 16);
-            const uint64_t kd = desc128(base + S::ring + k_stage * S::tile + half * (kHalf * 128), 16);
+            const uint32_t d = tm + 128 * s + 64 * (n_s & 1u);
+            const uint64_t kd = desc128(base + S::ring + k_stage * S::tile + half0 + (x & odd) * (kHalf * 128), 16);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-              mma_ss(lead, tm + 128 * s + 64 * buf, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
+              mma_ss(lead, d, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
             }
-            commit(lead, &bars->s_full[2 * s + buf]);
-            if (last_of_tile(x)) commit(lead, &bars->empty[k_stage]);
-            if (pair ? x == gs - 1 : x == g0 - 1 && last_of_tile(x)) commit(lead, &bars->q_empty[pair ? s : qb]);
-            ++n_s[s];
+            commit(lead, &bars->s_full[2 * s + (n_s & 1u)]);
+            ++n_s;
+            if ((x & odd) == odd || x == steps - 1) {
+              commit(lead, &bars->empty[k_stage]);
+              next_tile(k_stage, k_phase);
+            }
+            if (x == steps - 1) free_q();
           }
-          if (g >= 0 && g < gs) {
-            const uint32_t half = pair ? g & 1 : s, buf = n_pv[s] & 1u;
-            if (s == 0 && (!pair || half == 0)) {
-              const uint32_t at = ring + 2 * (pair ? g >> 1 : g) + 1;
-              v_stage = at % S::stages;
-              if (!wait(&bars->full[v_stage], (at / S::stages) & 1u)) return false;
+          if (g >= 0) {
+            if ((g & odd) == 0 && !wait(&bars->full[v_stage], v_phase)) {
+              ok = false;
+              break;
             }
-            if (!wait(&bars->p_full[2 * s + buf], (n_pv[s] >> 1) & 1u)) return false;
-            if (g == 0 && s == 0 && slot > 0) {  // the last segment's O has been read
-              if (!wait(&bars->o_free, o_phase)) return false;
-              o_phase ^= 1u;
+            if (!wait(&bars->p_full[2 * s + (n_pv & 1u)], (n_pv >> 1) & 1u) ||
+                (g == 0 && slot > 0 && !wait(&bars->o_free, (slot - 1) & 1u))) {  // the last segment's O has been read
+              ok = false;
+              break;
             }
             tc_fence_after();
-            const uint64_t vd = desc128(base + S::ring + v_stage * S::tile + half * (kHalf * 128), kTile * 128);
+            const uint32_t d = tm + kO + 128 * s, p = tm + 128 * s + 64 * (n_pv & 1u) + kPCol;
+            const uint64_t vd =
+                desc128(base + S::ring + v_stage * S::tile + half0 + (g & odd) * (kHalf * 128), kTile * 128);
 #pragma unroll
             for (int k = 0; k < kHalf / 16; ++k)
-              mma_ts(lead, tm + kO + 128 * s, tm + 128 * s + 64 * buf + kPCol + k * 8, vd + k * (2048 >> 4), kIdescO,
-                     (g > 0 || k > 0) ? 1u : 0u);
-            commit(lead, &bars->pv[2 * s + buf]);
-            if (last_of_tile(g)) commit(lead, &bars->empty[v_stage]);
-            ++n_pv[s];
+              mma_ts(lead, d, p + k * 8, vd + k * (2048 >> 4), kIdescO, (g > 0 || k > 0) ? 1u : 0u);
+            commit(lead, &bars->pv[2 * s + (n_pv & 1u)]);
+            ++n_pv;
+            if ((g & odd) == odd || g == steps - 1) {
+              commit(lead, &bars->empty[v_stage]);
+              next_tile(v_stage, v_phase);
+            }
           }
-          return true;
-        };
-#pragma unroll 1
-        for (int g = -1; g < g0 && ok; ++g) {
-          ok = turn(std::integral_constant<uint32_t, 0>{}, g);
-          if (ok) ok = turn(std::integral_constant<uint32_t, 1>{}, g);
         }
-        ring += 2 * n;
+        if (!ok) break;
+        if (!pair && steps < n) {  // both streams free a tile, also one without keys for this one
+          if (steps == 0) free_q();
+          commit(lead, &bars->empty[k_stage]);
+          commit(lead, &bars->empty[v_stage]);
+          next_tile(k_stage, k_phase);
+          next_tile(v_stage, v_phase);
+          // no phase of o_free may pass unseen: a parity tells two neighbours apart only
+          if (steps == 0 && slot > 0 && !wait(&bars->o_free, (slot - 1) & 1u)) break;
+        }
       }
       // nothing may be in flight when the columns are released
       commit(lead, &bars->done);
