@@ -184,7 +184,8 @@ __device__ __forceinline__ Item suffix_item(const SharedArgs& a, const Request& 
   it.tile_cost = kCostTile;
   return it;
 }
-__device__ __forceinline__ int64_t request_cost(const SharedArgs& a, const Request& r) {
+__device__ __noinline__ int64_t request_cost(const SharedArgs& a, int b) {
+  const Request r(a, b);
   int64_t c = 0;
   for (int t = 0; t * a.tile_tokens < r.n; ++t) c += suffix_item(a, r, 0, 0, t, 0).cost();
   return c;
@@ -405,8 +406,7 @@ __device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
       : "memory");
   return __all_sync(0xffffffffu, done != 0) != 0;
 }
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (poll(bar, parity)) return true;
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, volatile int* abort) {
   const uint64_t begin = now_ns();
   for (uint32_t i = 1;; ++i) {
     if (poll(bar, parity)) return true;
@@ -415,6 +415,10 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
       return false;
     }
   }
+}
+// The loop is kept out of line: the roles' code has to stay in the instruction caches.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return poll(bar, parity) || wait_long(bar, parity, abort);
 }
 
 // One arrival for a warp (arrivals of single lanes on one barrier would queue up).
@@ -434,6 +438,10 @@ __device__ __forceinline__ void store_o(float* p, const uint32_t (&o)[32]) {
   uint4* dst = reinterpret_cast<uint4*>(p);
 #pragma unroll
   for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+}
+
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
 }
 
 // Byte offset of 16-byte chunk c of row r in a swizzled [128][D] tile.
@@ -547,7 +555,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     const int per = (a.requests + kThreadsS - 1) / kThreadsS;
     const int b0 = min(tid * per, a.requests), b1 = min(b0 + per, a.requests);
     int64_t sum = 0;
-    for (int b = b0; b < b1; ++b) sum += request_cost(a, Request(a, b));
+    for (int b = b0; b < b1; ++b) sum += request_cost(a, b);
     int64_t incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -590,7 +598,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       int64_t at = excl;
       int b = b0;
       for (; b < b1; ++b) {
-        const int64_t c = request_cost(a, Request(a, b));
+        const int64_t c = request_cost(a, b);
         if (rem < at + c) break;
         at += c;
       }
@@ -610,7 +618,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       int64_t at = excl;
       for (int b = b0; b < b1; ++b) {
         a.req_cost[b] = at;
-        at += request_cost(a, Request(a, b));
+        at += request_cost(a, b);
       }
     }
   }
@@ -654,47 +662,6 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       drain();
       return wait_warp(bar, parity, abort);
     };
-    // Waits until stage `ring` may be refilled, copies this warp's rows of K (which = 0) or V
-    // into it: all inside the item (`whole`) by TMA, else row by row. The stage is full when
-    // every loader warp's rows have landed (Q's with the first K's).
-    auto emit = [&](int row, int which, bool whole, int head) {
-      const uint32_t st = ring % S::stages, use = ring / S::stages;
-      if (use > 0) {
-        ok = wait(&bars->empty[st], (use - 1) & 1u);
-        if (!ok) return;
-      }
-      const uint32_t dst = base + S::ring + st * S::tile;
-      const bool tma = whole && a.tma_rows > 0;
-      if (tma) {
-        if (lane == 0) expect_tx(&bars->full[st], 32 * D * 2);
-        __syncwarp();
-        if ((lane & (a.tma_rows - 1)) == 0) {
-          const int z = row < 0 ? a.all_rows : row + which * a.v_rows;  // past the last row: zeros
-#pragma unroll
-          for (int x = 0; x < D; x += 64)
-            tma_rows(dst + (x >> 6) * (kTile * 128) + (32 * lw + lane) * 128, &a.map, x, head, z, &bars->full[st]);
-        }
-        __syncwarp();
-      } else {
-        const uint16_t* src = a.cache + which * a.kv_stride + static_cast<int64_t>(head) * D + chunk * 8;
-#pragma unroll 4
-        for (int i = 0; i < 32 / kRowsPer; ++i) {
-          const int r = i * kRowsPer + sub;
-          const int cr = __shfl_sync(0xffffffffu, row, r);
-          cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
-        }
-      }
-      asm volatile("cp.async.commit_group;\n" ::: "memory");
-      ++ring;
-      if (tma && !q_pending && signalled + 1 == ring) {
-        if (lane == 0) mbar_arrive(&bars->full[st]);
-        signalled = ring;
-      } else if (ring - signalled > S::lag) {
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(S::lag) : "memory");
-        signal(ring - S::lag);
-      }
-      q_pending = false;
-    };
     for (;; ++slot) {
       ok = ok && wait(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u);
       if (!ok) break;
@@ -712,7 +679,8 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       };
       int key = seg.t0 * kTile + 32 * lw + lane;
       int row = row_of(key);
-      // Q: one row tile, into the buffer after the last one used, or both for a pair
+      // Q: one row tile, into the buffer after the last one used, or both for a pair. Rows past
+      // the end keep what lies there: they reach nothing but their own rows of S and O.
       if (seg.pair) q_next = 0;
 #pragma unroll 1
       for (int q = 0; q <= seg.pair; ++q) {
@@ -725,39 +693,79 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         }
         q_used |= 1u << buf;
         // lane l finds the query row of tile row 32 lw + l
+        const int mine = min(a.tile_tokens, seg.ntok - q * a.tile_tokens) * a.group - 32 * lw;  // rows of this warp
+        if (mine <= 0) continue;
         const int tile_row = 32 * lw + lane, tl = tile_row / a.group;
-        const int rows = min(a.tile_tokens, seg.ntok - q * a.tile_tokens) * a.group;
-        const int64_t at = tile_row < rows ? (seg.tok0 + static_cast<int64_t>(q) * a.tile_tokens + tl) * a.q_token +
-                                                 (seg.h * a.group + tile_row - tl * a.group) * a.q_head
-                                           : -1;
+        const int64_t at = (seg.tok0 + static_cast<int64_t>(q) * a.tile_tokens + tl) * a.q_token +
+                           (seg.h * a.group + tile_row - tl * a.group) * a.q_head;
         const uint32_t dst = base + buf * S::tile;
-#pragma unroll 2
-        for (int i = 0; i < 32 / kRowsPer; ++i) {
-          const int r = i * kRowsPer + sub;
-          const int64_t from = __shfl_sync(0xffffffffu, at, r);
-          const uint16_t* src = a.query + (from < 0 ? 0 : from) + chunk * 8;
-          if (a.q_vec) {
-            cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src, from >= 0);
-          } else {
-            uint32_t v[4] = {0u, 0u, 0u, 0u};
-            if (from >= 0) {
+#pragma unroll 1
+        for (int i = 0; i < min(mine, 32); i += 2 * kRowsPer) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) v[j] = src[2 * j] | (static_cast<uint32_t>(src[2 * j + 1]) << 16);
+          for (int j = 0; j < 2; ++j) {
+            const int r = i + j * kRowsPer + sub;
+            const uint16_t* src = a.query + __shfl_sync(0xffffffffu, at, r & 31) + chunk * 8;
+            if (r >= mine || r >= 32) continue;
+            if (a.q_vec) {
+              cp_async16_at(dst + chunk_off(32 * lw + r, chunk), src);
+            } else {
+              uint32_t v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = src[2 * e] | (static_cast<uint32_t>(src[2 * e + 1]) << 16);
+              *reinterpret_cast<uint4*>(sm + buf * S::tile + chunk_off(32 * lw + r, chunk)) =
+                  make_uint4(v[0], v[1], v[2], v[3]);
             }
-            *reinterpret_cast<uint4*>(sm + buf * S::tile + chunk_off(32 * lw + r, chunk)) =
-                make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
+        q_pending = true;
       }
       if (!ok) break;
-      q_pending = true;
 #pragma unroll 1
       for (int i = 0; i < seg.n && ok; ++i) {
-        const bool whole = __all_sync(0xffffffffu, key < seg.kend);
+        const bool tma = a.tma_rows > 0 && __all_sync(0xffffffffu, key < seg.kend);
         key += kTile;
         const int next_row = i + 1 < seg.n ? row_of(key) : -1;
-        emit(row, 0, whole, seg.h);
-        if (ok) emit(row, 1, whole, seg.h);
+        // Waits until stage `ring` may be refilled, copies this warp's rows of K (which = 0) and
+        // of V: all inside the item by TMA, else row by row. The stage is full when every
+        // loader warp's rows have landed (Q's with the first K's).
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+          const uint32_t st = ring % S::stages, use = ring / S::stages;
+          if (use > 0 && !wait(&bars->empty[st], (use - 1) & 1u)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = base + S::ring + st * S::tile;
+          if (tma) {
+            if (lane == 0) expect_tx(&bars->full[st], 32 * D * 2);
+            __syncwarp();
+            if ((lane & (a.tma_rows - 1)) == 0) {
+              const int z = row < 0 ? a.all_rows : row + which * a.v_rows;  // past the last row: zeros
+#pragma unroll
+              for (int x = 0; x < D; x += 64)
+                tma_rows(dst + (x >> 6) * (kTile * 128) + (32 * lw + lane) * 128, &a.map, x, seg.h, z, &bars->full[st]);
+            }
+            __syncwarp();
+          } else {
+            const uint16_t* src = a.cache + which * a.kv_stride + static_cast<int64_t>(seg.h) * D + chunk * 8;
+#pragma unroll 4
+            for (int j = 0; j < 32 / kRowsPer; ++j) {
+              const int r = j * kRowsPer + sub;
+              const int cr = __shfl_sync(0xffffffffu, row, r);
+              cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
+            }
+          }
+          asm volatile("cp.async.commit_group;\n" ::: "memory");
+          ++ring;
+          if (tma && !q_pending && signalled + 1 == ring) {
+            if (lane == 0) mbar_arrive(&bars->full[st]);
+            signalled = ring;
+          } else if (ring - signalled > S::lag) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(S::lag) : "memory");
+            signal(ring - S::lag);
+          }
+          q_pending = false;
+        }
         row = next_row;
       }
     }
@@ -949,7 +957,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(x[j + 2 * k]), __uint_as_float(x[j + 2 * k + 1])));
           }
           const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-          const bool grow = mt > m + 8.f || (m == -INFINITY && mt > -INFINITY);
+          const bool grow = row < rows && (mt > m + 8.f || (m == -INFINITY && mt > -INFINITY));
           if (__any_sync(0xffffffffu, grow)) {
             const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mt)) : 1.f;
             if (i > 0) {  // O is at rest once the product of the step before has ended
