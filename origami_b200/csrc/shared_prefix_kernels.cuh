@@ -21,11 +21,11 @@
 // 128-byte-swizzled tiles, by TMA where a block's rows come in eights (a box per block), else
 // and where a tile ends inside with 16-byte cp.async (rows past the end become zeros, so
 // garbage there cannot reach the products); one warp per stream issues its tcgen05.mma; two softmax
-// warpgroups own one stream each, a stream being, in TMEM, two score buffers of 64 keys and O:
+// warpgroups own one stream each, a stream being, in TMEM, 64 keys' scores, two buffers of P and O:
 //   S_s [128 rows x 64 keys] = Q K^T (shared memory operands),
-//   O_s [128 rows x D]      += P V   (P over the second half of its S, V the N-major B operand).
-// The next 64 scores are ready when a softmax step ends, so a stream's chain is its softmax
-// alone. One thread owns one row: the softmax needs no exchange. O is rescaled only when the
+//   O_s [128 rows x D]      += P V   (P in TMEM, V the N-major B operand).
+// The next scores are begun as soon as a step has read its own, so a stream's chain is its
+// softmax alone. One thread owns one row: the softmax needs no exchange. O is rescaled only when the
 // maximum grew by more than 2^8 (P stays below 2^8, exact in the same relative precision).
 // With more than 128 rows an item has two row tiles, one per stream, that share each K and V
 // tile ("pair"); with fewer, the streams take one half of each key tile for one row tile and
@@ -48,7 +48,7 @@ constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-1
 constexpr int kTile = 128;      // keys per tile, rows per row tile
 constexpr int kHalf = 64;       // keys per softmax step
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of a segment.
-constexpr int kCostTile = 8, kCostPair = 8, kCostItem = 4;
+constexpr int kCostTile = 8, kCostPair = 13, kCostItem = 6;
 
 // Shared memory: Q tiles, then the ring of K / V tiles (each [128][D] 16-bit), then scalars.
 template <int D>
@@ -383,6 +383,11 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -481,10 +486,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// Barriers of products have one entry per stream and score buffer: the step that uses a buffer
-// next begins only after the last use's phase was seen, so a parity is never ambiguous.
+// A stream's barriers: S begins anew only when every warp has read the last (s_empty), and P's
+// two buffers have a barrier each, so that a parity is never ambiguous.
 struct Bars {
-  uint64_t full[10], empty[10], q_empty[2], s_full[4], p_full[4], pv[4], seg_full[kSegments], seg_empty[kSegments];
+  uint64_t full[10], empty[10], q_empty[2], s_full[2], s_empty[2], p_full[4], pv[4], seg_full[kSegments], seg_empty[kSegments];
   uint64_t o_free, xch, done;
 };
 
@@ -510,8 +515,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   constexpr bool kBf16 = attn::is_bf16<QT>();
   constexpr uint32_t kIdescS = attn::instr_desc(kBf16, kHalf);
   constexpr uint32_t kIdescO = attn::instr_desc(kBf16, D) | (1u << 16);  // B (V) is N-major
-  constexpr uint32_t kO = 256;  // buffer b of S_s at column 128 s + 64 b, O_s at 256 + 128 s
-  constexpr uint32_t kPCol = 32;  // P lies over the second half of its S
+  constexpr uint32_t kP = 64, kO = 128;  // of stream s: S at column 256 s, P at + 64 and + 96, O at + 128
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = static_cast<int>(blockIdx.x);
@@ -525,9 +529,12 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       mbar_init(&bars->full[i], 4);
       mbar_init(&bars->empty[i], 2);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&bars->q_empty[i], 2);
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->q_empty[i], 2);
       mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->s_empty[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bars->pv[i], 1);
       mbar_init(&bars->p_full[i], 4);
     }
@@ -847,20 +854,19 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               ok = false;
               break;
             }
-            // P of two steps before lies in this S: the last product begun must have ended
-            if (n_pv > 0 && !wait(&bars->pv[2 * s + ((n_pv - 1) & 1u)], ((n_pv - 1) >> 1) & 1u)) {
+            if (n_s > 0 && !wait(&bars->s_empty[s], (n_s - 1) & 1u)) {  // the last S has been read
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint32_t d = tm + 128 * s + 64 * (n_s & 1u);
+            const uint32_t d = tm + 256 * s;
             const uint64_t kd = desc128(base + S::ring + k_stage * S::tile + half0 + (x & odd) * (kHalf * 128), 16);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
               mma_ss(lead, d, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
             }
-            commit(lead, &bars->s_full[2 * s + (n_s & 1u)]);
+            commit(lead, &bars->s_full[s]);
             ++n_s;
             if ((x & odd) == odd || x == steps - 1) {
               commit(lead, &bars->empty[k_stage]);
@@ -879,7 +885,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               break;
             }
             tc_fence_after();
-            const uint32_t d = tm + kO + 128 * s, p = tm + 128 * s + 64 * (n_pv & 1u) + kPCol;
+            const uint32_t d = tm + 256 * s + kO, p = tm + 256 * s + kP + 32 * (n_pv & 1u);
             const uint64_t vd =
                 desc128(base + S::ring + v_stage * S::tile + half0 + (g & odd) * (kHalf * 128), kTile * 128);
 #pragma unroll
@@ -914,7 +920,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     const int s = warp >> 2;
     const int row = tid & (kTile - 1);
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t ts = lane_base + 128 * s, to = lane_base + kO + 128 * s;
+    const uint32_t ts = lane_base + 256 * s, to = ts + kO;
     const int token_in_tile = row / a.group;
     uint32_t count = 0u, x_phase = 0u;  // steps so far
     bool ok = true;
@@ -938,25 +944,31 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
 #pragma unroll 1
       for (int i = 0; i < steps; ++i) {
         const uint32_t buf = count & 1u;
-        ok = wait_warp(&bars->s_full[2 * s + buf], (count >> 1) & 1u, abort);
+        ok = wait_warp(&bars->s_full[s], count & 1u, abort);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          uint32_t x[kHalf];  // P goes over the second half of S, so all of S is read first
-          ld64(ts + 64 * buf, x);
+          uint32_t x[kHalf];
+          ld64(ts, x);
+          tc_fence_before();
+          arrive_warp(&bars->s_empty[s]);
           if (!__all_sync(0xffffffffu, lim >= kHalf || row >= rows)) {
 #pragma unroll
             for (int j = 0; j < kHalf; ++j)
               if (j >= lim) x[j] = 0xFF800000u;  // -inf: not seen
           }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mx[4];
 #pragma unroll
-          for (int j = 0; j < kHalf; j += 8) {
+          for (int k = 0; k < 4; ++k) mx[k] = __uint_as_float(x[k]);
+#pragma unroll
+          for (int j = 4; j + 8 <= kHalf; j += 8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(x[j + 2 * k]), __uint_as_float(x[j + 2 * k + 1])));
+              mx[k] = max3(mx[k], __uint_as_float(x[j + 2 * k]), __uint_as_float(x[j + 2 * k + 1]));
           }
-          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          mx[0] = max3(mx[0], __uint_as_float(x[kHalf - 4]), __uint_as_float(x[kHalf - 3]));
+          mx[1] = max3(mx[1], __uint_as_float(x[kHalf - 2]), __uint_as_float(x[kHalf - 1]));
+          const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
           const bool grow = row < rows && (mt > m + 8.f || (m == -INFINITY && mt > -INFINITY));
           if (__any_sync(0xffffffffu, grow)) {
             const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mt)) : 1.f;
@@ -977,6 +989,8 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             l *= alpha;
             m = grow ? mt : m;
           }
+          // P's buffer is free: S of this step was begun after the product of two steps before,
+          // and its barrier tells that all products begun before it have ended
           const float neg = m == -INFINITY ? 0.f : -m;
           const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), neg2 = pair2(neg, neg);
           uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
@@ -993,12 +1007,14 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               sum[j & 3] = add2(sum[j & 3], pair2(p0, p1));
               p[j] = pack2<QT>(p0, p1);
             }
-            st16(ts + 64 * buf + kPCol + 16 * q, p);
+            st16(ts + kP + 32 * buf + 16 * q, p);
           }
           float l0, l1;
           split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
           l += l0 + l1;
           st_wait();
+        } else {
+          arrive_warp(&bars->s_empty[s]);
         }
         tc_fence_before();
         arrive_warp(&bars->p_full[2 * s + buf]);
@@ -1048,7 +1064,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             uint32_t o0[32], o1[32];
             ld32(lane_base + kO + col, o0);
             if (two) {
-              ld32(lane_base + kO + 128 + col, o1);
+              ld32(lane_base + 256 + kO + col, o1);
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 o0[j] = __float_as_uint(fmaf(__uint_as_float(o0[j]), w0, __uint_as_float(o1[j]) * w1));
@@ -1100,22 +1116,21 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
     b = lo;
   }
   const Request r(a, b);
-  Item its[2];
-  {
-    const int per = prefix_item_tokens(a, used);
-    const int64_t i = t / per;
-    its[0] = prefix_item(a, used, h, i * per, h * wp + i * prefix_item(a, used, 0, 0, 0).cost());
-    const int tile = clampi((t - r.begin) / a.tile_tokens, 0, r.n > 0 ? (r.n - 1) / a.tile_tokens : 0);
-    int64_t start = a.kv_heads * wp + h * ws + __ldcg(a.req_cost + b);
-    for (int k = 0; k < tile; ++k) start += suffix_item(a, r, h, b, k, 0).cost();
-    its[1] = suffix_item(a, r, h, b, tile, start);
-  }
   float acc[kPer], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
-    const Item& it = its[k];
+    Item it;
+    if (k == 0) {
+      const int per = prefix_item_tokens(a, used), i = static_cast<int>(t) / per;
+      it = prefix_item(a, used, h, static_cast<int64_t>(i) * per, h * wp + i * prefix_item(a, used, 0, 0, 0).cost());
+    } else {
+      const int tile = clampi((static_cast<int>(t) - r.begin) / a.tile_tokens, 0, r.n > 0 ? (r.n - 1) / a.tile_tokens : 0);
+      int64_t start = a.kv_heads * wp + h * ws + __ldcg(a.req_cost + b);
+      for (int j = 0; j < tile; ++j) start += suffix_item(a, r, h, b, j, 0).cost();
+      it = suffix_item(a, r, h, b, tile, start);
+    }
     if (it.kend <= 0) continue;
     // shares that can hold a tile of the item
     const float per = static_cast<float>(a.ctas) / static_cast<float>(all);  // off by less than one share
