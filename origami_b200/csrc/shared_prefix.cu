@@ -51,7 +51,7 @@ Workspace plan(int64_t tokens, int64_t query_heads, int64_t kv_heads, int64_t he
   w.item_rows_s = static_cast<int32_t>(std::min(per, tokens) * group);
   const int64_t rows = 2 * query_heads * tokens + static_cast<int64_t>(sms) * (w.item_rows_p + w.item_rows_s);
   w.req_cost = kAlign;
-  w.ml = w.req_cost + round_up(requests * 8, kAlign);
+  w.ml = w.req_cost + round_up(requests * 4, kAlign);
   w.o = w.ml + round_up(rows * 8, kAlign);
   w.bytes = w.o + round_up(rows * head_dim * 4, kAlign);
   return w;
@@ -162,6 +162,17 @@ int32_t origami_shared_prefix_attention(
   if (d_lse != nullptr && !aligned(d_lse, 4)) return fail(ORIGAMI_ERR_INVALID, "lse must be a float32 device array");
   int sms = 0;
   if ((rc = device_sms(sms))) return rc;
+  // every item's cost, at most, has to fit the 31-bit cost axis of the deal
+  const int64_t per_tile = origami::spa::kTile / (query->num_heads / cache->num_heads);
+  const int64_t row_tiles = (tokens + per_tile - 1) / per_tile;
+  const int64_t suffix_cap = std::min<int64_t>(suffix_width, 0x3FFFFFFF / cache->block_size) * cache->block_size;
+  auto cost = [](int64_t keys, int64_t tile) {
+    return origami::spa::kCostItem + (keys + origami::spa::kTile - 1) / origami::spa::kTile * tile;
+  };
+  const double most = static_cast<double>(cache->num_heads) *
+                      (static_cast<double>(row_tiles) * cost(prefix_tokens, origami::spa::kCostPair) +
+                       static_cast<double>(row_tiles + requests) * cost(suffix_cap, origami::spa::kCostTile));
+  if (most >= 2147483648.0) return fail(ORIGAMI_ERR_UNSUPPORTED, "too many tiles of keys and query rows for one call");
   const Workspace w = plan(tokens, query->num_heads, cache->num_heads, head_dim, requests, sms);
   if (d_workspace == nullptr || workspace_bytes < w.bytes || !aligned(d_workspace, 16))
     return fail(ORIGAMI_ERR_INVALID, "workspace must be 16-byte aligned and hold %lld bytes",
@@ -189,7 +200,7 @@ int32_t origami_shared_prefix_attention(
   a.tokens = static_cast<int32_t>(tokens);
   a.requests = static_cast<int32_t>(requests);
   a.prefix = static_cast<int32_t>(prefix_tokens);
-  a.suffix_cap = static_cast<int32_t>(std::min<int64_t>(suffix_width, 0x3FFFFFFF / cache->block_size) * cache->block_size);
+  a.suffix_cap = static_cast<int32_t>(suffix_cap);
   a.q_heads = static_cast<int32_t>(query->num_heads);
   a.kv_heads = static_cast<int32_t>(cache->num_heads);
   a.group = a.q_heads / a.kv_heads;
@@ -198,7 +209,7 @@ int32_t origami_shared_prefix_attention(
   a.item_rows_s = w.item_rows_s;
   a.all_rows = static_cast<int32_t>(2 * cache->num_blocks * cache->block_size);
   a.v_rows = static_cast<int32_t>(g.kv_stride / g.token_stride);
-  a.inv_ctas = sms > 1 ? ~0ull / static_cast<uint64_t>(sms) : ~0ull;
+  a.inv_ctas = static_cast<uint32_t>(0x100000000ull / static_cast<uint64_t>(std::max(sms, 2)));  // (unused for one CTA)
   // TMA boxes of at least one swizzle atom (8 rows) that lie inside one block and one warp's 32 rows
   a.tma_rows = 32;
   while (a.tma_rows >= 8 && cache->block_size % a.tma_rows != 0) a.tma_rows /= 2;
@@ -220,8 +231,8 @@ int32_t origami_shared_prefix_attention(
   a.ctas = sms;
   a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   uint8_t* ws = static_cast<uint8_t*>(d_workspace);
-  a.head = reinterpret_cast<int64_t*>(ws);
-  a.req_cost = reinterpret_cast<int64_t*>(ws + w.req_cost);
+  a.head = reinterpret_cast<int32_t*>(ws);
+  a.req_cost = reinterpret_cast<int32_t*>(ws + w.req_cost);
   a.ml = reinterpret_cast<float*>(ws + w.ml);
   a.o = reinterpret_cast<float*>(ws + w.o);
   a.err = d_error_flags;

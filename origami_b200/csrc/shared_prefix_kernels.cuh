@@ -84,11 +84,11 @@ struct SharedArgs {
   int32_t q_vec, o_vec, ctas;
   int32_t tma_rows;   // token rows per TMA box (divides the block size), 0: no TMA
   int32_t all_rows, v_rows;  // token rows of the cache; rows from a token's K to its V
-  uint64_t inv_ctas;  // floor(2^64 / ctas)
+  uint32_t inv_ctas;         // floor(2^32 / ctas)
   float scale_log2;
   // workspace
-  int64_t* head;      // {prefix cost per head, suffix cost per head}
-  int64_t* req_cost;  // [requests] suffix cost of the requests before this one
+  int32_t* head;      // {prefix cost per head, suffix cost per head}
+  int32_t* req_cost;  // [requests] suffix cost of the requests before this one
   float* ml;          // [rows][2]
   float* o;           // [rows][D]
   uint32_t* err;
@@ -101,104 +101,95 @@ using attn::proxy_fence;
 using attn::tc_fence_after;
 using attn::tc_fence_before;
 
-__device__ __forceinline__ int clampi(int64_t v, int64_t lo, int64_t hi) {
-  return static_cast<int>(v < lo ? lo : v > hi ? hi : v);
-}
-
 // ---------------------------------------------------------------------------------------
 // The deal: items in order (prefix items of head 0, 1, ..; then suffix items of head 0, 1,
-// .. by request and row tile), each with a start on the cost axis.
+// .. by request and row tile), each with a start on the cost axis (below 2^31: the host checks).
 // ---------------------------------------------------------------------------------------
 struct Item {
-  int64_t start;   // on the cost axis
-  int64_t tok0;    // first token
+  int32_t start;   // on the cost axis
+  int32_t tok0;    // first token
   int32_t ntok;    // its tokens
   int32_t kend;    // keys its last row sees
   int32_t vis0;    // suffix: keys its first token sees (may be negative)
   int32_t h, b;    // KV head; request, -1 for the prefix
-  int32_t tile_cost;
   bool pair;
   __device__ __forceinline__ int tiles() const { return (kend + kTile - 1) / kTile; }
-  __device__ __forceinline__ int64_t cost() const { return kend > 0 ? kCostItem + static_cast<int64_t>(tiles()) * tile_cost : 0; }
+  __device__ __forceinline__ int cost() const {
+    return kend > 0 ? kCostItem + tiles() * (pair ? kCostPair : kCostTile) : 0;
+  }
   // First tile that a share beginning at w takes.
-  __device__ __forceinline__ int tile_at(int64_t w) const {
-    const int64_t x = w - start - kCostItem;
+  __device__ __forceinline__ int tile_at(int w) const {
+    const int x = w - start - kCostItem;
     if (x <= 0) return 0;
-    const int64_t t = pair ? (x + kCostPair - 1) / kCostPair : (x + kCostTile - 1) / kCostTile;
-    return t > tiles() ? tiles() : static_cast<int>(t);
+    return min(pair ? (x + kCostPair - 1) / kCostPair : (x + kCostTile - 1) / kCostTile, tiles());
   }
 };
 
 // Where CTA c's share begins: monotone in c, 0 and `all` at the ends.
-__device__ __forceinline__ int64_t share_begin(const SharedArgs& a, int64_t all, int c) {
-  return c >= a.ctas ? all : static_cast<int64_t>(__umul64hi(static_cast<uint64_t>(all) * c, a.inv_ctas));
+__device__ __forceinline__ int share_begin(const SharedArgs& a, int all, int c) {
+  return c >= a.ctas ? all : static_cast<int>(__umulhi(static_cast<uint32_t>(all), static_cast<uint32_t>(c) * a.inv_ctas));
 }
+__device__ __forceinline__ int clamp32(int v, int lo, int hi) { return min(max(v, lo), hi); }
 __device__ __forceinline__ int used_tokens(const SharedArgs& a) {
-  return clampi(__ldg(a.query_start + a.requests), 0, a.tokens);
+  return clamp32(__ldg(a.query_start + a.requests), 0, a.tokens);
 }
 __device__ __forceinline__ int prefix_item_tokens(const SharedArgs& a, int used) {
   return used > a.tile_tokens ? 2 * a.tile_tokens : a.tile_tokens;
 }
-__device__ __forceinline__ Item prefix_item(const SharedArgs& a, int used, int h, int64_t tok0, int64_t start) {
+__device__ __forceinline__ Item prefix_item(const SharedArgs& a, int used, int h, int tok0, int start) {
   Item it;
   it.start = start;
   it.tok0 = tok0;
-  it.ntok = clampi(used - tok0, 0, prefix_item_tokens(a, used));
+  it.ntok = clamp32(used - tok0, 0, prefix_item_tokens(a, used));
   it.kend = a.prefix;
   it.vis0 = a.prefix;
   it.h = h;
   it.b = -1;
   it.pair = it.ntok > a.tile_tokens;
-  it.tile_cost = it.pair ? kCostPair : kCostTile;
   return it;
 }
 // Cost of all prefix items of one head.
-__device__ __forceinline__ int64_t prefix_cost(const SharedArgs& a, int used) {
+__device__ __forceinline__ int prefix_cost(const SharedArgs& a, int used) {
   if (used == 0 || a.prefix == 0) return 0;
-  const int per = prefix_item_tokens(a, used);
-  const int64_t items = (used + per - 1) / per;
-  const Item first = prefix_item(a, used, 0, 0, 0);
-  const Item last = prefix_item(a, used, 0, (items - 1) * per, 0);
-  return (items - 1) * first.cost() + last.cost();
+  const int per = prefix_item_tokens(a, used), before = (used - 1) / per;
+  return before * prefix_item(a, used, 0, 0, 0).cost() + prefix_item(a, used, 0, before * per, 0).cost();
 }
 
 struct Request {
   int32_t begin, n, len;
   __device__ __forceinline__ Request(const SharedArgs& a, int b) {
-    begin = clampi(__ldg(a.query_start + b), 0, a.tokens);
-    n = clampi(__ldg(a.query_start + b + 1), begin, a.tokens) - begin;
-    len = clampi(__ldg(a.suffix_lens + b), 0, a.suffix_cap);
+    begin = clamp32(__ldg(a.query_start + b), 0, a.tokens);
+    n = clamp32(__ldg(a.query_start + b + 1), begin, a.tokens) - begin;
+    len = clamp32(__ldg(a.suffix_lens + b), 0, a.suffix_cap);
   }
 };
-__device__ __forceinline__ Item suffix_item(const SharedArgs& a, const Request& r, int h, int b, int tile, int64_t start) {
+__device__ __forceinline__ Item suffix_item(const SharedArgs& a, const Request& r, int h, int b, int tile, int start) {
   Item it;
   it.start = start;
   const int t0 = tile * a.tile_tokens;
   it.tok0 = r.begin + t0;
   it.ntok = min(a.tile_tokens, r.n - t0);
   it.vis0 = r.len - r.n + t0 + 1;
-  it.kend = clampi(static_cast<int64_t>(it.vis0) + it.ntok - 1, 0, r.len);
+  it.kend = clamp32(it.vis0 + it.ntok - 1, 0, r.len);
   it.h = h;
   it.b = b;
   it.pair = false;
-  it.tile_cost = kCostTile;
   return it;
 }
-__device__ __noinline__ int64_t request_cost(const SharedArgs& a, int b) {
-  const Request r(a, b);
-  int64_t c = 0;
+// Cost of a request's row tiles.
+__device__ __forceinline__ int request_cost(const SharedArgs& a, const Request& r) {
+  int c = 0;
+#pragma unroll 1
   for (int t = 0; t * a.tile_tokens < r.n; ++t) c += suffix_item(a, r, 0, 0, t, 0).cost();
   return c;
 }
 
-// Where the shares begin, known to every thread of a CTA.
+// Where a CTA's share begins and ends, and its first suffix item.
 struct Deal {
-  int64_t wp, ws;  // cost of one head's prefix / suffix items
-  int64_t w0, w1;  // this CTA's share
+  int32_t wp;      // cost of one head's prefix items
+  int32_t w0, w1;  // this CTA's share
   int32_t used;
-  // the first suffix item of the share
-  int32_t h, b, tile;
-  int64_t start;
+  int32_t h, b, tile, start;
 };
 
 // Walks the segments of a CTA's share (one warp of the CTA).
@@ -207,15 +198,13 @@ struct Walk {
   const Deal& d;
   Item it;
   int t0, t1;      // tiles of the segment
-  int64_t next;    // start of the item after `it`
+  int next;        // start of the item after `it`
   int h, b, tile;  // next suffix item
-  int ph;          // next prefix item: head and first token
-  int64_t ptok;
+  int ph, ptok;    // next prefix item: head and first token
   bool in_prefix;
   Request r;
-  __device__ __forceinline__ Walk(const SharedArgs& args, const Deal& deal) : a(args), d(deal), r(args, deal.b < 0 ? 0 : deal.b) {
-    const int64_t all = d.wp * a.kv_heads;
-    in_prefix = d.w0 < all;
+  __device__ __forceinline__ Walk(const SharedArgs& args, const Deal& deal) : a(args), d(deal), r(args, deal.b) {
+    in_prefix = d.w0 < d.wp * a.kv_heads;
     h = d.h;
     b = d.b;
     tile = d.tile;
@@ -223,20 +212,18 @@ struct Walk {
     ph = 0;
     ptok = 0;
     if (in_prefix) {
-      const int per = prefix_item_tokens(a, d.used);
-      int64_t in_head = d.w0;
-      for (; in_head >= d.wp; in_head -= d.wp) ++ph;
-      const int64_t first = prefix_item(a, d.used, 0, 0, 0).cost();
-      const int64_t i = in_head < first ? 0 : min64(in_head / first, (d.used + per - 1) / per - 1);
+      const int per = prefix_item_tokens(a, d.used), first = prefix_item(a, d.used, 0, 0, 0).cost();
+      ph = d.w0 / d.wp;
+      const int i = min((d.w0 - ph * d.wp) / first, (d.used - 1) / per);
       ptok = i * per;
       next = ph * d.wp + i * first;
     }
   }
   __device__ __forceinline__ bool step() {
+#pragma unroll 1
     while (next < d.w1) {
       if (in_prefix) {
         it = prefix_item(a, d.used, ph, ptok, next);
-        next += it.cost();
         ptok += it.ntok;
         if (ptok >= d.used) {
           ptok = 0;
@@ -248,7 +235,7 @@ struct Walk {
           r = Request(a, 0);
         }
       } else {
-        // stop past the last head (requests without any tile cost nothing and end nowhere)
+        // past the last head there is nothing (requests without any tile cost nothing)
         if (h >= a.kv_heads) return false;
         if (tile * a.tile_tokens >= r.n) {
           tile = 0;
@@ -260,9 +247,9 @@ struct Walk {
           continue;
         }
         it = suffix_item(a, r, h, b, tile, next);
-        next += it.cost();
         ++tile;
       }
+      next += it.cost();
       if (it.kend <= 0) continue;
       t0 = it.tile_at(d.w0);
       t1 = it.tile_at(d.w1);
@@ -558,41 +545,42 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
 
   // The deal: suffix costs of contiguous runs of requests, scanned over the CTA.
   {
-    int64_t* scan = reinterpret_cast<int64_t*>(sm);  // [13] warp sums
+    int* scan = reinterpret_cast<int*>(sm);  // [16] warp sums
     const int per = (a.requests + kThreadsS - 1) / kThreadsS;
     const int b0 = min(tid * per, a.requests), b1 = min(b0 + per, a.requests);
-    int64_t sum = 0;
-    for (int b = b0; b < b1; ++b) sum += request_cost(a, b);
-    int64_t incl = sum;
+    const int used = used_tokens(a);
+    int sum = 0;
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) sum += request_cost(a, Request(a, b));
+    int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int64_t before = 0, total = 0;
-    for (int w = 0; w < kThreadsS / 32; ++w) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
+    int before = lane < kThreadsS / 32 ? scan[lane] : 0, total = before;
+    if (lane >= warp) before = 0;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
     }
-    const int64_t excl = before + incl - sum;
-    const int used = used_tokens(a);
-    const int64_t wp = prefix_cost(a, used), all_p = wp * a.kv_heads, all = all_p + total * a.kv_heads;
-    const int64_t w0 = share_begin(a, all, cta), w1 = share_begin(a, all, cta + 1);
-    // the share's first suffix item: in the run of requests that holds its cost
-    const int64_t y = w0 <= all_p ? 0 : w0 - all_p;
-    int fh = 0;
-    int64_t rem = y;
-    for (; total > 0 && rem >= total; rem -= total) ++fh;
+    before = __shfl_sync(0xffffffffu, before, 0);
+    total = __shfl_sync(0xffffffffu, total, 0);
+    const int excl = before + incl - sum;
+    const int wp = prefix_cost(a, used), all_p = wp * a.kv_heads, all = all_p + total * a.kv_heads;
+    const int w0 = share_begin(a, all, cta);
+    // the share's first suffix item lies in the run of requests that holds its cost
+    const int y = max(w0 - all_p, 0), fh = total > 0 ? y / total : a.kv_heads, rem = total > 0 ? y - fh * total : 0;
     if (tid == 0) {
       deal_sm->wp = wp;
-      deal_sm->ws = total;
       deal_sm->w0 = w0;
-      deal_sm->w1 = w1;
+      deal_sm->w1 = share_begin(a, all, cta + 1);
       deal_sm->used = used;
-      if (total == 0) {
-        deal_sm->h = a.kv_heads;  // no suffix anywhere
+      if (total == 0) {  // no suffix anywhere
+        deal_sm->h = fh;
         deal_sm->b = deal_sm->tile = 0;
         deal_sm->start = all_p;
       }
@@ -601,31 +589,27 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         a.head[1] = total;
       }
     }
-    if (sum > 0 && rem >= excl && rem < excl + sum) {
-      int64_t at = excl;
-      int b = b0;
-      for (; b < b1; ++b) {
-        const int64_t c = request_cost(a, b);
-        if (rem < at + c) break;
-        at += c;
-      }
-      const Request r(a, b);
-      int t = 0;
-      for (;; ++t) {
-        const int64_t c = suffix_item(a, r, 0, 0, t, 0).cost();
-        if (rem < at + c) break;
-        at += c;
-      }
-      deal_sm->h = fh;
-      deal_sm->b = b;
-      deal_sm->tile = t;
-      deal_sm->start = all_p + fh * total + at;
-    }
-    if (cta == 0) {
-      int64_t at = excl;
+    if ((sum > 0 && rem >= excl && rem < excl + sum) || cta == 0) {
+      int at = excl;
+#pragma unroll 1
       for (int b = b0; b < b1; ++b) {
-        a.req_cost[b] = at;
-        at += request_cost(a, b);
+        const Request r(a, b);
+        const int c = request_cost(a, r);
+        if (cta == 0) a.req_cost[b] = at;
+        if (c > 0 && rem >= at && rem < at + c) {
+          int t = 0, start = at;
+#pragma unroll 1
+          for (;; ++t) {
+            const int x = suffix_item(a, r, 0, 0, t, 0).cost();
+            if (rem < start + x) break;
+            start += x;
+          }
+          deal_sm->h = fh;
+          deal_sm->b = b;
+          deal_sm->tile = t;
+          deal_sm->start = all_p + fh * total + start;
+        }
+        at += c;
       }
     }
   }
@@ -798,7 +782,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           g.pair = w.it.pair;
           g.h = w.it.h;
           g.b = w.it.b;
-          g.tok0 = static_cast<int32_t>(w.it.tok0);
+          g.tok0 = w.it.tok0;
           g.ntok = w.it.ntok;
           g.kend = w.it.kend;
           g.vis0 = w.it.vis0;
@@ -938,7 +922,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       const bool warp_live = (warp & 3) * 32 < rows;
       // keys of the item this row sees, less those before the current step's
       int lim = 0;
-      if (row < rows) lim = seg.b < 0 ? seg.kend : clampi(static_cast<int64_t>(seg.vis0) + token_in_tile, 0, seg.kend);
+      if (row < rows) lim = seg.b < 0 ? seg.kend : clamp32(seg.vis0 + token_in_tile, 0, seg.kend);
       lim -= seg.t0 * kTile + (pair ? 0 : s * kHalf);
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
@@ -1097,16 +1081,15 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   constexpr int kPer = D / 32;  // dims per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t = blockIdx.x;
+  const int t = static_cast<int>(blockIdx.x);
   const int qh = static_cast<int>(blockIdx.y) * 8 + warp;
   const int used = used_tokens(a);
-  if (qh >= a.q_heads || t >= used || t < clampi(__ldg(a.query_start), 0, a.tokens)) return;
-  const int h = qh / a.group, g = qh - h * a.group;
-  const int64_t wp = __ldcg(a.head), ws = __ldcg(a.head + 1);
-  const int64_t all = (wp + ws) * a.kv_heads;
   // the request: token t itself in a step of one token each, else by bisection
-  int b = clampi(t, 0, a.requests - 1);
-  if (!(__ldg(a.query_start + b) <= t && t < __ldg(a.query_start + b + 1))) {
+  int b = clamp32(t, 0, a.requests - 1);
+  const int first = __ldg(a.query_start), lo0 = __ldg(a.query_start + b), hi0 = __ldg(a.query_start + b + 1);
+  const int wp = __ldcg(a.head), ws = __ldcg(a.head + 1);
+  if (qh >= a.q_heads || t >= used || t < first) return;
+  if (t < lo0 || t >= hi0) {
     int lo = 0, hi = a.requests;  // query_start[lo] <= t < query_start[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -1115,7 +1098,9 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
     }
     b = lo;
   }
-  const Request r(a, b);
+  const int h = qh / a.group, g = qh - h * a.group;
+  const int all = (wp + ws) * a.kv_heads;
+  const float shares = static_cast<float>(a.ctas) / static_cast<float>(all);
   float acc[kPer], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
@@ -1123,24 +1108,30 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
   for (int k = 0; k < 2; ++k) {
     Item it;
     if (k == 0) {
-      const int per = prefix_item_tokens(a, used), i = static_cast<int>(t) / per;
-      it = prefix_item(a, used, h, static_cast<int64_t>(i) * per, h * wp + i * prefix_item(a, used, 0, 0, 0).cost());
+      const int per = prefix_item_tokens(a, used), i = t / per;
+      it = prefix_item(a, used, h, i * per, h * wp + i * prefix_item(a, used, 0, 0, 0).cost());
     } else {
-      const int tile = clampi((static_cast<int>(t) - r.begin) / a.tile_tokens, 0, r.n > 0 ? (r.n - 1) / a.tile_tokens : 0);
-      int64_t start = a.kv_heads * wp + h * ws + __ldcg(a.req_cost + b);
-      for (int j = 0; j < tile; ++j) start += suffix_item(a, r, h, b, j, 0).cost();
-      it = suffix_item(a, r, h, b, tile, start);
+      const Request r(a, b);
+      const int tile = (t - r.begin) / a.tile_tokens;
+      int before = 0;  // cost of the request's row tiles before this one
+      for (int j = lane; j < tile; j += 32) before += suffix_item(a, r, h, b, j, 0).cost();
+      if (tile > 0) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      }
+      it = suffix_item(a, r, h, b, tile, a.kv_heads * wp + h * ws + __ldcg(a.req_cost + b) + before);
     }
     if (it.kend <= 0) continue;
     // shares that can hold a tile of the item
-    const float per = static_cast<float>(a.ctas) / static_cast<float>(all);  // off by less than one share
-    const int c0 = max(static_cast<int>(static_cast<float>(it.start) * per) - 2, 0);
-    const int c1 = min(static_cast<int>(static_cast<float>(it.start + it.cost()) * per) + 2, a.ctas - 1);
+    const int c0 = max(static_cast<int>(it.start * shares) - 2, 0);  // (float: off by less than one share)
+    const int c1 = min(static_cast<int>((it.start + it.cost()) * shares) + 2, a.ctas - 1);
+    const int64_t row0 = partial_base(a, it, 0) + static_cast<int64_t>(t - it.tok0) * a.group + g;
+    const int item_rows = it.b < 0 ? a.item_rows_p : a.item_rows_s;
     for (int cb = c0; cb <= c1; cb += 32) {
       const int c = cb + lane;
       float2 ml = make_float2(-INFINITY, 0.f);
       if (c <= c1 && it.tile_at(share_begin(a, all, c + 1)) > it.tile_at(share_begin(a, all, c)))
-        ml = __ldcg(reinterpret_cast<const float2*>(a.ml) + partial_base(a, it, c) + (t - it.tok0) * a.group + g);
+        ml = __ldcg(reinterpret_cast<const float2*>(a.ml) + row0 + static_cast<int64_t>(c) * item_rows);
       float mx = ml.x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -1156,8 +1147,8 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
 #pragma unroll
       for (int i = 0; i < kPer; ++i) acc[i] *= alpha;
       unsigned live = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
-      const float* o0 = a.o + (partial_base(a, it, cb) + (t - it.tok0) * a.group + g) * D + lane * kPer;
-      const int64_t stride = static_cast<int64_t>(it.b < 0 ? a.item_rows_p : a.item_rows_s) * D;
+      const float* o0 = a.o + (row0 + static_cast<int64_t>(cb) * item_rows) * D + lane * kPer;
+      const int64_t stride = static_cast<int64_t>(item_rows) * D;
       while (live) {
         float v[4][kPer], wv[4];
 #pragma unroll
@@ -1189,7 +1180,7 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
   }
   // l > 0 wherever a key has weight; NaN stays NaN
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* out = a.output + t * a.o_token + static_cast<int64_t>(qh) * a.o_head + lane * kPer;
+  uint16_t* out = a.output + static_cast<int64_t>(t) * a.o_token + static_cast<int64_t>(qh) * a.o_head + lane * kPer;
   uint32_t packed[kPer / 2];
 #pragma unroll
   for (int i = 0; i < kPer / 2; ++i) packed[i] = pack2<QT>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
@@ -1201,7 +1192,7 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
     for (int i = 0; i < kPer; ++i) out[i] = static_cast<uint16_t>(packed[i / 2] >> (16 * (i & 1)));
   }
   if (a.lse && lane == 0)
-    a.lse[t * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    a.lse[static_cast<int64_t>(t) * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
 }  // namespace origami
