@@ -84,8 +84,9 @@ int32_t launch(const origami::SharedArgs& a, cudaStream_t st) {
   rc = launch_dependent(fn, dim3(static_cast<unsigned>(a.ctas)), origami::spa::kThreadsS, smem, st,
                         "shared_prefix_attention launch", a);
   if (rc) return rc;
+  const int64_t warps = static_cast<int64_t>(a.tokens) * a.kv_heads * ((a.group + a.merge_rows - 1) / a.merge_rows);
   return launch_dependent(&origami::merge_partials<QT, D>,
-                          dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>((a.q_heads + 7) / 8)), 256, 0, st,
+                          dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st,
                           "merge_partials launch", a);
 }
 
@@ -229,6 +230,9 @@ int32_t origami_shared_prefix_attention(
   a.q_vec = rows_vec(query);
   a.o_vec = rows_vec(output);
   a.ctas = sms;
+  // One row a warp while the rows are few (their latency counts), more when their lists' lookup would
+  // be what an SM spends its issue slots on.
+  a.merge_rows = static_cast<int32_t>(std::clamp<int64_t>(tokens * a.q_heads / (32 * sms), 1, a.group));
   a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   uint8_t* ws = static_cast<uint8_t*>(d_workspace);
   a.head = reinterpret_cast<int32_t*>(ws);

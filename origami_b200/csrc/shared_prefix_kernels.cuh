@@ -82,12 +82,13 @@ struct SharedArgs {
   int32_t q_heads, kv_heads, group, tile_tokens;  // tokens per row tile
   int32_t item_rows_p, item_rows_s;               // partial rows a CTA may need for a prefix / suffix item
   int32_t q_vec, o_vec, ctas;
+  int32_t merge_rows;  // rows a warp of merge_partials joins
   int32_t tma_rows;   // token rows per TMA box (divides the block size), 0: no TMA
   int32_t all_rows, v_rows;  // token rows of the cache; rows from a token's K to its V
   uint32_t inv_ctas;         // floor(2^32 / ctas)
   float scale_log2;
   // workspace
-  int32_t* head;      // {prefix cost per head, suffix cost per head}
+  int32_t* head;      // suffix cost of one head
   int32_t* req_cost;  // [requests] suffix cost of the requests before this one
   float* ml;          // [rows][2]
   float* o;           // [rows][D]
@@ -584,10 +585,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         deal_sm->b = deal_sm->tile = 0;
         deal_sm->start = all_p;
       }
-      if (cta == 0) {
-        a.head[0] = wp;
-        a.head[1] = total;
-      }
+      if (cta == 0) *a.head = total;
     }
     if ((sum > 0 && rem >= excl && rem < excl + sum) || cta == 0) {
       int at = excl;
@@ -1073,22 +1071,46 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
 }
 
 // ---------------------------------------------------------------------------------------
-// Joins the partials of each row: one warp per (token, query head).
+// Joins the partials of the rows: a warp takes merge_rows rows (query heads) of one token and
+// KV head, which share their list of partials. A lane stands for one partial (its place and
+// weight) and, in the sum, for D / 32 dims.
 // ---------------------------------------------------------------------------------------
+namespace spa {
+
+// The shares that can hold a tile of an item, and where its partial rows lie.
+struct Parts {
+  Item it;
+  int32_t first, count, stride;
+  int64_t row0;
+  __device__ __forceinline__ Parts(const SharedArgs& a, const Item& item, int t, int all, float shares) : it(item) {
+    // (float: off by less than one share)
+    first = max(static_cast<int>(static_cast<float>(it.start) * shares) - 2, 0);
+    const int last = min(static_cast<int>(static_cast<float>(it.start + it.cost()) * shares) + 2, a.ctas - 1);
+    count = it.kend > 0 ? last - first + 1 : 0;
+    stride = it.b < 0 ? a.item_rows_p : a.item_rows_s;
+    row0 = partial_base(a, it, first) + static_cast<int64_t>(t - it.tok0) * a.group;
+  }
+};
+
+}  // namespace spa
+
 template <typename QT, int D>
 __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ SharedArgs a) {
   using namespace spa;
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   constexpr int kPer = D / 32;  // dims per lane
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = static_cast<int>(blockIdx.x);
-  const int qh = static_cast<int>(blockIdx.y) * 8 + warp;
+  constexpr int kAhead = 8;     // partials' loads in flight
+  const int lane = threadIdx.x & 31;
+  const int per_head = (a.group + a.merge_rows - 1) / a.merge_rows, per_token = a.kv_heads * per_head;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int t = static_cast<int>(unit / per_token), in_token = static_cast<int>(unit - static_cast<int64_t>(t) * per_token);
+  const int h = in_token / per_head, g0 = (in_token - h * per_head) * a.merge_rows;
+  // The lists are this launch's inputs as much as the first kernel's, which had waited for what
+  // wrote them before it let this one start: read ahead of the wait for its partials.
   const int used = used_tokens(a);
   // the request: token t itself in a step of one token each, else by bisection
   int b = clamp32(t, 0, a.requests - 1);
   const int first = __ldg(a.query_start), lo0 = __ldg(a.query_start + b), hi0 = __ldg(a.query_start + b + 1);
-  const int wp = __ldcg(a.head), ws = __ldcg(a.head + 1);
-  if (qh >= a.q_heads || t >= used || t < first) return;
+  if (t >= used || t < first) return;
   if (t < lo0 || t >= hi0) {
     int lo = 0, hi = a.requests;  // query_start[lo] <= t < query_start[hi]
     while (hi - lo > 1) {
@@ -1098,44 +1120,52 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
     }
     b = lo;
   }
-  const int h = qh / a.group, g = qh - h * a.group;
+  const Request r(a, b);
+  const int tile = (t - r.begin) / a.tile_tokens;
+  int before = 0;  // cost of the request's row tiles before this one
+  if (tile > 0) {
+    for (int j = lane; j < tile; j += 32) before += suffix_item(a, r, h, b, j, 0).cost();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  const int wp = prefix_cost(a, used), per = prefix_item_tokens(a, used), pi = t / per;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int ws = __ldcg(a.head);
+  before += __ldcg(a.req_cost + b);
   const int all = (wp + ws) * a.kv_heads;
   const float shares = static_cast<float>(a.ctas) / static_cast<float>(all);
-  float acc[kPer], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+  const Parts pre(a, prefix_item(a, used, h, pi * per, h * wp + pi * prefix_item(a, used, 0, 0, 0).cost()), t, all, shares);
+  const Parts suf(a, suffix_item(a, r, h, b, tile, a.kv_heads * wp + h * ws + before), t, all, shares);
+  const int parts = pre.count + suf.count;
+  // partial row of the token's first row in partial i of the list, -1 where the share holds none
+  auto place = [&](int i) -> int64_t {
+    if (i >= parts) return -1;
+    const bool p = i < pre.count;
+    const Item& it = p ? pre.it : suf.it;
+    const int k = p ? i : i - pre.count, c = (p ? pre.first : suf.first) + k;
+    if (it.tile_at(share_begin(a, all, c + 1)) <= it.tile_at(share_begin(a, all, c))) return -1;
+    return (p ? pre.row0 : suf.row0) + static_cast<int64_t>(k) * (p ? pre.stride : suf.stride);
+  };
+  const int64_t mine = place(lane);
+  auto load_ml = [&](int64_t row) {
+    return row < 0 ? make_float2(-INFINITY, 0.f) : __ldcg(reinterpret_cast<const float2*>(a.ml) + row);
+  };
+  const int g_end = min(g0 + a.merge_rows, a.group);
+  float2 ml_next = load_ml(mine < 0 ? mine : mine + g0);
 #pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    Item it;
-    if (k == 0) {
-      const int per = prefix_item_tokens(a, used), i = t / per;
-      it = prefix_item(a, used, h, i * per, h * wp + i * prefix_item(a, used, 0, 0, 0).cost());
-    } else {
-      const Request r(a, b);
-      const int tile = (t - r.begin) / a.tile_tokens;
-      int before = 0;  // cost of the request's row tiles before this one
-      for (int j = lane; j < tile; j += 32) before += suffix_item(a, r, h, b, j, 0).cost();
-      if (tile > 0) {
+  for (int g = g0; g < g_end; ++g) {
+    const float2 ml_mine = ml_next;
+    if (g + 1 < g_end) ml_next = load_ml(mine < 0 ? mine : mine + g + 1);
+    float acc[kPer], m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-      }
-      it = suffix_item(a, r, h, b, tile, a.kv_heads * wp + h * ws + __ldcg(a.req_cost + b) + before);
-    }
-    if (it.kend <= 0) continue;
-    // shares that can hold a tile of the item
-    const int c0 = max(static_cast<int>(it.start * shares) - 2, 0);  // (float: off by less than one share)
-    const int c1 = min(static_cast<int>((it.start + it.cost()) * shares) + 2, a.ctas - 1);
-    const int64_t row0 = partial_base(a, it, 0) + static_cast<int64_t>(t - it.tok0) * a.group + g;
-    const int item_rows = it.b < 0 ? a.item_rows_p : a.item_rows_s;
-    for (int cb = c0; cb <= c1; cb += 32) {
-      const int c = cb + lane;
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (c <= c1 && it.tile_at(share_begin(a, all, c + 1)) > it.tile_at(share_begin(a, all, c)))
-        ml = __ldcg(reinterpret_cast<const float2*>(a.ml) + row0 + static_cast<int64_t>(c) * item_rows);
-      float mx = ml.x;
+    for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+#pragma unroll 1
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      const int64_t row = i0 == 0 ? mine : place(i0 + lane);
+      const float2 ml = i0 == 0 ? ml_mine : load_ml(row < 0 ? row : row + g);
+      float mn = fmaxf(m, ml.x);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float mn = fmaxf(m, mx);
+      for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
       if (mn == -INFINITY) continue;  // nothing with weight here
       const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
       const float wgt = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
@@ -1144,19 +1174,19 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       l = fmaf(l, alpha, sum);
       m = mn;
+      if (i0 > 0) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) acc[i] *= alpha;
+        for (int i = 0; i < kPer; ++i) acc[i] *= alpha;
+      }
       unsigned live = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
-      const float* o0 = a.o + (row0 + static_cast<int64_t>(cb) * item_rows) * D + lane * kPer;
-      const int64_t stride = static_cast<int64_t>(item_rows) * D;
       while (live) {
-        float v[4][kPer], wv[4];
+        float v[kAhead][kPer], wv[kAhead];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kAhead; ++u) {
           const int src = live ? __ffs(live) - 1 : 0;
-          wv[u] = live ? 1.f : 0.f;
-          wv[u] *= __shfl_sync(0xffffffffu, wgt, src);
-          const float* p = o0 + src * stride;
+          const float w = __shfl_sync(0xffffffffu, wgt, src);
+          const float* p = a.o + (__shfl_sync(0xffffffffu, row, src) + g) * D + lane * kPer;
+          wv[u] = live ? w : 0.f;
           if (live) {
             if constexpr (kPer == 4) {
               const float4 f = __ldcg(reinterpret_cast<const float4*>(p));
@@ -1172,27 +1202,28 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
           live &= live - 1;
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < kAhead; ++u)
 #pragma unroll
           for (int i = 0; i < kPer; ++i) acc[i] = fmaf(v[u][i], wv[u], acc[i]);
       }
     }
-  }
-  // l > 0 wherever a key has weight; NaN stays NaN
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* out = a.output + static_cast<int64_t>(t) * a.o_token + static_cast<int64_t>(qh) * a.o_head + lane * kPer;
-  uint32_t packed[kPer / 2];
+    // l > 0 wherever a key has weight; NaN stays NaN
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t qh = static_cast<int64_t>(h) * a.group + g;
+    uint16_t* out = a.output + static_cast<int64_t>(t) * a.o_token + qh * a.o_head + lane * kPer;
+    uint32_t packed[kPer / 2];
 #pragma unroll
-  for (int i = 0; i < kPer / 2; ++i) packed[i] = pack2<QT>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-  if (a.o_vec) {
-    if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(packed[0], packed[1]);
-    else *reinterpret_cast<uint32_t*>(out) = packed[0];
-  } else {
+    for (int i = 0; i < kPer / 2; ++i) packed[i] = pack2<QT>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    if (a.o_vec) {
+      if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(packed[0], packed[1]);
+      else *reinterpret_cast<uint32_t*>(out) = packed[0];
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) out[i] = static_cast<uint16_t>(packed[i / 2] >> (16 * (i & 1)));
+      for (int i = 0; i < kPer; ++i) out[i] = static_cast<uint16_t>(packed[i / 2] >> (16 * (i & 1)));
+    }
+    if (a.lse && lane == 0)
+      a.lse[static_cast<int64_t>(t) * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
   }
-  if (a.lse && lane == 0)
-    a.lse[static_cast<int64_t>(t) * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
 }  // namespace origami
