@@ -45,8 +45,14 @@ namespace spa {
 
 constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12 / 14: products of
                                 // stream 0 / 1; 13: scheduler
+// Registers per thread at launch, then of the softmax warpgroups and of the others:
+// 256 * 168 + 256 * 88 = 512 * 128, all that the block was launched with.
+constexpr int kRegsLaunch = 128, kRegsSoftmax = 168, kRegsOther = 88;
+static_assert(256 * (kRegsSoftmax + kRegsOther) <= kThreadsS * kRegsLaunch, "register shares");
 constexpr int kTile = 128;      // keys per tile, rows per row tile
 constexpr int kHalf = 64;       // keys per softmax step
+// Of 8 pairs of exponentials, those taken by the FMA pipe (ex2_poly); the others by ex2, of which an SM has 16 a clock.
+constexpr int kPolyPairs = 0;
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of a segment.
 constexpr int kCostTile = 8, kCostPair = 13, kCostItem = 6;
 
@@ -382,14 +388,8 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A warp's bounded wait, agreed by its lanes, that gives up early when another role has: 2 s,
-// far beyond any copy or product. The ready barrier costs one poll and one vote.
-constexpr uint64_t kWaitNs = 2000000000ull;
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
-  return t;
-}
+// A warp's bounded wait, agreed by its lanes, that gives up early when another role has. The
+// ready barrier costs one poll and one vote; the loop is kept short, as every role has several.
 __device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -399,19 +399,14 @@ __device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
       : "memory");
   return __all_sync(0xffffffffu, done != 0) != 0;
 }
-__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  const uint64_t begin = now_ns();
-  for (uint32_t i = 1;; ++i) {
-    if (poll(bar, parity)) return true;
-    if ((i & 63u) == 0 && __any_sync(0xffffffffu, *abort != 0 || now_ns() - begin > kWaitNs)) {
-      *abort = 1;
-      return false;
-    }
-  }
-}
-// The loop is kept out of line: the roles' code has to stay in the instruction caches.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return poll(bar, parity) || wait_long(bar, parity, abort);
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWaitPolls; ++i) {
+    if (poll(bar, parity)) return true;
+    if (__any_sync(0xffffffffu, *abort)) return false;
+  }
+  *abort = 1;
+  return false;
 }
 
 // One arrival for a warp (arrivals of single lanes on one barrier would queue up).
@@ -442,12 +437,14 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
   return static_cast<uint32_t>((c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// TMA: a box of the cache's token rows from row z, one head, 64 dims from x.
-__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int z, uint64_t* bar) {
+// TMA: a box of the cache's token rows from row z, one head, 64 dims from x; the elected thread's
+// (lanes that each issue their own take 65 clocks a box, an elected one 18).
+__device__ __forceinline__ void tma_rows(uint32_t lead, uint32_t dst, const CUtensorMap* map, int x, int head, int z, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"
+      " @q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n}\n" ::"r"(
           dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(z), "r"(smem_u32(bar))
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(z), "r"(smem_u32(bar)), "r"(lead)
       : "memory");
 }
 __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
@@ -472,6 +469,34 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// 2^x of two floats on the FMA pipe: x = n + f with n the nearest integer (the magic addend
+// leaves n in the low bits), a degree-5 polynomial of f on [-1/2, 1/2] fitted for the least
+// greatest relative error (2^-22 as evaluated, about ex2.approx's), and n added to the exponent.
+// Below 2^-125 it stays at that; NaN stays NaN.
+constexpr float kE0 = 1.000000119e+00f, kE1 = 6.931469440e-01f, kE2 = 2.402212024e-01f, kE3 = 5.550713092e-02f,
+                kE4 = 9.675540961e-03f, kE5 = 1.327647245e-03f;
+__device__ __forceinline__ void ex2_poly(uint64_t x, float& y0, float& y1) {
+  float x0, x1;
+  split2(x, x0, x1);
+  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(x0));  // -125
+  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(x1));
+  x = pair2(x0, x1);
+  const uint64_t magic = pair2(12582912.f, 12582912.f);  // 1.5 * 2^23
+  const uint64_t t = add2(x, magic);
+  const uint64_t f = add2(x, fma2(t, pair2(-1.f, -1.f), magic));
+  uint64_t p = pair2(kE5, kE5);
+  p = fma2(p, f, pair2(kE4, kE4));
+  p = fma2(p, f, pair2(kE3, kE3));
+  p = fma2(p, f, pair2(kE2, kE2));
+  p = fma2(p, f, pair2(kE1, kE1));
+  p = fma2(p, f, pair2(kE0, kE0));
+  float t0, t1;
+  split2(t, t0, t1);
+  split2(p, y0, y1);
+  y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
+  y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
 }
 
 // A stream's barriers: S begins anew only when every warp has read the last (s_empty), and P's
@@ -620,9 +645,11 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   if (warp >= 8 && warp < 12) {
     // ---------------------------------------------------------------- loaders
     // Warp lw fills rows 32 lw .. 32 lw + 31 of every tile; lane l knows row 32 lw + l.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
     constexpr int kChunks = D / 8;          // 16-byte chunks per row
     constexpr int kRowsPer = 32 / kChunks;  // rows a warp copies at once
-    const int lw = warp - 8;
+    const int lw = __shfl_sync(0xffffffffu, warp - 8, 0);
+    const uint32_t lead = elect_one();
     const int sub = lane / kChunks, chunk = lane % kChunks;
     // this lane's chunk of row 32 lw + sub; kRowsPer rows on, the row's swizzle changes
     const uint32_t base = smem_u32(sm);
@@ -658,6 +685,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->seg_empty[slot % kSegments]);
       if (seg.n == 0) break;
+      const int head = __shfl_sync(0xffffffffu, seg.h, 0);
       const int32_t* table = seg.b < 0 ? a.prefix_blocks : a.suffix_blocks + seg.b * a.suffix_stride;
       // cache row of key `key`, negative past the end of the item or outside the cache
       auto row_of = [&](int key) -> int {
@@ -724,30 +752,31 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             ok = false;
             break;
           }
-          const uint32_t dst = base + S::ring + st * S::tile;
+          const uint32_t dst = base + S::ring + st * S::tile + lw * (32 * 128);  // this warp's rows
           if (tma) {
-            if (lane == 0) expect_tx(&bars->full[st], 32 * D * 2);
+            if (lead) expect_tx(&bars->full[st], 32 * D * 2);
             __syncwarp();
-            if ((lane & (a.tma_rows - 1)) == 0) {
-              const int z = row < 0 ? a.all_rows : row + which * a.v_rows;  // past the last row: zeros
+            const int z = row < 0 ? a.all_rows : row + which * a.v_rows;  // past the last row: zeros
+#pragma unroll 1
+            for (int r = 0; r < 32; r += a.tma_rows) {
+              const int zr = __shfl_sync(0xffffffffu, z, r);
 #pragma unroll
               for (int x = 0; x < D; x += 64)
-                tma_rows(dst + (x >> 6) * (kTile * 128) + (32 * lw + lane) * 128, &a.map, x, seg.h, z, &bars->full[st]);
+                tma_rows(lead, dst + (x >> 6) * (kTile * 128) + r * 128, &a.map, x, head, zr, &bars->full[st]);
             }
-            __syncwarp();
           } else {
             const uint16_t* src = a.cache + which * a.kv_stride + static_cast<int64_t>(seg.h) * D + chunk * 8;
 #pragma unroll 4
             for (int j = 0; j < 32 / kRowsPer; ++j) {
               const int r = j * kRowsPer + sub;
               const int cr = __shfl_sync(0xffffffffu, row, r);
-              cp16_or_zero(dst + chunk_off(32 * lw + r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
+              cp16_or_zero(dst + chunk_off(r, chunk), src + (cr < 0 ? 0 : cr) * a.row_elems, cr >= 0);
             }
           }
           asm volatile("cp.async.commit_group;\n" ::: "memory");
           ++ring;
           if (tma && !q_pending && signalled + 1 == ring) {
-            if (lane == 0) mbar_arrive(&bars->full[st]);
+            if (lead) mbar_arrive(&bars->full[st]);
             signalled = ring;
           } else if (ring - signalled > S::lag) {
             asm volatile("cp.async.wait_group %0;\n" ::"n"(S::lag) : "memory");
@@ -764,6 +793,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       for (uint32_t i = ring > S::stages ? ring - S::stages : 0; i < ring; ++i)
         mbar_wait_bounded(&bars->full[i % S::stages], (i / S::stages) & 1u, 1u << 16);
   } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
     if (warp == 13) {
       // -------------------------------------------------------------- scheduler
       const Deal deal = *deal_sm;
@@ -899,6 +929,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax of stream s
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax));
     const int s = warp >> 2;
     const int row = tid & (kTile - 1);
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -934,7 +965,8 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           ld64(ts, x);
           tc_fence_before();
           arrive_warp(&bars->s_empty[s]);
-          if (!__all_sync(0xffffffffu, lim >= kHalf || row >= rows)) {
+          const bool masked = !__all_sync(0xffffffffu, lim >= kHalf || row >= rows);
+          if (masked) {
 #pragma unroll
             for (int j = 0; j < kHalf; ++j)
               if (j >= lim) x[j] = 0xFF800000u;  // -inf: not seen
@@ -981,11 +1013,20 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             uint32_t p[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
+              const uint64_t arg =
+                  fma2(pair2(__uint_as_float(x[32 * q + 2 * j]), __uint_as_float(x[32 * q + 2 * j + 1])), scale2, neg2);
               float p0, p1;
-              split2(fma2(pair2(__uint_as_float(x[32 * q + 2 * j]), __uint_as_float(x[32 * q + 2 * j + 1])), scale2, neg2),
-                     p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
+              if ((j & 7) < kPolyPairs) {
+                ex2_poly(arg, p0, p1);
+                if (masked) {  // exactly nothing
+                  if (32 * q + 2 * j >= lim) p0 = 0.f;
+                  if (32 * q + 2 * j + 1 >= lim) p1 = 0.f;
+                }
+              } else {
+                split2(arg, p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+              }
               sum[j & 3] = add2(sum[j & 3], pair2(p0, p1));
               p[j] = pack2<QT>(p0, p1);
             }
