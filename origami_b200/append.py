@@ -21,85 +21,110 @@ import ctypes
 import torch
 
 from origami_b200 import _lib
-from origami_b200.layer import _stream_handle, paged_desc
+from origami_b200.layer import paged_desc
 
 _DTYPE = {torch.float16: _lib.ORIGAMI_DTYPE_F16, torch.bfloat16: _lib.ORIGAMI_DTYPE_BF16,
           torch.float32: _lib.ORIGAMI_DTYPE_F32}
 
 
-def _on(device: torch.device, t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda or t.device != device:
+def _device_index(t: torch.Tensor, name: str) -> int:
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return index
+
+
+def _on(index: int, t: torch.Tensor, name: str) -> None:
+    if t.get_device() != index:
         raise ValueError(f"{name} must be a CUDA tensor on the device of the others")
 
 
-def _rows(t: torch.Tensor, name: str, tokens: int, head_dim: int, device: torch.device) -> _lib.HeadRows:
-    _on(device, t, name)
-    if t.dim() != 3 or int(t.shape[0]) != tokens or int(t.shape[2]) != head_dim:
-        raise ValueError(f"{name} must have shape [{tokens}, heads, {head_dim}], got {tuple(t.shape)}")
-    if t.dtype not in _DTYPE:
+def _rows(t: torch.Tensor, name: str, tokens: int, head_dim: int, index: int) -> _lib.HeadRows:
+    _on(index, t, name)
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim:
+        raise ValueError(f"{name} must have shape [{tokens}, heads, {head_dim}], got {tuple(shape)}")
+    dtype = _DTYPE.get(t.dtype)
+    if dtype is None:
         raise ValueError(f"{name} must be float16, bfloat16 or float32")
-    if head_dim > 1 and t.stride(2) != 1:
+    token_stride, head_stride, stride = t.stride()
+    if stride != 1 and head_dim > 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
-    return _lib.HeadRows(t.data_ptr(), _DTYPE[t.dtype], int(t.shape[1]), int(t.stride(0)), int(t.stride(1)))
+    return _lib.HeadRows(t.data_ptr(), dtype, shape[1], token_stride, head_stride)
 
 
-def _index(t: torch.Tensor, name: str, tokens: int, device: torch.device) -> int:
+def _index(t: torch.Tensor, name: str, tokens: int, index: int) -> int:
     """Bytes per element of a contiguous int32 / int64 vector of one entry per token."""
-    _on(device, t, name)
-    if t.dtype not in (torch.int32, torch.int64):
+    _on(index, t, name)
+    if t.dtype is not torch.int32 and t.dtype is not torch.int64:
         raise ValueError(f"{name} must be int32 or int64")
-    if t.dim() != 1 or int(t.shape[0]) != tokens or not t.is_contiguous():
+    if t.dim() != 1 or t.shape[0] != tokens or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous vector of {tokens} entries, one per token")
     return t.element_size()
 
 
-def _rotation(positions: torch.Tensor | None, cos_sin: torch.Tensor | None, interleaved: bool, tokens: int,
-              device: torch.device):
+def _rotation(positions: torch.Tensor | None, cos_sin: torch.Tensor | None, interleaved: bool, tokens: int, index: int):
     if positions is None and cos_sin is None:
         return None
     if positions is None or cos_sin is None:
         raise ValueError("positions and cos_sin go together")
-    width = _index(positions, "positions", tokens, device)
-    _on(device, cos_sin, "cos_sin")
-    if cos_sin.dim() != 2 or cos_sin.dtype not in _DTYPE:
+    width = _index(positions, "positions", tokens, index)
+    _on(index, cos_sin, "cos_sin")
+    dtype = _DTYPE.get(cos_sin.dtype)
+    if cos_sin.dim() != 2 or dtype is None:
         raise ValueError("cos_sin must be a float16, bfloat16 or float32 matrix [max_positions, rotated dims]")
-    if cos_sin.shape[1] > 1 and cos_sin.stride(1) != 1:
+    rows, dims = cos_sin.shape
+    row_stride, stride = cos_sin.stride()
+    if dims > 1 and stride != 1:
         raise ValueError("cos_sin must be contiguous in its last dimension")
     # a table of one row has no row stride to speak of
-    stride = int(cos_sin.stride(0)) if cos_sin.shape[0] > 1 else int(cos_sin.shape[1])
-    return _lib.Rotation(cos_sin.data_ptr(), _DTYPE[cos_sin.dtype], int(bool(interleaved)), int(cos_sin.shape[0]),
-                         int(cos_sin.shape[1]), stride, positions.data_ptr(), width)
+    return _lib.Rotation(cos_sin.data_ptr(), dtype, 1 if interleaved else 0, rows, dims, row_stride if rows > 1 else dims,
+                         positions.data_ptr(), width)
 
 
-def _norm(query_weight: torch.Tensor | None, key_weight: torch.Tensor | None, eps: float, head_dim: int,
-          device: torch.device):
+def _norm(query_weight: torch.Tensor | None, key_weight: torch.Tensor | None, eps: float, head_dim: int, index: int):
     if query_weight is None and key_weight is None:
         return None
     n = _lib.HeadNorm(None, None, 0, 0, float(eps))
     for w, name in ((query_weight, "query_weight"), (key_weight, "key_weight")):
         if w is None:
             continue
-        _on(device, w, name)
-        if w.dtype not in _DTYPE or tuple(w.shape) != (head_dim,) or not w.is_contiguous():
+        _on(index, w, name)
+        if w.dtype not in _DTYPE or w.dim() != 1 or w.shape[0] != head_dim or not w.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float16, bfloat16 or float32 vector of {head_dim} elements")
         setattr(n, f"d_{name}", w.data_ptr())
         setattr(n, f"{name}_dtype", _DTYPE[w.dtype])
     return n
 
 
-def _error(error_count: torch.Tensor | None, device: torch.device):
+def _error(error_count: torch.Tensor | None, index: int):
     if error_count is None:
         return None
-    _on(device, error_count, "error_count")
+    _on(index, error_count, "error_count")
     if error_count.dtype not in (torch.int32, torch.uint32) or error_count.numel() < 1:
         raise ValueError("error_count must be an int32 tensor of one element")
     return error_count.data_ptr()
 
 
-def _alloc_like(t: torch.Tensor, stream: torch.cuda.Stream | None, device: torch.device) -> torch.Tensor:
-    """A contiguous tensor of t's shape from the pool of the stream that will write it."""
-    with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device)):
-        return torch.empty(t.shape, dtype=t.dtype, device=device)
+def _empty(like: torch.Tensor, shape, dtype: torch.dtype, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """A contiguous tensor on like's device, from the pool of the stream that will write it."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _launch(index: int, stream: torch.cuda.Stream | None, what: str, entry, *args) -> None:
+    """Calls a library entry point on the tensors' device with the stream's handle last."""
+    if stream is not None and stream.device_index != index:
+        raise ValueError("stream must be a stream of the tensors' device")
+    handle = torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
+    if torch._C._cuda_getDevice() == index:
+        rc = entry(*args, handle)
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, handle)
+    _lib.check(rc, what)
 
 
 def _ref(struct):
@@ -115,27 +140,26 @@ def norm_rope(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, c
 
     query and key may be strided slices of one projection's output; query_out / key_out may
     be query / key themselves (in place). Returns (query_out, key_out)."""
-    device = query.device
+    index = _device_index(query, "query")
     if query.dim() != 3:
         raise ValueError(f"query must have shape [tokens, heads, head_dim], got {tuple(query.shape)}")
-    tokens, head_dim = int(query.shape[0]), int(query.shape[2])
-    q = _rows(query, "query", tokens, head_dim, device)
-    k = _rows(key, "key", tokens, head_dim, device)
+    tokens, _, head_dim = query.shape
+    q = _rows(query, "query", tokens, head_dim, index)
+    k = _rows(key, "key", tokens, head_dim, index)
     if positions is None or cos_sin is None:
         raise ValueError("norm_rope needs positions and cos_sin")
-    rot = _rotation(positions, cos_sin, interleaved, tokens, device)
-    norm = _norm(query_weight, key_weight, eps, head_dim, device)
-    err = _error(error_count, device)
-    query_out = _alloc_like(query, stream, device) if query_out is None else query_out
-    key_out = _alloc_like(key, stream, device) if key_out is None else key_out
-    qo = _rows(query_out, "query_out", tokens, head_dim, device)
-    ko = _rows(key_out, "key_out", tokens, head_dim, device)
-    if tokens == 0:
-        return query_out, key_out
-    with torch.cuda.device(device):
-        rc = _lib.lib().origami_norm_rope(ctypes.byref(q), ctypes.byref(qo), ctypes.byref(k), ctypes.byref(ko), tokens,
-                                          head_dim, _ref(rot), _ref(norm), err, _stream_handle(stream, device))
-    _lib.check(rc, "origami_norm_rope")
+    rot = _rotation(positions, cos_sin, interleaved, tokens, index)
+    norm = _norm(query_weight, key_weight, eps, head_dim, index)
+    err = _error(error_count, index)
+    if query_out is None:
+        query_out = _empty(query, query.shape, query.dtype, stream)
+    if key_out is None:
+        key_out = _empty(key, key.shape, key.dtype, stream)
+    qo = _rows(query_out, "query_out", tokens, head_dim, index)
+    ko = _rows(key_out, "key_out", tokens, head_dim, index)
+    if tokens > 0:
+        _launch(index, stream, "origami_norm_rope", _lib.lib().origami_norm_rope, ctypes.byref(q), ctypes.byref(qo),
+                ctypes.byref(k), ctypes.byref(ko), tokens, head_dim, _ref(rot), _ref(norm), err)
     return query_out, key_out
 
 
@@ -152,29 +176,27 @@ def append_kv(kv_layer: torch.Tensor, key: torch.Tensor, value: torch.Tensor, sl
     key, value and query share a type (bf16, fp16 or fp32). A token with slot -1 gets no
     cache row; its query is still written. Slots must differ from one another. query_out may
     be query itself."""
-    device = kv_layer.device
+    index = _device_index(kv_layer, "the paged KV cache")
     desc = paged_desc(kv_layer)
-    if kv_layer.dtype not in (torch.float16, torch.bfloat16):
+    cache_dtype = _DTYPE.get(kv_layer.dtype)
+    if cache_dtype is None:
         raise ValueError("the paged KV cache must be float16 or bfloat16")
-    tokens, head_dim = int(key.shape[0]), int(desc.head_dim)
-    k = _rows(key, "key", tokens, head_dim, device)
-    v = _rows(value, "value", tokens, head_dim, device)
-    width = _index(slots, "slots", tokens, device)
-    rot = _rotation(positions, cos_sin, interleaved, tokens, device)
-    norm = _norm(query_weight, key_weight, eps, head_dim, device)
-    err = _error(error_count, device)
+    tokens, head_dim = key.shape[0], desc.head_dim
+    k = _rows(key, "key", tokens, head_dim, index)
+    v = _rows(value, "value", tokens, head_dim, index)
+    width = _index(slots, "slots", tokens, index)
+    rot = _rotation(positions, cos_sin, interleaved, tokens, index)
+    norm = _norm(query_weight, key_weight, eps, head_dim, index)
+    err = _error(error_count, index)
     q = qo = None
     if query is not None:
-        q = _rows(query, "query", tokens, head_dim, device)
-        query_out = _alloc_like(query, stream, device) if query_out is None else query_out
-        qo = _rows(query_out, "query_out", tokens, head_dim, device)
+        q = _rows(query, "query", tokens, head_dim, index)
+        if query_out is None:
+            query_out = _empty(query, query.shape, query.dtype, stream)
+        qo = _rows(query_out, "query_out", tokens, head_dim, index)
     elif query_out is not None or query_weight is not None:
         raise ValueError("query_out and query_weight need a query")
-    if tokens == 0:
-        return query_out
-    with torch.cuda.device(device):
-        rc = _lib.lib().origami_append_kv(ctypes.byref(k), ctypes.byref(v), _ref(q), _ref(qo), ctypes.byref(desc),
-                                          _DTYPE[kv_layer.dtype], slots.data_ptr(), width, tokens, _ref(rot),
-                                          _ref(norm), err, _stream_handle(stream, device))
-    _lib.check(rc, "origami_append_kv")
+    if tokens > 0:
+        _launch(index, stream, "origami_append_kv", _lib.lib().origami_append_kv, ctypes.byref(k), ctypes.byref(v), _ref(q),
+                _ref(qo), ctypes.byref(desc), cache_dtype, slots.data_ptr(), width, tokens, _ref(rot), _ref(norm), err)
     return query_out

@@ -18,26 +18,29 @@ import ctypes
 import torch
 
 from origami_b200 import _lib
-from origami_b200.append import _DTYPE, _error, _on, _rows
-from origami_b200.layer import _stream_handle, paged_desc
+from origami_b200.append import _DTYPE, _device_index, _empty, _error, _launch, _on, _rows
+from origami_b200.layer import paged_desc
 
 
 def workspace_bytes(tokens: int, query_heads: int, kv_heads: int, head_dim: int, requests: int,
-                    device: torch.device | None = None) -> int:
+                    device: torch.device | int | None = None) -> int:
     """Workspace the kernels need for these shapes on `device`."""
-    out = ctypes.c_int64(0)
-    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
-        rc = _lib.lib().origami_shared_prefix_attention_workspace(int(tokens), int(query_heads), int(kv_heads),
-                                                                  int(head_dim), int(requests), ctypes.byref(out))
+    entry, out = _lib.lib().origami_shared_prefix_attention_workspace, ctypes.c_int64(0)
+    args = (tokens, query_heads, kv_heads, head_dim, requests, ctypes.byref(out))
+    if device is None or device == torch.cuda.current_device():
+        rc = entry(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args)
     _lib.check(rc, "origami_shared_prefix_attention_workspace")
-    return int(out.value)
+    return out.value
 
 
-def _ints(t: torch.Tensor, name: str, dims: int, device: torch.device) -> None:
-    _on(device, t, name)
-    if t.dtype != torch.int32 or t.dim() != dims:
+def _ints(t: torch.Tensor, name: str, dims: int, index: int) -> None:
+    _on(index, t, name)
+    if t.dtype is not torch.int32 or t.dim() != dims:
         raise ValueError(f"{name} must be an int32 tensor of {dims} dimension{'s' if dims > 1 else ''}")
-    if t.numel() > 1 and t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
 
 
@@ -63,43 +66,41 @@ def shared_prefix_attention(query: torch.Tensor, kv_layer: torch.Tensor, query_s
     workspace: a uint8 tensor of workspace_bytes(...) bytes, allocated per call when omitted;
     calls that share one must not overlap. error_flags (int32): bit 31 is set if a bounded
     wait inside the kernel ran out."""
-    device = query.device
+    index = _device_index(query, "query")
     if query.dim() != 3:
         raise ValueError(f"query must have shape [tokens, heads, head_dim], got {tuple(query.shape)}")
-    tokens, heads, head_dim = (int(x) for x in query.shape)
-    q = _rows(query, "query", tokens, head_dim, device)
+    tokens, heads, head_dim = query.shape
+    q = _rows(query, "query", tokens, head_dim, index)
+    _on(index, kv_layer, "the paged KV cache")
     desc = paged_desc(kv_layer)
-    _on(device, kv_layer, "the paged KV cache")
-    if kv_layer.dtype not in (torch.float16, torch.bfloat16):
+    cache_dtype = _DTYPE.get(kv_layer.dtype)
+    if cache_dtype is None:
         raise ValueError("the paged KV cache must be float16 or bfloat16")
-    _ints(query_start, "query_start", 1, device)
-    _ints(prefix_blocks, "prefix_blocks", 1, device)
-    _ints(suffix_blocks, "suffix_blocks", 2, device)
-    _ints(suffix_lens, "suffix_lens", 1, device)
-    requests, width = (int(x) for x in suffix_blocks.shape)
-    if int(suffix_lens.shape[0]) != requests or int(query_start.shape[0]) != requests + 1:
+    _ints(query_start, "query_start", 1, index)
+    _ints(prefix_blocks, "prefix_blocks", 1, index)
+    _ints(suffix_blocks, "suffix_blocks", 2, index)
+    _ints(suffix_lens, "suffix_lens", 1, index)
+    requests, width = suffix_blocks.shape
+    if suffix_lens.shape[0] != requests or query_start.shape[0] != requests + 1:
         raise ValueError("suffix_lens needs one entry and query_start one more than suffix_blocks has rows")
     if lse is not None:
-        _on(device, lse, "lse")
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (tokens, heads) or not lse.is_contiguous():
+        _on(index, lse, "lse")
+        if lse.dtype is not torch.float32 or tuple(lse.shape) != (tokens, heads) or not lse.is_contiguous():
             raise ValueError(f"lse must be a contiguous float32 tensor of shape [{tokens}, {heads}]")
-    err = _error(error_flags, device)
-    scale = float(head_dim) ** -0.5 if softmax_scale is None else float(softmax_scale)
-    with torch.cuda.device(device), torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device)):
-        if out is None:
-            out = torch.empty(query.shape, dtype=query.dtype, device=device)
-        o = _rows(out, "out", tokens, head_dim, device)
-        if workspace is None:
-            need = workspace_bytes(tokens, heads, int(desc.num_heads), head_dim, requests, device)
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        _on(device, workspace, "workspace")
-        if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-            raise ValueError("workspace must be a contiguous uint8 tensor")
-        rc = _lib.lib().origami_shared_prefix_attention(
-            ctypes.byref(q), ctypes.byref(o), lse.data_ptr() if lse is not None else None, tokens, head_dim,
-            ctypes.byref(desc), _DTYPE[kv_layer.dtype], prefix_blocks.data_ptr(), int(prefix_blocks.shape[0]),
-            int(prefix_tokens), suffix_blocks.data_ptr(), int(suffix_blocks.stride(0)), width, suffix_lens.data_ptr(),
-            query_start.data_ptr(), requests, scale, workspace.data_ptr(), workspace.numel(), err,
-            _stream_handle(stream, device))
-    _lib.check(rc, "origami_shared_prefix_attention")
+    err = _error(error_flags, index)
+    scale = head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if out is None:
+        out = _empty(query, query.shape, query.dtype, stream)
+    o = _rows(out, "out", tokens, head_dim, index)
+    if workspace is None:
+        need = workspace_bytes(tokens, heads, desc.num_heads, head_dim, requests, index)
+        workspace = _empty(query, (need,), torch.uint8, stream)
+    _on(index, workspace, "workspace")
+    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor")
+    _launch(index, stream, "origami_shared_prefix_attention", _lib.lib().origami_shared_prefix_attention, ctypes.byref(q),
+            ctypes.byref(o), lse.data_ptr() if lse is not None else None, tokens, head_dim, ctypes.byref(desc), cache_dtype,
+            prefix_blocks.data_ptr(), prefix_blocks.shape[0], int(prefix_tokens), suffix_blocks.data_ptr(),
+            suffix_blocks.stride(0), width, suffix_lens.data_ptr(), query_start.data_ptr(), requests, scale,
+            workspace.data_ptr(), workspace.numel(), err)
     return out
