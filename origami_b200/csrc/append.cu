@@ -119,6 +119,7 @@ void set_shared(origami::AppendArgs& a, int64_t tokens, int64_t head_dim, const 
     a.interleaved = rot->interleaved != 0;
   }
   a.eps = norm ? static_cast<float>(norm->eps) : 0.f;
+  a.inv_d = 1.f / static_cast<float>(head_dim);
 }
 
 bool rows16(const origami::HeadRows& r, int64_t es) {
@@ -134,8 +135,7 @@ bool fast_rows(const origami::AppendArgs& a, int64_t es) {
   if (!rows16(a.q, es) || !rows16(a.k, es) || !rows16(a.v, es) || !aligned(a.cache, 16)) return false;
   if (a.positions == nullptr) return true;
   const int64_t ts = dtype_bytes(a.table_dtype);
-  return a.R % (a.interleaved ? 8 : 16) == 0 && aligned(a.table, 16) && (a.table_stride * ts) % 16 == 0 &&
-         (a.R / 2 * ts) % 8 == 0;
+  return a.R % 16 == 0 && aligned(a.table, 16) && (a.table_stride * ts) % 16 == 0;
 }
 
 template <typename TI, typename TC>
@@ -145,19 +145,25 @@ int32_t launch(origami::AppendArgs& a, cudaStream_t st) {
     const int lanes = (a.D / 8 + 1) / 2;
     while ((1 << a.lanes_log2) < lanes) ++a.lanes_log2;
     // One walker per head while that many threads fit the device at once (the step of a few
-    // tokens is bound by latency), else kUnroll heads per walker, all of them in flight.
+    // tokens is bound by latency); else four query heads a walker beside a key and a value
+    // head, all requested at once.
     int sms = 0, dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
-    const int64_t resident = static_cast<int64_t>(sms) * 1024;
-    a.groups = a.tokens * total << a.lanes_log2 <= resident
-                   ? total
-                   : (total + origami::app::kUnroll - 1) / origami::app::kUnroll;
-    const int64_t threads = (a.tokens * a.groups) << a.lanes_log2;
-    const int64_t ctas = (threads + 255) / 256;
-    if (ctas > 0x7FFFFFFF) return fail(ORIGAMI_ERR_UNSUPPORTED, "too many rows");
-    origami::append_rows<TI, TC><<<static_cast<unsigned>(ctas), 256, 0, st>>>(a);
+    const int64_t resident = static_cast<int64_t>(sms) * 512;
+    a.groups = a.tokens * total << a.lanes_log2 <= resident ? total : std::max(a.k.heads, (a.q.heads + 3) / 4);
+    const bool full = a.D == 16 << a.lanes_log2;
+    auto* fn = full ? &origami::append_rows<TI, TC, true> : &origami::append_rows<TI, TC, false>;
+    int slots = 0;
+    const int32_t rc = persistent_slots(reinterpret_cast<const void*>(fn), 0, slots);
+    if (rc) return rc;
+    const int64_t per_cta = 256 >> a.lanes_log2;  // walkers
+    const int64_t needed = (a.tokens * a.groups + per_cta - 1) / per_cta;
+    // as many CTAs as fit at once, but at least one token's walkers; whole tokens per pass
+    const int64_t ctas = std::min(needed, std::max<int64_t>(slots, (a.groups + per_cta - 1) / per_cta));
+    a.step = static_cast<int32_t>(ctas * per_cta / a.groups);
+    fn<<<static_cast<unsigned>(ctas), 256, 0, st>>>(a);
     return after_launch("append_rows launch");
   }
   const int64_t ctas = (a.tokens * total + 7) / 8;

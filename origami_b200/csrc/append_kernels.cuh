@@ -15,13 +15,18 @@
 // a lane holds 16 elements of a head as two 8-element chunks that contain both members of
 // each of its pairs (chunks c and c + R/16 for halves, 2c and 2c + 1 interleaved), so the
 // rotation needs no exchange between lanes, the norm is log2(lanes per head) shuffles, and
-// the 8 (cos, sin) a lane needs are loaded once for all the heads it walks of its token.
+// the 8 (cos, sin) and the weights a lane needs are loaded once for all the heads it walks of
+// its token. A walker's key and value rows and its first query rows are all requested before
+// the first is used.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace origami {
 
@@ -48,13 +53,16 @@ struct AppendArgs {
   int32_t D, R, interleaved, table_dtype, slots64, positions64;
   int32_t lanes_log2;  // lanes per head (fast kernel)
   int32_t groups;      // head walkers per token (fast kernel)
-  float eps;
+  int32_t step;        // tokens from one of a walker's to the next
+  float eps, inv_d;
 };
 
 namespace app {
 
 constexpr int kF16 = 1, kBF16 = 2, kF32 = 3;
-constexpr int kUnroll = 4;  // heads a lane has in flight
+// Query heads a lane has in flight (beside a key and a value head).
+template <typename T>
+__host__ __device__ constexpr int unroll() { return sizeof(T) == 4 ? 1 : 2; }
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -90,18 +98,51 @@ __device__ __forceinline__ void store8(T* p, const Raw8<T>& r) {
   *reinterpret_cast<uint4*>(p) = r.w[0];
   if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p + 4) = r.w[1];
 }
+// Words of two 16-bit elements to and from floats.
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xFFFF0000u);
+  } else {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = h.x;
+    hi = h.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
 template <typename T>
 __device__ __forceinline__ void unpack8(const Raw8<T>& r, float* f) {
-  const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = to_f<T>(e[i]);
+  for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k) {
+    const uint32_t w[4] = {r.w[k].x, r.w[k].y, r.w[k].z, r.w[k].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) f[4 * k + i] = __uint_as_float(w[i]);
+      else unpack2<T>(w[i], f[2 * i], f[2 * i + 1]);
+    }
+  }
 }
 template <typename T>
 __device__ __forceinline__ Raw8<T> pack8(const float* f) {
   Raw8<T> r;
-  T* e = reinterpret_cast<T*>(&r);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_f<T>(f[i]);
+    for (int k = 0; k < 2; ++k)
+      r.w[k] = make_uint4(__float_as_uint(f[4 * k]), __float_as_uint(f[4 * k + 1]), __float_as_uint(f[4 * k + 2]),
+                          __float_as_uint(f[4 * k + 3]));
+  } else {
+    r.w[0] = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+  }
   return r;
 }
 
@@ -139,8 +180,11 @@ __device__ __forceinline__ int64_t index_at(const void* p, int wide, int64_t i) 
   return wide ? __ldg(static_cast<const long long*>(p) + i) : __ldg(static_cast<const int*>(p) + i);
 }
 
-__device__ __forceinline__ float inv_rms(float sum, int D, float eps) {
-  return __frcp_rn(__fsqrt_rn(sum / static_cast<float>(D) + eps));
+// 1 / sqrt(sum / D + eps): rsqrt and one Newton step (within an ulp or two; 0 and infinity as they are).
+__device__ __forceinline__ float inv_rms(float sum, float inv_d, float eps) {
+  const float x = fmaf(sum, inv_d, eps), r = rsqrtf(x);
+  const float n = fmaf(r * 0.5f, fmaf(-x * r, r, 1.f), r);
+  return x > 0.f && x < INFINITY ? n : r;
 }
 
 // A token's place: its cache row (-1: none), whether its position lies in the table, and the
@@ -161,7 +205,12 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int64_t t, uint32
     p.rotates = p.position >= 0 && p.position < a.max_positions;
   }
   if (in_cache)
-    p.cache_row = (slot / a.block_size) * a.block_stride + (slot % a.block_size) * a.token_stride;
+  {
+    int64_t block;
+    if (((slot | a.block_size) >> 31) == 0) block = static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.block_size);
+    else block = slot / a.block_size;
+    p.cache_row = block * a.block_stride + (slot - block * a.block_size) * a.token_stride;
+  }
   // slot -1 asks for no cache row; any other slot outside the cache is an error
   if (a.slots && !in_cache && slot != -1) skipped += static_cast<uint32_t>(a.k.heads + a.v.heads);
   if (!p.rotates) {
@@ -173,123 +222,155 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int64_t t, uint32
 
 }  // namespace app
 
-// Fast kernel: D % 8 == 0, 16-byte rows, R % 16 == 0 (halves) or R % 8 == 0 (interleaved).
-// 1 << lanes_log2 lanes per head; `groups` such walkers share a token's heads (query heads,
-// then key heads, then value heads), kUnroll heads in flight each.
-template <typename TI, typename TC>
-__global__ void __launch_bounds__(256) append_rows(const __grid_constant__ AppendArgs a) {
+// Fast kernel: D % 8 == 0, 16-byte rows, R % 16 == 0. 1 << lanes_log2 lanes per head; `groups`
+// such walkers share a token's heads: walker g takes its part of the query heads, key head g
+// and value head groups - 1 - g; or, in a step of few tokens (groups = all heads), one head.
+// A walker keeps its g and steps through the tokens, so that all but the rows, the position
+// and the slot is set up once (the weights in shared memory, in fp32). FULL: every lane has
+// both chunks (D is 16 << lanes_log2).
+template <typename TI, typename TC, bool FULL>
+__global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ AppendArgs a) {
   using namespace app;
+  constexpr int U = unroll<TI>();
+  __shared__ __align__(16) float w_sm[2][512];
   const int lph = 1 << a.lanes_log2;
   const int lane = threadIdx.x & (lph - 1);
-  const int64_t walker = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lanes_log2;
-  const int64_t t = walker / a.groups;
-  const int g = static_cast<int>(walker - t * a.groups);
-  const bool live = t < a.tokens;
-  const int total = a.q.heads + a.k.heads + a.v.heads;
+  const int walker = static_cast<int>((blockIdx.x * blockDim.x + threadIdx.x) >> a.lanes_log2);
+  const int first = walker / a.groups, g = walker - first * a.groups;
+  // this walker's heads
+  const bool single = a.groups == a.q.heads + a.k.heads + a.v.heads;
+  const int kh = single ? g - a.q.heads : g;
+  const int vh = single ? g - a.q.heads - a.k.heads : a.groups - 1 - g;
+  const bool has_k = kh >= 0 && kh < a.k.heads, has_v = vh >= 0 && vh < a.v.heads;
+  const int q_per = single ? (a.q.heads > 0 ? 1 : 0) : (a.q.heads + a.groups - 1) / a.groups;
+  const int q0 = single ? g : g * q_per, q1 = min(q0 + q_per, a.q.heads);
 
-  Place pl{-1, 0, false};
-  if (live) {
-    uint32_t skipped;
-    pl = place_of(a, t, skipped);
-    if (skipped && g == 0 && lane == 0 && a.err) atomicAdd(a.err, skipped);
-  }
-  // this lane's two chunks; nchunks may be odd (the last lane then has one)
-  const int nchunks = a.D >> 3;
+  // this lane's two chunks; D / 8 may be odd (the last lane then has one)
   const bool split = !a.interleaved && lane < (a.R >> 4);
-  const int c0 = split ? lane : 2 * lane;
-  const int c1 = split ? lane + (a.R >> 4) : 2 * lane + 1;
-  const bool has0 = c0 < nchunks, has1 = c1 < nchunks;
-  // pairs 8*lane .. 8*lane+7 in both arrangements; the first four and last four may differ
-  // in whether they turn (interleaved with R % 16 == 8)
-  const bool turn0 = a.positions && (a.interleaved ? 8 * c0 < a.R : split);
-  const bool turn1 = a.positions && (a.interleaved ? 8 * c1 < a.R : split);
+  const int e0 = 8 * (split ? lane : 2 * lane), e1 = 8 * (split ? lane + (a.R >> 4) : 2 * lane + 1);
+  const bool has0 = FULL || e0 < a.D, has1 = FULL || e1 < a.D;
+  // pairs 8 lane .. 8 lane + 7 in both arrangements
+  const bool turns = a.positions && 16 * lane < a.R;
+  const int64_t k_in = (has_k ? kh : 0) * a.k.in_head, v_in = (has_v ? vh : 0) * a.v.in_head;
+  const int64_t q_last = a.q.heads - 1;
+  for (int i = threadIdx.x; i < a.D; i += blockDim.x) {
+    if (a.q.weight) w_sm[0][i] = small_at(a.q.weight, a.q.weight_dtype, i);
+    if (a.k.weight) w_sm[1][i] = small_at(a.k.weight, a.k.weight_dtype, i);
+  }
+  __syncthreads();
+  auto fetch = [&](const void* in, int64_t at, Raw8<TI> (&x)[2]) {
+    const TI* p = static_cast<const TI*>(in) + at;
+    if (!FULL) x[0] = x[1] = Raw8<TI>{};
+    if (has0) x[0] = load8(p + e0);
+    if (has1) x[1] = load8(p + e1);
+  };
+  auto put = [&](auto* o, const float (&f)[16]) {
+    using T = std::remove_reference_t<decltype(*o)>;
+    if (has0) store8(o + e0, pack8<T>(f));
+    if (has1) store8(o + e1, pack8<T>(f + 8));
+  };
   float co[8], si[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) co[i] = 1.f, si[i] = 0.f;
-  if (live && pl.rotates && turn0) {
-    const int64_t row = pl.position * a.table_stride + 8 * lane;
-    if (turn1) {
-      small8(a.table, a.table_dtype, row, co);
-      small8(a.table, a.table_dtype, row + (a.R >> 1), si);
+  // norm and rotation of one head's 16 elements (the whole warp takes part in the shuffles)
+  auto turn = [&](const float* w, bool norm, const Raw8<TI> (&x)[2], float (&f)[16]) {
+    unpack8(x[0], f);
+    unpack8(x[1], f + 8);
+    if (norm) {
+      uint64_t s2 = 0ull, s3 = 0ull;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        s2 = fma2(pair2(f[i], f[i + 1]), pair2(f[i], f[i + 1]), s2);
+        s3 = fma2(pair2(f[i + 8], f[i + 9]), pair2(f[i + 8], f[i + 9]), s3);
+      }
+      float s0, s1;
+      split2(add2(s2, s3), s0, s1);
+      float s = s0 + s1;
+#pragma unroll 1
+      for (int o = lph >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      const float inv = inv_rms(s, a.inv_d, a.eps);
+      const uint64_t inv2 = pair2(inv, inv);
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        if (i < 8 ? has0 : has1) {
+          const float4 v = *reinterpret_cast<const float4*>(w + (i < 8 ? e0 + i : e1 + i - 8));
+          split2(mul2(mul2(pair2(f[i], f[i + 1]), inv2), pair2(v.x, v.y)), f[i], f[i + 1]);
+          split2(mul2(mul2(pair2(f[i + 2], f[i + 3]), inv2), pair2(v.z, v.w)), f[i + 2], f[i + 3]);
+        }
+      }
+    }
+    if (!turns) return;
+    if (a.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x0 = f[2 * i], x1 = f[2 * i + 1];
+        f[2 * i] = fmaf(x0, co[i], -(x1 * si[i]));
+        f[2 * i + 1] = fmaf(x1, co[i], x0 * si[i]);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        co[i] = small_at(a.table, a.table_dtype, row + i);
-        si[i] = small_at(a.table, a.table_dtype, row + (a.R >> 1) + i);
+      for (int i = 0; i < 8; i += 2) {
+        const uint64_t x0 = pair2(f[i], f[i + 1]), x1 = pair2(f[i + 8], f[i + 9]);
+        const uint64_t c = pair2(co[i], co[i + 1]), s = pair2(si[i], si[i + 1]);
+        split2(sub2(mul2(x0, c), mul2(x1, s)), f[i], f[i + 1]);
+        split2(fma2(x0, s, mul2(x1, c)), f[i + 8], f[i + 9]);
       }
     }
-  }
-
-  // Uniform trip count: walkers of one warp shuffle together.
-  for (int u0 = g; u0 - g < total; u0 += kUnroll * a.groups) {
-    Raw8<TI> x[kUnroll][2];
+  };
+  // uniform trip counts: the walkers of a warp shuffle together
+#pragma unroll 1
+  // (walkers beyond the last whole token of a pass have none)
+  for (int64_t t = first < a.step ? first : a.tokens; __any_sync(0xffffffffu, t < a.tokens); t += a.step) {
+    const bool live = t < a.tokens;
+    // rows that a walker does not have are read as its neighbours' and not stored
+    const int64_t tr = live ? t : a.tokens - 1;
+    Raw8<TI> xk[2], xv[2], xq[U][2];
+    if (a.k.heads > 0) fetch(a.k.in, tr * a.k.in_token + k_in, xk);
+    if (a.v.heads > 0) fetch(a.v.in, tr * a.v.in_token + v_in, xv);
+    const int64_t q_at = tr * a.q.in_token;
+    if (a.q.heads > 0) {
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int u = u0 + j * a.groups;
-      x[j][0] = Raw8<TI>{};
-      x[j][1] = Raw8<TI>{};
-      if (!live || u >= total) continue;
-      const HeadRows& r = u < a.q.heads ? a.q : u < a.q.heads + a.k.heads ? a.k : a.v;
-      const int h = u < a.q.heads ? u : u < a.q.heads + a.k.heads ? u - a.q.heads : u - a.q.heads - a.k.heads;
-      const TI* p = static_cast<const TI*>(r.in) + t * r.in_token + h * r.in_head;
-      if (has0) x[j][0] = load8(p + 8 * c0);
-      if (has1) x[j][1] = load8(p + 8 * c1);
+      for (int j = 0; j < U; ++j) fetch(a.q.in, q_at + min64(q0 + j, q_last) * a.q.in_head, xq[j]);
     }
-#pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int u = u0 + j * a.groups;
-      const bool is_q = u < a.q.heads, is_k = !is_q && u < a.q.heads + a.k.heads;
-      const HeadRows& r = is_q ? a.q : is_k ? a.k : a.v;
-      const int h = is_q ? u : is_k ? u - a.q.heads : u - a.q.heads - a.k.heads;
+    Place pl{-1, 0, false};
+    if (live) {
+      uint32_t skipped;
+      pl = place_of(a, t, skipped);
+      if (skipped && g == 0 && lane == 0 && a.err) atomicAdd(a.err, skipped);
+    }
+    if (pl.rotates && turns && (has_k || q0 < q1)) {
+      const int64_t row = pl.position * a.table_stride + 8 * lane;
+      small8(a.table, a.table_dtype, row, co);
+      small8(a.table, a.table_dtype, row + (a.R >> 1), si);
+    }
+    TC* cache_row = static_cast<TC*>(a.cache) + pl.cache_row;
+    if (a.k.heads > 0) {
       float f[16];
-      unpack8(x[j][0], f);
-      unpack8(x[j][1], f + 8);
-      // the branch is taken by the whole warp or the shuffles run anyway: any weight at all
-      if (a.q.weight || a.k.weight) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s = fmaf(f[i], f[i], s);
-        for (int o = lph >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (r.weight && u < total) {
-          const float inv = inv_rms(s, a.D, a.eps);
-          float w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = 0.f;
-          if (has0) small8(r.weight, r.weight_dtype, 8 * c0, w);
-          if (has1) small8(r.weight, r.weight_dtype, 8 * c1, w + 8);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = f[i] * inv * w[i];
-        }
+      turn(w_sm[1], a.k.weight != nullptr, xk, f);
+      if (has_k && pl.rotates) {
+        if (a.k.out) put(static_cast<TI*>(a.k.out) + t * a.k.out_token + kh * a.k.out_head, f);
+        else if (pl.cache_row >= 0) put(cache_row + static_cast<int64_t>(kh) * a.D, f);
       }
-      if (!live || u >= total || !pl.rotates) continue;
-      if (!is_q && !r.out && pl.cache_row < 0) continue;
-      if (is_q || is_k) {
-        if (a.interleaved) {
+    }
+    if (has_v && pl.rotates && pl.cache_row >= 0) {
+      float f[16];
+      unpack8(xv[0], f);
+      unpack8(xv[1], f + 8);
+      put(cache_row + a.kv_stride + static_cast<int64_t>(vh) * a.D, f);
+    }
+    TI* out = static_cast<TI*>(a.q.out) + t * a.q.out_token + q0 * a.q.out_head;
+#pragma unroll 1
+    for (int i0 = 0; i0 < q_per; i0 += U) {
+      if (i0 > 0) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (i < 4 ? turn0 : turn1) {
-              const float x0 = f[2 * i], x1 = f[2 * i + 1];
-              f[2 * i] = fmaf(x0, co[i], -(x1 * si[i]));
-              f[2 * i + 1] = fmaf(x1, co[i], x0 * si[i]);
-            }
-          }
-        } else if (turn0) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x0 = f[i], x1 = f[i + 8];
-            f[i] = fmaf(x0, co[i], -(x1 * si[i]));
-            f[i + 8] = fmaf(x1, co[i], x0 * si[i]);
-          }
-        }
+        for (int j = 0; j < U; ++j)
+          fetch(a.q.in, q_at + min64(q0 + i0 + j, q_last) * a.q.in_head, xq[j]);
       }
-      if (r.out) {
-        TI* o = static_cast<TI*>(r.out) + t * r.out_token + h * r.out_head;
-        if (has0) store8(o + 8 * c0, pack8<TI>(f));
-        if (has1) store8(o + 8 * c1, pack8<TI>(f + 8));
-      } else {
-        TC* o = static_cast<TC*>(a.cache) + (is_k ? 0 : a.kv_stride) + pl.cache_row + static_cast<int64_t>(h) * a.D;
-        if (has0) store8(o + 8 * c0, pack8<TC>(f));
-        if (has1) store8(o + 8 * c1, pack8<TC>(f + 8));
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        float f[16];
+        turn(w_sm[0], a.q.weight != nullptr, xq[j], f);
+        if (q0 + i0 + j < q1 && pl.rotates) put(out + (i0 + j) * a.q.out_head, f);
       }
     }
   }
@@ -323,7 +404,7 @@ __global__ void __launch_bounds__(256) append_rows_any(const __grid_constant__ A
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    inv = inv_rms(s, a.D, a.eps);
+    inv = inv_rms(s, a.inv_d, a.eps);
   }
   auto value = [&](int i) {
     const float v = to_f<TI>(x[i]);
