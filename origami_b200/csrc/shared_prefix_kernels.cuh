@@ -29,7 +29,8 @@
 // maximum grew by more than 2^8 (P stays below 2^8, exact in the same relative precision).
 // With more than 128 rows an item has two row tiles, one per stream, that share each K and V
 // tile ("pair"); with fewer, the streams take one half of each key tile for one row tile and
-// join at the end of the segment ("split").
+// join at the end of the segment ("split"); segments of one tile go to the streams in turn
+// ("solo"), so that one's epilogue runs under the other's work.
 #pragma once
 
 #include <cuda.h>
@@ -52,8 +53,6 @@ constexpr int kRegsLaunch = 128, kRegsSoftmax = 168, kRegsOther = 88;
 static_assert(256 * (kRegsSoftmax + kRegsOther) <= kThreadsS * kRegsLaunch, "register shares");
 constexpr int kTile = 128;      // keys per tile, rows per row tile
 constexpr int kHalf = 64;       // keys per softmax step
-// Of 8 pairs of exponentials, those taken by the FMA pipe (ex2_poly); the others by ex2, of which an SM has 16 a clock.
-constexpr int kPolyPairs = 0;
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of a segment.
 constexpr int kCostTile = 8, kCostPair = 13, kCostItem = 6;
 
@@ -272,9 +271,10 @@ struct Segment {
   int64_t prow;       // partial row of its first row
   int32_t t0, n;      // first tile, tiles; n = 0 ends the share
   int32_t halves;     // 64-key halves of its tiles that hold keys
-  int32_t pair, h, b;  // two row tiles; KV head; request, -1 for the prefix
+  int32_t mode, h, b;  // kSplit .. kSolo + 1; KV head; request, -1 for the prefix
   int32_t tok0, ntok, kend, vis0;
 };
+constexpr int kSplit = 0, kPair = 1, kSolo = 2;  // how the streams share a segment; kSolo + s: stream s alone
 constexpr int kSegments = 4;  // in the ring between the scheduler and the others
 
 // Partial rows: an item's rows begin at its place among all rows of its kind plus its CTA's
@@ -326,22 +326,9 @@ __device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
       : "memory");
 }
 
-// 32 consecutive TMEM columns of this thread's lane.
-__device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr)
-      : "memory");
-}
-// 64 columns: two loads in flight, one wait. The empty statements tie every value to the
-// wait, so that none is used before it.
-__device__ __forceinline__ void ld64(uint32_t addr, uint32_t (&r)[64]) {
+// 32 TMEM columns of this thread's lane from each of two addresses: two loads in flight, one
+// wait. The empty statements tie every value to the wait, so that none is used before it.
+__device__ __forceinline__ void ld64(uint32_t a0, uint32_t a1, uint32_t (&r)[64]) {
 #pragma unroll
   for (int c = 0; c < 64; c += 32)
     asm volatile(
@@ -354,7 +341,7 @@ __device__ __forceinline__ void ld64(uint32_t addr, uint32_t (&r)[64]) {
           "=r"(r[c + 19]), "=r"(r[c + 20]), "=r"(r[c + 21]), "=r"(r[c + 22]), "=r"(r[c + 23]), "=r"(r[c + 24]),
           "=r"(r[c + 25]), "=r"(r[c + 26]), "=r"(r[c + 27]), "=r"(r[c + 28]), "=r"(r[c + 29]), "=r"(r[c + 30]),
           "=r"(r[c + 31])
-        : "r"(addr + c)
+        : "r"(c == 0 ? a0 : a1)
         : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
@@ -422,11 +409,14 @@ __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
-// 32 consecutive floats of a partial row.
-__device__ __forceinline__ void store_o(float* p, const uint32_t (&o)[32]) {
-  uint4* dst = reinterpret_cast<uint4*>(p);
+// The first n of o as consecutive floats of a partial row, whole 32-byte sectors a store.
+__device__ __forceinline__ void store_o(float* p, const uint32_t (&o)[64], int n) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+  for (int j = 0; j < 64; j += 8)
+    if (j < n)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p + j), "r"(o[j]), "r"(o[j + 1]),
+                   "r"(o[j + 2]), "r"(o[j + 3]), "r"(o[j + 4]), "r"(o[j + 5]), "r"(o[j + 6]), "r"(o[j + 7])
+                   : "memory");
 }
 
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
@@ -452,39 +442,11 @@ __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
-// 2^x of two floats on the FMA pipe: x = n + f with n the nearest integer (the magic addend
-// leaves n in the low bits), a degree-5 polynomial of f on [-1/2, 1/2] fitted for the least
-// greatest relative error (2^-22 as evaluated, about ex2.approx's), and n added to the exponent.
-// Below 2^-125 it stays at that; NaN stays NaN.
-constexpr float kE0 = 1.000000119e+00f, kE1 = 6.931469440e-01f, kE2 = 2.402212024e-01f, kE3 = 5.550713092e-02f,
-                kE4 = 9.675540961e-03f, kE5 = 1.327647245e-03f;
-__device__ __forceinline__ void ex2_poly(uint64_t x, float& y0, float& y1) {
-  float x0, x1;
-  split2(x, x0, x1);
-  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(x0));  // -125
-  asm("max.NaN.f32 %0, %0, 0fC2FA0000;" : "+f"(x1));
-  x = pair2(x0, x1);
-  const uint64_t magic = pair2(12582912.f, 12582912.f);  // 1.5 * 2^23
-  const uint64_t t = add2(x, magic);
-  const uint64_t f = add2(x, fma2(t, pair2(-1.f, -1.f), magic));
-  uint64_t p = pair2(kE5, kE5);
-  p = fma2(p, f, pair2(kE4, kE4));
-  p = fma2(p, f, pair2(kE3, kE3));
-  p = fma2(p, f, pair2(kE2, kE2));
-  p = fma2(p, f, pair2(kE1, kE1));
-  p = fma2(p, f, pair2(kE0, kE0));
-  float t0, t1;
-  split2(t, t0, t1);
-  split2(p, y0, y1);
-  y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
-  y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
-}
-
 // A stream's barriers: S begins anew only when every warp has read the last (s_empty), and P's
 // two buffers have a barrier each, so that a parity is never ambiguous.
 struct Bars {
   uint64_t full[10], empty[10], q_empty[2], s_full[2], s_empty[2], p_full[4], pv[4], seg_full[kSegments], seg_empty[kSegments];
-  uint64_t o_free, xch, done;
+  uint64_t o_free[2], xch, done;
 };
 
 }  // namespace spa
@@ -536,7 +498,8 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       mbar_init(&bars->seg_full[i], 1);
       mbar_init(&bars->seg_empty[i], 8 + 4 + 2);  // softmax, loader and product warps
     }
-    mbar_init(&bars->o_free, 8);
+    mbar_init(&bars->o_free[0], 8);
+    mbar_init(&bars->o_free[1], 8);
     mbar_init(&bars->xch, 8);
     mbar_init(&bars->done, 2);
     *abort_sm = 0;
@@ -679,9 +642,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       int row = row_of(key);
       // Q: one row tile, into the buffer after the last one used, or both for a pair. Rows past
       // the end keep what lies there: they reach nothing but their own rows of S and O.
-      if (seg.pair) q_next = 0;
+      if (seg.mode == kPair) q_next = 0;
 #pragma unroll 1
-      for (int q = 0; q <= seg.pair; ++q) {
+      for (int q = 0; q <= (seg.mode == kPair); ++q) {
         const uint32_t buf = q_next;
         q_next ^= 1u;
         if ((q_used >> buf) & 1u) {
@@ -779,6 +742,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       // -------------------------------------------------------------- scheduler
       const Deal deal = *deal_sm;
       Walk w(a, deal);
+      uint32_t solos = 0u;
       for (uint32_t slot = 0;; ++slot) {
         const uint32_t at = slot % kSegments, use = slot / kSegments;
         const bool more = w.step();
@@ -788,7 +752,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           g.n = more ? w.t1 - w.t0 : 0;
           g.t0 = w.t0;
           g.halves = (min(w.it.kend - w.t0 * kTile, g.n * kTile) + kHalf - 1) / kHalf;
-          g.pair = w.it.pair;
+          // one tile: a stream of its own, unless it is all that this CTA has and both can work at it
+          const bool solo = !w.it.pair && g.n == 1 && (g.halves == 1 || slot > 0 || w.next < deal.w1);
+          g.mode = w.it.pair ? kPair : solo ? kSolo + static_cast<int>(solos++ & 1u) : kSplit;
           g.h = w.it.h;
           g.b = w.it.b;
           g.tok0 = w.it.tok0;
@@ -815,28 +781,38 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           phase ^= 1u;
         }
       };
-      uint32_t n_s = 0u, n_pv = 0u, q_next = 0u;  // S and P V products begun
+      uint32_t n_s = 0u, n_pv = 0u, n_seg = 0u, q_next = 0u;  // S and P V products begun, segments ended
       bool ok = true;
 #pragma unroll 1
       for (uint32_t slot = 0;; ++slot) {
         if (!ok || !wait(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u)) break;
         const int n = __shfl_sync(0xffffffffu, segs[slot % kSegments].n, 0);
-        const bool pair = __shfl_sync(0xffffffffu, segs[slot % kSegments].pair, 0) != 0;
+        const int mode = __shfl_sync(0xffffffffu, segs[slot % kSegments].mode, 0);
         const int halves = __shfl_sync(0xffffffffu, segs[slot % kSegments].halves, 0);
         if (lead) mbar_arrive(&bars->seg_empty[slot % kSegments]);
         if (n == 0) break;
-        if (pair) q_next = 0;
-        const uint32_t qb = pair ? s : q_next;
-        if (!pair) q_next ^= 1u;
-        // Step g of the stream is half g & 1 of tile g >> 1 (pair) or half s of tile g (split).
-        const int steps = pair ? halves : (halves + 1 - static_cast<int>(s)) / 2;
-        const int odd = pair ? 1 : 0;  // a tile's first step has (g & odd) == 0, its last odd, or ends the segment
-        const uint32_t half0 = pair ? 0u : s * (kHalf * 128);
+        if (mode == kPair) q_next = 0;
+        const uint32_t qb = mode == kPair ? s : q_next;
+        if (mode != kPair) q_next ^= 1u;
+        if (mode >= kSolo && mode - kSolo != static_cast<int>(s)) {  // one tile, the other stream's
+          next_tile(k_stage, k_phase);
+          next_tile(v_stage, v_phase);
+          continue;
+        }
+        // Step g of the stream is half s of tile g (split) or half g & 1 of tile g >> 1.
+        const int steps = mode == kSplit ? (halves + 1 - static_cast<int>(s)) / 2 : halves;
+        const int odd = mode == kSplit ? 0 : 1;  // a tile's first step has (g & odd) == 0, its last odd, or ends the segment
+        const uint32_t half0 = mode == kSplit ? s * (kHalf * 128) : 0u;
         const uint64_t qd = desc128(base + qb * S::tile, 16);
-        // both streams free a Q buffer, for the other one too where it does not read it
+        // A tile and a Q buffer are freed by two arrivals: one of each stream that reads it, or
+        // both of the only one.
+        auto free_tile = [&](uint32_t stage) {
+          commit(lead, &bars->empty[stage]);
+          if (mode >= kSolo) commit(lead, &bars->empty[stage]);
+        };
         auto free_q = [&]() {
           commit(lead, &bars->q_empty[qb]);
-          if (pair) commit(lead, &bars->q_empty[qb]);
+          if (mode != kSplit) commit(lead, &bars->q_empty[qb]);
         };
         // S of step g + 1 is begun before P V of step g
 #pragma unroll 1
@@ -862,7 +838,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             commit(lead, &bars->s_full[s]);
             ++n_s;
             if ((x & odd) == odd || x == steps - 1) {
-              commit(lead, &bars->empty[k_stage]);
+              free_tile(k_stage);
               next_tile(k_stage, k_phase);
             }
             if (x == steps - 1) free_q();
@@ -873,7 +849,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               break;
             }
             if (!wait(&bars->p_full[2 * s + (n_pv & 1u)], (n_pv >> 1) & 1u) ||
-                (g == 0 && slot > 0 && !wait(&bars->o_free, (slot - 1) & 1u))) {  // the last segment's O has been read
+                (g == 0 && n_seg > 0 && !wait(&bars->o_free[s], (n_seg - 1) & 1u))) {  // the last segment's O has been read
               ok = false;
               break;
             }
@@ -887,20 +863,18 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             commit(lead, &bars->pv[2 * s + (n_pv & 1u)]);
             ++n_pv;
             if ((g & odd) == odd || g == steps - 1) {
-              commit(lead, &bars->empty[v_stage]);
+              free_tile(v_stage);
               next_tile(v_stage, v_phase);
             }
           }
         }
         if (!ok) break;
-        if (!pair && steps < n) {  // both streams free a tile, also one without keys for this one
-          if (steps == 0) free_q();
-          commit(lead, &bars->empty[k_stage]);
-          commit(lead, &bars->empty[v_stage]);
+        ++n_seg;
+        if (mode == kSplit && steps < n) {  // the last tile has no keys for this stream
+          free_tile(k_stage);
+          free_tile(v_stage);
           next_tile(k_stage, k_phase);
           next_tile(v_stage, v_phase);
-          // no phase of o_free may pass unseen: a parity tells two neighbours apart only
-          if (steps == 0 && slot > 0 && !wait(&bars->o_free, (slot - 1) & 1u)) break;
         }
       }
       // nothing may be in flight when the columns are released
@@ -925,15 +899,16 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->seg_empty[slot % kSegments]);
       if (seg.n == 0) break;
-      const bool pair = seg.pair != 0;
-      const int steps = pair ? seg.halves : s == 0 ? (seg.halves + 1) / 2 : seg.halves / 2;
-      const int first_tok = pair ? s * a.tile_tokens : 0;
+      if (seg.mode >= kSolo && seg.mode - kSolo != s) continue;
+      const bool split = seg.mode == kSplit;
+      const int steps = !split ? seg.halves : s == 0 ? (seg.halves + 1) / 2 : seg.halves / 2;
+      const int first_tok = seg.mode == kPair ? s * a.tile_tokens : 0;
       const int rows = min(a.tile_tokens, seg.ntok - first_tok) * a.group;
       const bool warp_live = (warp & 3) * 32 < rows;
       // keys of the item this row sees, less those before the current step's
       int lim = 0;
       if (row < rows) lim = seg.b < 0 ? seg.kend : clamp32(seg.vis0 + token_in_tile, 0, seg.kend);
-      lim -= seg.t0 * kTile + (pair ? 0 : s * kHalf);
+      lim -= seg.t0 * kTile + (split ? s * kHalf : 0);
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int i = 0; i < steps; ++i) {
@@ -943,11 +918,10 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         tc_fence_after();
         if (warp_live) {
           uint32_t x[kHalf];
-          ld64(ts, x);
+          ld64(ts, ts + 32, x);
           tc_fence_before();
           arrive_warp(&bars->s_empty[s]);
-          const bool masked = !__all_sync(0xffffffffu, lim >= kHalf || row >= rows);
-          if (masked) {
+          if (!__all_sync(0xffffffffu, lim >= kHalf || row >= rows)) {
 #pragma unroll
             for (int j = 0; j < kHalf; ++j)
               if (j >= lim) x[j] = 0xFF800000u;  // -inf: not seen
@@ -997,17 +971,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               const uint64_t arg =
                   fma2(pair2(__uint_as_float(x[32 * q + 2 * j]), __uint_as_float(x[32 * q + 2 * j + 1])), scale2, neg2);
               float p0, p1;
-              if ((j & 7) < kPolyPairs) {
-                ex2_poly(arg, p0, p1);
-                if (masked) {  // exactly nothing
-                  if (32 * q + 2 * j >= lim) p0 = 0.f;
-                  if (32 * q + 2 * j + 1 >= lim) p1 = 0.f;
-                }
-              } else {
-                split2(arg, p0, p1);
-                p0 = ex2(p0);
-                p1 = ex2(p1);
-              }
+              split2(arg, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
               sum[j & 3] = add2(sum[j & 3], pair2(p0, p1));
               p[j] = pack2<QT>(p0, p1);
             }
@@ -1022,24 +988,23 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         }
         tc_fence_before();
         arrive_warp(&bars->p_full[2 * s + buf]);
-        lim -= pair ? kHalf : kTile;
+        lim -= split ? kTile : kHalf;
         ++count;
       }
       if (!ok) break;
       // ------------------------------------------------------------ the segment's partial
       // scores that are all NaN leave no maximum: any reference carries their NaN on
       if (l != l && m == -INFINITY) m = 0.f;
-      if (steps > 0) {
+      {
         const uint32_t last = count - 1;
         ok = wait_warp(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort);
         if (!ok) break;
       }
-      if (!pair) {
-        // Both streams' sums belong to the same rows: exchange (m, l), then each stream joins
-        // and writes half of the dims. A stream without a tile waits here too, so that it
-        // cannot arrive twice in one phase of o_free. (m, l) of the segment before were read
-        // before this segment's first product could begin.
-        if (steps > 0) ml_sm[s * kTile + row] = make_float2(m, l);
+      if (split) {
+        // Both streams' sums belong to the same rows: exchange (m, l), then each stream joins and
+        // writes half of the dims. (m, l) of the split segment before were read before a stream's
+        // next product into O could begin.
+        ml_sm[s * kTile + row] = make_float2(m, l);
         tc_fence_before();
         arrive_warp(&bars->xch);
         ok = wait_warp(&bars->xch, x_phase, abort);
@@ -1049,38 +1014,42 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       tc_fence_after();
       if (warp_live) {
         const int64_t prow = seg.prow + first_tok * a.group + row;
-        if (pair) {
+        if (!split) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            ld32(to + c, o);
-            if (row < rows) store_o(a.o + prow * D + c, o);
+          for (int c = 0; c < D; c += 64) {
+            uint32_t o[64];
+            ld64(to + c, to + c + 32, o);
+            if (row < rows) store_o(a.o + prow * D + c, o, 64);
           }
           if (row < rows) reinterpret_cast<float2*>(a.ml)[prow] = make_float2(m, l);
         } else {
-          const bool two = seg.halves > 1;
-          const float2 ml0 = ml_sm[row], ml1 = two ? ml_sm[kTile + row] : make_float2(-INFINITY, 0.f);
+          const float2 ml0 = ml_sm[row], ml1 = ml_sm[kTile + row];
           const float mm = fmaxf(ml0.x, ml1.x);
           const float w0 = ml0.x == -INFINITY ? 0.f : ex2(ml0.x - mm), w1 = ml1.x == -INFINITY ? 0.f : ex2(ml1.x - mm);
 #pragma unroll 1
           for (int c = 0; c < D / 2; c += 32) {
             const int col = s * (D / 2) + c;
-            uint32_t o0[32], o1[32];
-            ld32(lane_base + kO + col, o0);
-            if (two) {
-              ld32(lane_base + 256 + kO + col, o1);
+            uint32_t o[64];  // 32 dims of each stream's O
+            ld64(lane_base + kO + col, lane_base + 256 + kO + col, o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                o0[j] = __float_as_uint(fmaf(__uint_as_float(o0[j]), w0, __uint_as_float(o1[j]) * w1));
-            }
-            if (row < rows) store_o(a.o + prow * D + col, o0);
+            for (int j = 0; j < 32; ++j)
+              o[j] = __float_as_uint(fmaf(__uint_as_float(o[j]), w0, __uint_as_float(o[32 + j]) * w1));
+            if (row < rows) store_o(a.o + prow * D + col, o, 32);
           }
-          if (row < rows && s == 0)
-            reinterpret_cast<float2*>(a.ml)[prow] = two ? make_float2(mm, fmaf(ml0.y, w0, ml1.y * w1)) : ml0;
+          if (row < rows && s == 0) reinterpret_cast<float2*>(a.ml)[prow] = make_float2(mm, fmaf(ml0.y, w0, ml1.y * w1));
         }
       }
       tc_fence_before();
-      arrive_warp(&bars->o_free);
+      __syncwarp();
+      if (lane == 0) {  // 8 arrivals free an O: of all warps that read it
+        if (split) {
+          mbar_arrive(&bars->o_free[0]);
+          mbar_arrive(&bars->o_free[1]);
+        } else {
+          mbar_arrive(&bars->o_free[s]);
+          mbar_arrive(&bars->o_free[s]);
+        }
+      }
     }
   }
   tc_fence_before();
