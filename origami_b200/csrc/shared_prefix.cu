@@ -175,7 +175,7 @@ int32_t origami_shared_prefix_attention(
   const int64_t row_tiles = (tokens + per_tile - 1) / per_tile;
   const int64_t suffix_cap = std::min<int64_t>(suffix_width, 0x3FFFFFFF / cache->block_size) * cache->block_size;
   auto cost = [](int64_t keys, int64_t tile) {
-    return origami::spa::kCostItem + (keys + origami::spa::kTile - 1) / origami::spa::kTile * tile;
+    return origami::spa::kCostPairItem + (keys + origami::spa::kTile - 1) / origami::spa::kTile * tile;
   };
   const double most = static_cast<double>(cache->num_heads) *
                       (static_cast<double>(row_tiles) * cost(prefix_tokens, origami::spa::kCostPair) +

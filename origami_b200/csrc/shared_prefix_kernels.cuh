@@ -53,8 +53,8 @@ constexpr int kRegsLaunch = 128, kRegsSoftmax = 168, kRegsOther = 88;
 static_assert(256 * (kRegsSoftmax + kRegsOther) <= kThreadsS * kRegsLaunch, "register shares");
 constexpr int kTile = 128;      // keys per tile, rows per row tile
 constexpr int kHalf = 64;       // keys per softmax step
-// Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of a segment.
-constexpr int kCostTile = 8, kCostPair = 13, kCostItem = 6;
+// Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of an item of either kind.
+constexpr int kCostTile = 8, kCostPair = 12, kCostItem = 8, kCostPairItem = 22;
 
 // Shared memory: Q tiles, then the ring of K / V tiles (each [128][D] 16-bit), then scalars.
 template <int D>
@@ -122,11 +122,11 @@ struct Item {
   bool pair;
   __device__ __forceinline__ int tiles() const { return (kend + kTile - 1) / kTile; }
   __device__ __forceinline__ int cost() const {
-    return kend > 0 ? kCostItem + tiles() * (pair ? kCostPair : kCostTile) : 0;
+    return kend > 0 ? (pair ? kCostPairItem + tiles() * kCostPair : kCostItem + tiles() * kCostTile) : 0;
   }
   // First tile that a share beginning at w takes.
   __device__ __forceinline__ int tile_at(int w) const {
-    const int x = w - start - kCostItem;
+    const int x = w - start - (pair ? kCostPairItem : kCostItem);
     if (x <= 0) return 0;
     return min(pair ? (x + kCostPair - 1) / kCostPair : (x + kCostTile - 1) / kCostTile, tiles());
   }
@@ -599,7 +599,10 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     const uint32_t base = smem_u32(sm);
     uint32_t ring = 0, signalled = 0;  // stages begun, stages whose arrival this warp has made
     uint32_t slot = 0, q_used = 0u, q_phase = 0u, q_next = 0u;
-    bool ok = true, q_pending = false;
+    // a segment's first tile is signalled with its Q: held back until Q is requested, and then
+    // until it has landed (q_wait)
+    bool ok = true, q_hold = false, q_wait = false;
+    uint32_t hold = 0;
     // Copies of this warp's own threads are generic-proxy writes: the fence that orders the
     // products' reads behind them is made here, once they have landed (in the products' warp it
     // would wait for the products under way). TMA stages need none and arrive at once unless an
@@ -614,7 +617,8 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     };
     auto drain = [&]() {
       asm volatile("cp.async.wait_all;\n" ::: "memory");
-      signal(ring);
+      signal(q_hold ? hold : ring);
+      q_wait = q_wait && q_hold;
     };
     // Waits with nothing unsignalled behind: whoever makes the arrival may need it.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -640,47 +644,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       };
       int key = seg.t0 * kTile + 32 * lw + lane;
       int row = row_of(key);
-      // Q: one row tile, into the buffer after the last one used, or both for a pair. Rows past
-      // the end keep what lies there: they reach nothing but their own rows of S and O.
-      if (seg.mode == kPair) q_next = 0;
-#pragma unroll 1
-      for (int q = 0; q <= (seg.mode == kPair); ++q) {
-        const uint32_t buf = q_next;
-        q_next ^= 1u;
-        if ((q_used >> buf) & 1u) {
-          ok = wait(&bars->q_empty[buf], (q_phase >> buf) & 1u);
-          if (!ok) break;
-          q_phase ^= 1u << buf;
-        }
-        q_used |= 1u << buf;
-        // lane l finds the query row of tile row 32 lw + l
-        const int mine = min(a.tile_tokens, seg.ntok - q * a.tile_tokens) * a.group - 32 * lw;  // rows of this warp
-        if (mine <= 0) continue;
-        const int tile_row = 32 * lw + lane, tl = tile_row / a.group;
-        const int64_t at = (seg.tok0 + static_cast<int64_t>(q) * a.tile_tokens + tl) * a.q_token +
-                           (seg.h * a.group + tile_row - tl * a.group) * a.q_head;
-        const uint32_t dst = base + buf * S::tile;
-#pragma unroll 1
-        for (int i = 0; i < min(mine, 32); i += 2 * kRowsPer) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = i + j * kRowsPer + sub;
-            const uint16_t* src = a.query + __shfl_sync(0xffffffffu, at, r & 31) + chunk * 8;
-            if (r >= mine || r >= 32) continue;
-            if (a.q_vec) {
-              cp_async16_at(dst + chunk_off(32 * lw + r, chunk), src);
-            } else {
-              uint32_t v[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = src[2 * e] | (static_cast<uint32_t>(src[2 * e + 1]) << 16);
-              *reinterpret_cast<uint4*>(sm + buf * S::tile + chunk_off(32 * lw + r, chunk)) =
-                  make_uint4(v[0], v[1], v[2], v[3]);
-            }
-          }
-        }
-        q_pending = true;
-      }
-      if (!ok) break;
+      if (signalled != ring) drain();
+      q_hold = true;
+      hold = ring;
 #pragma unroll 1
       for (int i = 0; i < seg.n && ok; ++i) {
         const bool tma = a.tma_rows > 0 && __all_sync(0xffffffffu, key < seg.kend);
@@ -719,16 +685,61 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           }
           asm volatile("cp.async.commit_group;\n" ::: "memory");
           ++ring;
-          if (tma && !q_pending && signalled + 1 == ring) {
+          if (q_hold) continue;
+          if (q_wait) {
+            drain();
+          } else if (tma && signalled + 1 == ring) {
             if (lead) mbar_arrive(&bars->full[st]);
             signalled = ring;
           } else if (ring - signalled > S::lag) {
             asm volatile("cp.async.wait_group %0;\n" ::"n"(S::lag) : "memory");
             signal(ring - S::lag);
           }
-          q_pending = false;
         }
         row = next_row;
+        if (i > 0) continue;
+        // Q, behind the first tile's requests: one row tile, into the buffer after the last one
+        // used, or both for a pair. Rows past the end keep what lies there: they reach nothing but
+        // their own rows of S and O.
+        if (seg.mode == kPair) q_next = 0;
+#pragma unroll 1
+        for (int q = 0; q <= (seg.mode == kPair); ++q) {
+          const uint32_t buf = q_next;
+          q_next ^= 1u;
+          if ((q_used >> buf) & 1u) {
+            ok = wait(&bars->q_empty[buf], (q_phase >> buf) & 1u);
+            if (!ok) break;
+            q_phase ^= 1u << buf;
+          }
+          q_used |= 1u << buf;
+          // lane l finds the query row of tile row 32 lw + l
+          const int mine = min(a.tile_tokens, seg.ntok - q * a.tile_tokens) * a.group - 32 * lw;  // rows of this warp
+          if (mine <= 0) continue;
+          const int tile_row = 32 * lw + lane, tl = tile_row / a.group;
+          const int64_t at = (seg.tok0 + static_cast<int64_t>(q) * a.tile_tokens + tl) * a.q_token +
+                             (seg.h * a.group + tile_row - tl * a.group) * a.q_head;
+          const uint32_t dst = base + buf * S::tile;
+#pragma unroll 1
+          for (int i = 0; i < min(mine, 32); i += 2 * kRowsPer) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int r = i + j * kRowsPer + sub;
+              const uint16_t* src = a.query + __shfl_sync(0xffffffffu, at, r & 31) + chunk * 8;
+              if (r >= mine || r >= 32) continue;
+              if (a.q_vec) {
+                cp_async16_at(dst + chunk_off(32 * lw + r, chunk), src);
+              } else {
+                uint32_t v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = src[2 * e] | (static_cast<uint32_t>(src[2 * e + 1]) << 16);
+                *reinterpret_cast<uint4*>(sm + buf * S::tile + chunk_off(32 * lw + r, chunk)) =
+                    make_uint4(v[0], v[1], v[2], v[3]);
+              }
+            }
+          }
+        }
+        q_hold = false;
+        q_wait = true;
       }
     }
     drain();
