@@ -239,7 +239,7 @@ int32_t origami_shared_prefix_attention(
   a.ctas = sms;
   // One row a warp while the rows are few (their latency counts), more when their lists' lookup would
   // be what an SM spends its issue slots on.
-  a.merge_rows = static_cast<int32_t>(std::clamp<int64_t>(tokens * a.q_heads / (32 * sms), 1, a.group));
+  a.merge_rows = static_cast<int32_t>(std::clamp<int64_t>(tokens * a.q_heads / (16 * sms), 1, a.group));
   a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   uint8_t* ws = static_cast<uint8_t*>(d_workspace);
   a.head = reinterpret_cast<int32_t*>(ws);
