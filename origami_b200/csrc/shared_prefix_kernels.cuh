@@ -21,17 +21,15 @@
 // 128-byte-swizzled tiles, by TMA where a block's rows come in eights (a box per block), else
 // and where a tile ends inside with 16-byte cp.async (rows past the end become zeros, so
 // garbage there cannot reach the products); one warp per stream issues its tcgen05.mma; two softmax
-// warpgroups own one stream each, a stream being an (S, O) pair in TMEM:
-//   S_s [128 rows x 128 keys] = Q K^T (shared memory operands),
-//   O_s [128 rows x D]       += P V   (P in TMEM over half of S, V the N-major B operand).
-// A stream's S, softmax and P V follow one another; the other stream's softmax runs under its
-// products and the other way round. (Steps of 64 keys with two buffers of S or of P let a
-// stream's next scores begin early, but cost more: half as many columns make Q K^T 1.5 times
-// slower, bound by shared memory, and the barriers' latencies count twice.) One thread owns one row: the softmax needs no exchange. O is rescaled only when the
+// warpgroups own one stream each, a stream being, in TMEM, 64 keys' scores, two buffers of P and O:
+//   S_s [128 rows x 64 keys] = Q K^T (shared memory operands),
+//   O_s [128 rows x D]      += P V   (P in TMEM, V the N-major B operand).
+// The next scores are begun as soon as a step has read its own, so a stream's chain is its
+// softmax alone. One thread owns one row: the softmax needs no exchange. O is rescaled only when the
 // maximum grew by more than 2^8 (P stays below 2^8, exact in the same relative precision).
 // With more than 128 rows an item has two row tiles, one per stream, that share each K and V
-// tile ("pair"); with fewer, the streams take alternate key tiles of one row tile and join at
-// the end of the segment ("split"); segments of one tile go to the streams in turn
+// tile ("pair"); with fewer, the streams take one half of each key tile for one row tile and
+// join at the end of the segment ("split"); segments of one tile go to the streams in turn
 // ("solo"), so that one's epilogue runs under the other's work.
 #pragma once
 
@@ -50,10 +48,11 @@ namespace spa {
 constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12 / 14: products of
                                 // stream 0 / 1; 13: scheduler
 // Registers per thread at launch, then of the softmax warpgroups and of the others:
-// 256 * 184 + 256 * 72 = 512 * 128, all that the block was launched with.
-constexpr int kRegsLaunch = 128, kRegsSoftmax = 184, kRegsOther = 72;
+// 256 * 168 + 256 * 88 = 512 * 128, all that the block was launched with.
+constexpr int kRegsLaunch = 128, kRegsSoftmax = 168, kRegsOther = 88;
 static_assert(256 * (kRegsSoftmax + kRegsOther) <= kThreadsS * kRegsLaunch, "register shares");
 constexpr int kTile = 128;      // keys per tile, rows per row tile
+constexpr int kHalf = 64;       // keys per softmax step
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of an item of either kind.
 constexpr int kCostTile = 8, kCostPair = 12, kCostItem = 8, kCostPairItem = 22;
 
@@ -271,14 +270,13 @@ struct Walk {
 struct Segment {
   int64_t prow;       // partial row of its first row
   int32_t t0, n;      // first tile, tiles; n = 0 ends the share
+  int32_t halves;     // 64-key halves of its tiles that hold keys
   int32_t mode, h, b;  // kSplit .. kSolo + 1; KV head; request, -1 for the prefix
   int32_t tok0, ntok, kend, vis0;
 };
 constexpr int kSplit = 0, kPair = 1, kSolo = 2;  // how the streams share a segment; kSolo + s: stream s alone
-// The readers of tile i of a segment: stream 0, stream 1, or 2 for both.
-__device__ __forceinline__ uint32_t readers(int mode, int i) {
-  return mode == kPair ? 2u : mode == kSplit ? static_cast<uint32_t>(i & 1) : static_cast<uint32_t>(mode - kSolo);
-}
+// The readers of a segment's tiles: stream 0, stream 1, or 2 for both.
+__device__ __forceinline__ uint32_t readers(int mode) { return mode < kSolo ? 2u : static_cast<uint32_t>(mode - kSolo); }
 constexpr int kSegments = 4;  // in the ring between the scheduler and the others
 
 // Partial rows: an item's rows begin at its place among all rows of its kind plus its CTA's
@@ -350,25 +348,6 @@ __device__ __forceinline__ void ld64(uint32_t a0, uint32_t a1, uint32_t (&r)[64]
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
   for (int j = 0; j < 64; ++j) asm volatile("" : "+r"(r[j]));
-}
-__device__ __forceinline__ void ld128(uint32_t addr, uint32_t (&r)[128]) {
-#pragma unroll
-  for (int c = 0; c < 128; c += 32)
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-        "%30,%31}, [%32];\n"
-        : "=r"(r[c]), "=r"(r[c + 1]), "=r"(r[c + 2]), "=r"(r[c + 3]), "=r"(r[c + 4]), "=r"(r[c + 5]), "=r"(r[c + 6]),
-          "=r"(r[c + 7]), "=r"(r[c + 8]), "=r"(r[c + 9]), "=r"(r[c + 10]), "=r"(r[c + 11]), "=r"(r[c + 12]),
-          "=r"(r[c + 13]), "=r"(r[c + 14]), "=r"(r[c + 15]), "=r"(r[c + 16]), "=r"(r[c + 17]), "=r"(r[c + 18]),
-          "=r"(r[c + 19]), "=r"(r[c + 20]), "=r"(r[c + 21]), "=r"(r[c + 22]), "=r"(r[c + 23]), "=r"(r[c + 24]),
-          "=r"(r[c + 25]), "=r"(r[c + 26]), "=r"(r[c + 27]), "=r"(r[c + 28]), "=r"(r[c + 29]), "=r"(r[c + 30]),
-          "=r"(r[c + 31])
-        : "r"(addr + c)
-        : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-#pragma unroll
-  for (int j = 0; j < 128; ++j) asm volatile("" : "+r"(r[j]));
 }
 __device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
@@ -467,10 +446,11 @@ __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
 }
 
 // A parity tells a barrier's last phase from the one before only, so whoever waits on a barrier
-// has to see each of its phases. A stage's tile is read by stream 0, by stream 1 or by both:
-// its arrival goes to the barrier of that set of readers, who see all phases of theirs.
+// has to see each of its phases. S begins anew only when every warp has read the last (s_empty),
+// and P's two buffers have a barrier each. A stage's tile is read by stream 0, by stream 1 or by
+// both: its arrival goes to the barrier of that set of readers.
 struct Bars {
-  uint64_t full[3][10], empty[10], q_empty[2], s_full[2], p_full[2], pv[2], seg_full[kSegments], seg_empty[kSegments];
+  uint64_t full[3][10], empty[10], q_empty[2], s_full[2], s_empty[2], p_full[4], pv[4], seg_full[kSegments], seg_empty[kSegments];
   uint64_t o_free[2], xch, done;
 };
 
@@ -494,9 +474,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   static_assert(sizeof(Bars) + 8 + sizeof(Deal) + kSegments * sizeof(Segment) <= 1024, "scalars fit");
   static_assert(S::bytes <= 227 * 1024, "shared memory of one SM");
   constexpr bool kBf16 = attn::is_bf16<QT>();
-  constexpr uint32_t kIdescS = attn::instr_desc(kBf16, kTile);
+  constexpr uint32_t kIdescS = attn::instr_desc(kBf16, kHalf);
   constexpr uint32_t kIdescO = attn::instr_desc(kBf16, D) | (1u << 16);  // B (V) is N-major
-  constexpr uint32_t kP = 64, kO = 128;  // of stream s: S at column 256 s, P at + 64, O at + 128
+  constexpr uint32_t kP = 64, kO = 128;  // of stream s: S at column 256 s, P at + 64 and + 96, O at + 128
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = static_cast<int>(blockIdx.x);
@@ -513,8 +493,11 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->q_empty[i], 2);
       mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->p_full[i], 4);
+      mbar_init(&bars->s_empty[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bars->pv[i], 1);
+      mbar_init(&bars->p_full[i], 4);
     }
     for (int i = 0; i < kSegments; ++i) {
       mbar_init(&bars->seg_full[i], 1);
@@ -634,7 +617,10 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       proxy_fence();
       __syncwarp();
       if (lane == 0)
-        for (uint32_t i = signalled; i < upto; ++i) mbar_arrive(&bars->full[(sets >> (2 * (i % S::stages))) & 3u][i % S::stages]);
+        for (uint32_t i = signalled; i < upto; ++i) {
+          const uint32_t st = i % S::stages;
+          mbar_arrive(&bars->full[(sets >> (2 * st)) & 3u][st]);
+        }
       signalled = upto;
     };
     auto drain = [&]() {
@@ -669,12 +655,12 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       if (signalled != ring) drain();
       q_hold = true;
       hold = ring;
+      const uint32_t set = readers(seg.mode);
 #pragma unroll 1
       for (int i = 0; i < seg.n && ok; ++i) {
         const bool tma = a.tma_rows > 0 && __all_sync(0xffffffffu, key < seg.kend);
         key += kTile;
         const int next_row = i + 1 < seg.n ? row_of(key) : -1;
-        const uint32_t set = readers(seg.mode, i);
         // Waits until stage `ring` may be refilled, copies this warp's rows of K (which = 0) and
         // of V: all inside the item by TMA, else row by row. The stage is full when every
         // loader warp's rows have landed (Q's with the first K's).
@@ -789,7 +775,10 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           Segment& g = segs[at];
           g.n = more ? w.t1 - w.t0 : 0;
           g.t0 = w.t0;
-          g.mode = w.it.pair ? kPair : g.n == 1 ? kSolo + static_cast<int>(solos++ & 1u) : kSplit;
+          g.halves = (min(w.it.kend - w.t0 * kTile, g.n * kTile) + kHalf - 1) / kHalf;
+          // one tile: a stream of its own, unless it is all that this CTA has and both can work at it
+          const bool solo = !w.it.pair && g.n == 1 && (g.halves == 1 || slot > 0 || w.next < deal.w1);
+          g.mode = w.it.pair ? kPair : solo ? kSolo + static_cast<int>(solos++ & 1u) : kSplit;
           g.h = w.it.h;
           g.b = w.it.b;
           g.tok0 = w.it.tok0;
@@ -807,68 +796,115 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t lead = elect_one();
       auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_warp(bar, parity, abort); };
-      uint32_t ring = 0u;  // stage at which the segment begins; tile t's K and V are the 2 t-th and the next
-      uint32_t n_step = 0u, n_seg = 0u, q_next = 0u;  // steps and segments so far
-      uint32_t own = 0u, both = 0u;  // phases of this stream's own full barriers and of the shared ones, a bit per stage
+      // stages of the tiles that S and P V use next (K and V alternate in the ring); phases of this
+      // stream's own full barriers and of the shared ones, a bit per stage
+      uint32_t k_stage = 0u, v_stage = 1u, own = 0u, both = 0u;
+      auto next_tile = [](uint32_t& stage) {
+        stage += 2;
+        if (stage >= S::stages) stage -= S::stages;
+      };
+      uint32_t n_s = 0u, n_pv = 0u, n_seg = 0u, q_next = 0u;  // S and P V products begun, segments ended
       bool ok = true;
 #pragma unroll 1
       for (uint32_t slot = 0;; ++slot) {
         if (!ok || !wait(&bars->seg_full[slot % kSegments], (slot / kSegments) & 1u)) break;
         const int n = __shfl_sync(0xffffffffu, segs[slot % kSegments].n, 0);
         const int mode = __shfl_sync(0xffffffffu, segs[slot % kSegments].mode, 0);
+        const int halves = __shfl_sync(0xffffffffu, segs[slot % kSegments].halves, 0);
         if (lead) mbar_arrive(&bars->seg_empty[slot % kSegments]);
         if (n == 0) break;
         if (mode == kPair) q_next = 0;
         const uint32_t qb = mode == kPair ? s : q_next;
         if (mode != kPair) q_next ^= 1u;
-        const bool mine = mode < kSolo || mode - kSolo == static_cast<int>(s);
-        const uint64_t qd = desc128(base + qb * S::tile, 16);
-        // Tiles of this stream: all of them (pair), every other one (split), the only one (solo).
-        const int begin = mode == kSplit ? static_cast<int>(s) : 0, by = mode == kSplit ? 2 : 1;
-#pragma unroll 1
-        for (int t = begin; t < n && mine; t += by) {
-          const uint32_t at = ring + 2 * static_cast<uint32_t>(t), k_stage = at % S::stages, v_stage = (at + 1) % S::stages;
-          auto wait_full = [&](uint32_t stage) {
-            const bool full = wait(&bars->full[mode == kPair ? 2u : s][stage], ((mode == kPair ? both : own) >> stage) & 1u);
-            if (mode == kPair) both ^= 1u << stage;
-            else own ^= 1u << stage;
-            return full;
-          };
-          // P lies in S: the product that reads it must have ended before S is written again
-          ok = wait_full(k_stage) && (n_step == 0 || wait(&bars->pv[s], (n_step - 1) & 1u));
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t kd = desc128(base + S::ring + k_stage * S::tile, 16);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
-            mma_ss(lead, tm + 256 * s, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
-          }
-          commit(lead, &bars->s_full[s]);
-          // a tile and a Q buffer are freed by two arrivals: one of each stream that reads it, or
-          // both of the only one
-          commit(lead, &bars->empty[k_stage]);
-          if (mode != kPair) commit(lead, &bars->empty[k_stage]);
-          if (t + by >= n) {
-            commit(lead, &bars->q_empty[qb]);
-            if (mode != kSplit) commit(lead, &bars->q_empty[qb]);
-          }
-          ok = wait_full(v_stage) && wait(&bars->p_full[s], n_step & 1u) &&
-               (t != begin || n_seg == 0 || wait(&bars->o_free[s], (n_seg - 1) & 1u));  // the last segment's O was read
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t vd = desc128(base + S::ring + v_stage * S::tile, kTile * 128);
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            mma_ts(lead, tm + 256 * s + kO, tm + 256 * s + kP + k * 8, vd + k * (2048 >> 4), kIdescO,
-                   (t != begin || k > 0) ? 1u : 0u);
-          commit(lead, &bars->pv[s]);
-          commit(lead, &bars->empty[v_stage]);
-          if (mode != kPair) commit(lead, &bars->empty[v_stage]);
-          ++n_step;
+        if (mode >= kSolo && mode - kSolo != static_cast<int>(s)) {  // one tile, the other stream's
+          next_tile(k_stage);
+          next_tile(v_stage);
+          continue;
         }
-        if (mine) ++n_seg;
-        ring += 2 * static_cast<uint32_t>(n);
+        // Step g of the stream is half s of tile g (split) or half g & 1 of tile g >> 1.
+        const int steps = mode == kSplit ? (halves + 1 - static_cast<int>(s)) / 2 : halves;
+        const int odd = mode == kSplit ? 0 : 1;  // a tile's first step has (g & odd) == 0, its last odd, or ends the segment
+        const uint32_t half0 = mode == kSplit ? s * (kHalf * 128) : 0u;
+        const uint64_t qd = desc128(base + qb * S::tile, 16);
+        auto wait_full = [&](uint32_t stage) {
+          const bool full = wait(&bars->full[readers(mode)][stage], ((mode < kSolo ? both : own) >> stage) & 1u);
+          if (mode < kSolo) both ^= 1u << stage;
+          else own ^= 1u << stage;
+          return full;
+        };
+        // A tile and a Q buffer are freed by two arrivals: one of each stream that reads it, or
+        // both of the only one.
+        auto free_tile = [&](uint32_t stage) {
+          commit(lead, &bars->empty[stage]);
+          if (mode >= kSolo) commit(lead, &bars->empty[stage]);
+        };
+        auto free_q = [&]() {
+          commit(lead, &bars->q_empty[qb]);
+          if (mode != kSplit) commit(lead, &bars->q_empty[qb]);
+        };
+        // S of step g + 1 is begun before P V of step g
+#pragma unroll 1
+        for (int g = -1; g < steps; ++g) {
+          if (g + 1 < steps) {
+            const int x = g + 1;
+            if ((x & odd) == 0 && !wait_full(k_stage)) {
+              ok = false;
+              break;
+            }
+            if (n_s > 0 && !wait(&bars->s_empty[s], (n_s - 1) & 1u)) {  // the last S has been read
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t d = tm + 256 * s;
+            const uint64_t kd = desc128(base + S::ring + k_stage * S::tile + half0 + (x & odd) * (kHalf * 128), 16);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+              mma_ss(lead, d, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
+            }
+            commit(lead, &bars->s_full[s]);
+            ++n_s;
+            if ((x & odd) == odd || x == steps - 1) {
+              free_tile(k_stage);
+              next_tile(k_stage);
+            }
+            if (x == steps - 1) free_q();
+          }
+          if (g >= 0) {
+            if ((g & odd) == 0 && !wait_full(v_stage)) {
+              ok = false;
+              break;
+            }
+            if (!wait(&bars->p_full[2 * s + (n_pv & 1u)], (n_pv >> 1) & 1u) ||
+                (g == 0 && n_seg > 0 && !wait(&bars->o_free[s], (n_seg - 1) & 1u))) {  // the last segment's O has been read
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t d = tm + 256 * s + kO, p = tm + 256 * s + kP + 32 * (n_pv & 1u);
+            const uint64_t vd =
+                desc128(base + S::ring + v_stage * S::tile + half0 + (g & odd) * (kHalf * 128), kTile * 128);
+#pragma unroll
+            for (int k = 0; k < kHalf / 16; ++k)
+              mma_ts(lead, d, p + k * 8, vd + k * (2048 >> 4), kIdescO, (g > 0 || k > 0) ? 1u : 0u);
+            commit(lead, &bars->pv[2 * s + (n_pv & 1u)]);
+            ++n_pv;
+            if ((g & odd) == odd || g == steps - 1) {
+              free_tile(v_stage);
+              next_tile(v_stage);
+            }
+          }
+        }
+        if (!ok) break;
+        ++n_seg;
+        if (mode == kSplit && steps < n) {  // the last tile has no keys for this stream: seen and freed
+          ok = wait_full(k_stage) && wait_full(v_stage);
+          free_tile(k_stage);
+          free_tile(v_stage);
+          next_tile(k_stage);
+          next_tile(v_stage);
+        }
       }
       // nothing may be in flight when the columns are released
       commit(lead, &bars->done);
@@ -894,44 +930,51 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       if (seg.n == 0) break;
       if (seg.mode >= kSolo && seg.mode - kSolo != s) continue;
       const bool split = seg.mode == kSplit;
-      const int steps = split ? (seg.n + 1 - s) / 2 : seg.n;
+      const int steps = !split ? seg.halves : s == 0 ? (seg.halves + 1) / 2 : seg.halves / 2;
       const int first_tok = seg.mode == kPair ? s * a.tile_tokens : 0;
       const int rows = min(a.tile_tokens, seg.ntok - first_tok) * a.group;
       const bool warp_live = (warp & 3) * 32 < rows;
       // keys of the item this row sees, less those before the current step's
       int lim = 0;
       if (row < rows) lim = seg.b < 0 ? seg.kend : clamp32(seg.vis0 + token_in_tile, 0, seg.kend);
-      lim -= (seg.t0 + (split ? s : 0)) * kTile;
+      lim -= seg.t0 * kTile + (split ? s * kHalf : 0);
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int i = 0; i < steps; ++i) {
+        const uint32_t buf = count & 1u;
         ok = wait_warp(&bars->s_full[s], count & 1u, abort);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          uint32_t x[kTile];  // P goes over half of S, so all of S is read first
-          ld128(ts, x);
-          if (!__all_sync(0xffffffffu, lim >= kTile || row >= rows)) {
+          uint32_t x[kHalf];
+          ld64(ts, ts + 32, x);
+          tc_fence_before();
+          arrive_warp(&bars->s_empty[s]);
+          if (!__all_sync(0xffffffffu, lim >= kHalf || row >= rows)) {
 #pragma unroll
-            for (int j = 0; j < kTile; ++j)
+            for (int j = 0; j < kHalf; ++j)
               if (j >= lim) x[j] = 0xFF800000u;  // -inf: not seen
           }
           float mx[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) mx[k] = __uint_as_float(x[k]);
 #pragma unroll
-          for (int j = 4; j + 8 <= kTile; j += 8) {
+          for (int j = 4; j + 8 <= kHalf; j += 8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               mx[k] = max3(mx[k], __uint_as_float(x[j + 2 * k]), __uint_as_float(x[j + 2 * k + 1]));
           }
-          mx[0] = max3(mx[0], __uint_as_float(x[kTile - 4]), __uint_as_float(x[kTile - 3]));
-          mx[1] = max3(mx[1], __uint_as_float(x[kTile - 2]), __uint_as_float(x[kTile - 1]));
+          mx[0] = max3(mx[0], __uint_as_float(x[kHalf - 4]), __uint_as_float(x[kHalf - 3]));
+          mx[1] = max3(mx[1], __uint_as_float(x[kHalf - 2]), __uint_as_float(x[kHalf - 1]));
           const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
           const bool grow = row < rows && (mt > m + 8.f || (m == -INFINITY && mt > -INFINITY));
           if (__any_sync(0xffffffffu, grow)) {
             const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mt)) : 1.f;
-            if (i > 0) {  // O is at rest: S was begun after the product of the step before
+            if (i > 0) {  // O is at rest once the product of the step before has ended
+              const uint32_t last = count - 1;
+              ok = wait_warp(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D; c += 16) {
                 uint32_t o[16];
@@ -944,11 +987,13 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             l *= alpha;
             m = grow ? mt : m;
           }
+          // P's buffer is free: S of this step was begun after the product of two steps before,
+          // and its barrier tells that all products begun before it have ended
           const float neg = m == -INFINITY ? 0.f : -m;
           const uint64_t scale2 = pair2(a.scale_log2, a.scale_log2), neg2 = pair2(neg, neg);
           uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             uint32_t p[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -961,24 +1006,29 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               sum[j & 3] = add2(sum[j & 3], pair2(p0, p1));
               p[j] = pack2<QT>(p0, p1);
             }
-            st16(ts + kP + 16 * q, p);
+            st16(ts + kP + 32 * buf + 16 * q, p);
           }
           float l0, l1;
           split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), l0, l1);
           l += l0 + l1;
           st_wait();
+        } else {
+          arrive_warp(&bars->s_empty[s]);
         }
         tc_fence_before();
-        arrive_warp(&bars->p_full[s]);
-        lim -= split ? 2 * kTile : kTile;
+        arrive_warp(&bars->p_full[2 * s + buf]);
+        lim -= split ? kTile : kHalf;
         ++count;
       }
       if (!ok) break;
       // ------------------------------------------------------------ the segment's partial
       // scores that are all NaN leave no maximum: any reference carries their NaN on
       if (l != l && m == -INFINITY) m = 0.f;
-      ok = wait_warp(&bars->pv[s], (count - 1) & 1u, abort);
-      if (!ok) break;
+      {
+        const uint32_t last = count - 1;
+        ok = wait_warp(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort);
+        if (!ok) break;
+      }
       if (split) {
         // Both streams' sums belong to the same rows: exchange (m, l), then each stream joins and
         // writes half of the dims. (m, l) of the split segment before were read before a stream's
