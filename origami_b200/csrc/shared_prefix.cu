@@ -92,7 +92,8 @@ int32_t launch(const origami::SharedArgs& a, cudaStream_t st) {
                         "shared_prefix_attention launch", a);
   if (rc) return rc;
   const int64_t warps = static_cast<int64_t>(a.tokens) * a.kv_heads * ((a.group + a.merge_rows - 1) / a.merge_rows);
-  return launch_dependent(&origami::merge_partials<QT, D>,
+  auto* merge = a.merge_rows == 1 ? &origami::merge_partials<QT, D, 16> : &origami::merge_partials<QT, D, 8>;
+  return launch_dependent(merge,
                           dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st,
                           "merge_partials launch", a);
 }

@@ -1114,11 +1114,12 @@ struct Parts {
 
 }  // namespace spa
 
-template <typename QT, int D>
-__global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ SharedArgs a) {
+// AHEAD: partials' loads in flight; 16 while a warp has one row and latency counts (a batch of
+// 64: 90 -> 88 us), else 8, which leaves room for a third block.
+template <typename QT, int D, int AHEAD>
+__global__ void __launch_bounds__(256, AHEAD > 8 ? 2 : 3) merge_partials(const __grid_constant__ SharedArgs a) {
   using namespace spa;
   constexpr int kPer = D / 32;  // dims per lane
-  constexpr int kAhead = 8;     // partials' loads in flight
   const int lane = threadIdx.x & 31;
   const int per_head = (a.group + a.merge_rows - 1) / a.merge_rows, per_token = a.kv_heads * per_head;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -1200,9 +1201,9 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
       }
       unsigned live = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
       while (live) {
-        float v[kAhead][kPer], wv[kAhead];
+        float v[AHEAD][kPer], wv[AHEAD];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+        for (int u = 0; u < AHEAD; ++u) {
           const int src = live ? __ffs(live) - 1 : 0;
           const float w = __shfl_sync(0xffffffffu, wgt, src);
           const float* p = a.o + (__shfl_sync(0xffffffffu, row, src) + g) * D + lane * kPer;
@@ -1222,7 +1223,7 @@ __global__ void __launch_bounds__(256) merge_partials(const __grid_constant__ Sh
           live &= live - 1;
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
+        for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
           for (int i = 0; i < kPer; ++i) acc[i] = fmaf(v[u][i], wv[u], acc[i]);
       }
