@@ -82,19 +82,22 @@ def _rotation(positions: torch.Tensor | None, cos_sin: torch.Tensor | None, inte
                          positions.data_ptr(), width)
 
 
+def _weight(w: torch.Tensor | None, name: str, head_dim: int, index: int) -> tuple[int | None, int]:
+    if w is None:
+        return None, 0
+    _on(index, w, name)
+    dtype = _DTYPE.get(w.dtype)
+    if dtype is None or w.dim() != 1 or w.shape[0] != head_dim or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float16, bfloat16 or float32 vector of {head_dim} elements")
+    return w.data_ptr(), dtype
+
+
 def _norm(query_weight: torch.Tensor | None, key_weight: torch.Tensor | None, eps: float, head_dim: int, index: int):
     if query_weight is None and key_weight is None:
         return None
-    n = _lib.HeadNorm(None, None, 0, 0, float(eps))
-    for w, name in ((query_weight, "query_weight"), (key_weight, "key_weight")):
-        if w is None:
-            continue
-        _on(index, w, name)
-        if w.dtype not in _DTYPE or w.dim() != 1 or w.shape[0] != head_dim or not w.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous float16, bfloat16 or float32 vector of {head_dim} elements")
-        setattr(n, f"d_{name}", w.data_ptr())
-        setattr(n, f"{name}_dtype", _DTYPE[w.dtype])
-    return n
+    q, q_dtype = _weight(query_weight, "query_weight", head_dim, index)
+    k, k_dtype = _weight(key_weight, "key_weight", head_dim, index)
+    return _lib.HeadNorm(q, k, q_dtype, k_dtype, eps)
 
 
 def _error(error_count: torch.Tensor | None, index: int):
@@ -106,12 +109,12 @@ def _error(error_count: torch.Tensor | None, index: int):
     return error_count.data_ptr()
 
 
-def _empty(like: torch.Tensor, shape, dtype: torch.dtype, stream: torch.cuda.Stream | None) -> torch.Tensor:
-    """A contiguous tensor on like's device, from the pool of the stream that will write it."""
+def _empty_like(t: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """A dense tensor of t's shape and type, from the pool of the stream that will write it."""
     if stream is None:
-        return like.new_empty(shape, dtype=dtype)
+        return torch.empty_like(t)
     with torch.cuda.stream(stream):
-        return like.new_empty(shape, dtype=dtype)
+        return torch.empty_like(t)
 
 
 def _launch(index: int, stream: torch.cuda.Stream | None, what: str, entry, *args) -> None:
@@ -152,9 +155,9 @@ def norm_rope(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, c
     norm = _norm(query_weight, key_weight, eps, head_dim, index)
     err = _error(error_count, index)
     if query_out is None:
-        query_out = _empty(query, query.shape, query.dtype, stream)
+        query_out = _empty_like(query, stream)
     if key_out is None:
-        key_out = _empty(key, key.shape, key.dtype, stream)
+        key_out = _empty_like(key, stream)
     qo = _rows(query_out, "query_out", tokens, head_dim, index)
     ko = _rows(key_out, "key_out", tokens, head_dim, index)
     if tokens > 0:
@@ -192,7 +195,7 @@ def append_kv(kv_layer: torch.Tensor, key: torch.Tensor, value: torch.Tensor, sl
     if query is not None:
         q = _rows(query, "query", tokens, head_dim, index)
         if query_out is None:
-            query_out = _empty(query, query.shape, query.dtype, stream)
+            query_out = _empty_like(query, stream)
         qo = _rows(query_out, "query_out", tokens, head_dim, index)
     elif query_out is not None or query_weight is not None:
         raise ValueError("query_out and query_weight need a query")

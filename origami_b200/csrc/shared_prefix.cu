@@ -81,13 +81,6 @@ int32_t launch(const origami::SharedArgs& a, cudaStream_t st) {
   int resident = 0;
   int32_t rc = persistent_slots(reinterpret_cast<const void*>(fn), smem, resident);  // raises the shared-memory limit
   if (rc) return rc;
-  // the kernel's warpgroups share out exactly the registers of this launch
-  static const int regs = [fn] {
-    cudaFuncAttributes at{};
-    return cudaFuncGetAttributes(&at, fn) == cudaSuccess ? at.numRegs : 0;
-  }();
-  if (regs != origami::spa::kRegsLaunch)
-    return fail(ORIGAMI_ERR_CUDA, "shared_prefix_attention was built with %d registers", regs);
   rc = launch_dependent(fn, dim3(static_cast<unsigned>(a.ctas)), origami::spa::kThreadsS, smem, st,
                         "shared_prefix_attention launch", a);
   if (rc) return rc;

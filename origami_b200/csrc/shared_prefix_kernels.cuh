@@ -6,8 +6,9 @@
 // pieces; a piece leaves (O, m, l) = (sum e^(s - m) v, reference maximum, sum e^(s - m)) and
 // pieces join as O = sum O_i e^(m_i - m), l = sum l_i e^(m_i - m). Softmax statistics, O and
 // the joins are fp32; the probabilities are rounded to the type of V for the product (the
-// tensor cores take both operands in one type; half a step, 2^-9 bf16 / 2^-12 fp16, relative
-// to each probability, is below the output's own rounding after averaging over keys).
+// tensor cores take both operands in one type; half a step, 2^-8 bf16 / 2^-11 fp16, of each
+// probability at most, which averages over the keys: measured against 64 bits, 2.2e-3 of the
+// output's norm in bf16 where the output's own rounding is 1.7e-3).
 //
 // Work. The prefix is one attention problem per KV head whose rows are the new tokens of ALL
 // requests x the query heads of the group: its K and V are read once for every 128 or 256
@@ -47,10 +48,6 @@ namespace spa {
 
 constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12 / 14: products of
                                 // stream 0 / 1; 13: scheduler
-// Registers per thread at launch, then of the softmax warpgroups and of the others:
-// 256 * 168 + 256 * 88 = 512 * 128, all that the block was launched with.
-constexpr int kRegsLaunch = 128, kRegsSoftmax = 168, kRegsOther = 88;
-static_assert(256 * (kRegsSoftmax + kRegsOther) <= kThreadsS * kRegsLaunch, "register shares");
 constexpr int kTile = 128;      // keys per tile, rows per row tile
 constexpr int kHalf = 64;       // keys per softmax step
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of an item of either kind.
@@ -594,7 +591,6 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   if (warp >= 8 && warp < 12) {
     // ---------------------------------------------------------------- loaders
     // Warp lw fills rows 32 lw .. 32 lw + 31 of every tile; lane l knows row 32 lw + l.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
     constexpr int kChunks = D / 8;          // 16-byte chunks per row
     constexpr int kRowsPer = 32 / kChunks;  // rows a warp copies at once
     const int lw = __shfl_sync(0xffffffffu, warp - 8, 0);
@@ -761,7 +757,6 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       }
     }
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
     if (warp == 13) {
       // -------------------------------------------------------------- scheduler
       const Deal deal = *deal_sm;
@@ -913,7 +908,6 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax of stream s
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax));
     const int s = warp >> 2;
     const int row = tid & (kTile - 1);
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);

@@ -14,11 +14,12 @@ the query's device and never synchronises. The reference's attention takes one r
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 
 import torch
 
 from origami_b200 import _lib
-from origami_b200.append import _DTYPE, _device_index, _empty, _error, _launch, _on, _rows
+from origami_b200.append import _DTYPE, _device_index, _empty_like, _error, _launch, _on, _rows
 from origami_b200.layer import paged_desc
 
 
@@ -90,11 +91,12 @@ def shared_prefix_attention(query: torch.Tensor, kv_layer: torch.Tensor, query_s
     err = _error(error_flags, index)
     scale = head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
     if out is None:
-        out = _empty(query, query.shape, query.dtype, stream)
+        out = _empty_like(query, stream)
     o = _rows(out, "out", tokens, head_dim, index)
     if workspace is None:
         need = workspace_bytes(tokens, heads, desc.num_heads, head_dim, requests, index)
-        workspace = _empty(query, (need,), torch.uint8, stream)
+        with torch.cuda.stream(stream) if stream is not None else nullcontext():
+            workspace = query.new_empty((need,), dtype=torch.uint8)
     _on(index, workspace, "workspace")
     if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 tensor")
