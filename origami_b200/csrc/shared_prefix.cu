@@ -162,8 +162,6 @@ int32_t origami_shared_prefix_attention(
     return fail(ORIGAMI_ERR_INVALID, "suffix_blocks must be an int32 device array");
   if (suffix_stride < 0) return fail(ORIGAMI_ERR_INVALID, "suffix_blocks has a negative stride");
   if (d_lse != nullptr && !aligned(d_lse, 4)) return fail(ORIGAMI_ERR_INVALID, "lse must be a float32 device array");
-  int sms = 0;
-  if ((rc = device_sms(sms))) return rc;
   // every item's cost, at most, has to fit the 31-bit cost axis of the deal
   const int64_t per_tile = origami::spa::kTile / (query->num_heads / cache->num_heads);
   const int64_t row_tiles = (tokens + per_tile - 1) / per_tile;
@@ -175,6 +173,8 @@ int32_t origami_shared_prefix_attention(
                       (static_cast<double>(row_tiles) * cost(prefix_tokens, origami::spa::kCostPair) +
                        static_cast<double>(row_tiles + requests) * cost(suffix_cap, origami::spa::kCostTile));
   if (most >= 2147483648.0) return fail(ORIGAMI_ERR_UNSUPPORTED, "too many tiles of keys and query rows for one call");
+  int sms = 0;
+  if ((rc = device_sms(sms))) return rc;
   const Workspace w = plan(tokens, query->num_heads, cache->num_heads, head_dim, requests, sms);
   if (d_workspace == nullptr || workspace_bytes < w.bytes || !aligned(d_workspace, 16))
     return fail(ORIGAMI_ERR_INVALID, "workspace must be 16-byte aligned and hold %lld bytes",

@@ -123,6 +123,11 @@ CASES = [  # new, suffix, prefix, Hq, Hk, D, block size
     ([1], [5], 40000, 8, 1, 128, 16),                 # one long prefix over every CTA
     ([1], [30000], 5, 8, 1, 128, 16),                 # one long suffix over every CTA
     ([2] * 300, [2 + i % 200 for i in range(300)], 90, 2, 2, 64, 16),
+    # blocks of 8, 24, 64 and 256 rows: every size of box, boxes beside rows copied one by one
+    ([1, 2, 1], [200, 129, 31], 517, 8, 2, 128, 8),
+    ([1, 2, 1], [200, 129, 31], 517, 8, 2, 64, 24),
+    ([1] * 50, [1 + 13 * i for i in range(50)], 1025, 16, 4, 128, 64),
+    ([3, 1], [700, 300], 900, 8, 2, 64, 256),
 ]
 
 
@@ -209,6 +214,49 @@ def test_non_finite_values_reach_their_rows_only(cuda):
     x.q[0, 0, 0] = float("nan")
     out = x.run()
     assert bool(torch.isnan(out[0, 0]).all()) and bool(torch.isfinite(out[0, 1:]).all())
+
+
+@pytest.mark.parametrize("B, Hq, Hk, D, prefix", [(64, 32, 8, 128, 16384), (200, 32, 8, 128, 8192), (96, 8, 2, 64, 20000)])
+def test_under_load(cuda, B, Hq, Hk, D, prefix):
+    """Segments of every kind in every CTA with the memory busy: the same bits each time."""
+    x = Batch(cuda, [1] * B, [1 + 37 * i % 700 for i in range(B)], prefix, Hq, Hk, D, 16, BF16, seed=B)
+    flags = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = x.run(error_flags=flags)
+    x.check(out)
+    for _ in range(20):
+        assert torch.equal(x.run(error_flags=flags), out)
+    assert int(flags) == 0
+
+
+def test_tokens_before_the_first_request_and_empty_tables(cuda):
+    x = Batch(cuda, [2, 1], [3, 0], 70, 4, 2, 64, 16, BF16, seed=13)
+    wide = torch.cat([torch.full_like(x.q[:2], float("nan")), x.q])
+    out = torch.full_like(wide, 7.0)
+    x.run(query=wide, query_start=x.query_start + 2, out=out)
+    x.check(out[2:])
+    assert bool((out[:2] == 7.0).all())
+    # no suffix columns at all, and no prefix either
+    x.suffix, x.skv = [0, 0], [kv[:, :0] for kv in x.skv]
+    x.check(x.run(suffix_blocks=x.suffix_blocks[:, :0]))
+    out = x.run(suffix_blocks=x.suffix_blocks[:, :0], prefix_blocks=x.prefix_blocks[:0], prefix_tokens=0)
+    assert not out.any()
+
+
+def test_calls_that_share_a_workspace_in_turn(cuda):
+    """Other shapes, and a captured call, over the workspace another call left behind."""
+    x = Batch(cuda, [1] * 3, [20, 300, 4], 500, 8, 2, 128, 16, BF16, seed=14)
+    y = Batch(cuda, [5, 1], [5, 90], 40, 32, 2, 64, 16, F16, seed=15)
+    need = max(shared_prefix.workspace_bytes(3, 8, 2, 128, 3, cuda), shared_prefix.workspace_bytes(6, 32, 2, 64, 2, cuda))
+    ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+    a, b = x.run(), y.run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ga = x.run(workspace=ws)
+    for _ in range(3):
+        assert torch.equal(y.run(workspace=ws), b)
+        graph.replay()
+        assert torch.equal(ga, a)
+        assert torch.equal(y.run(workspace=ws), b)
 
 
 def test_streams_graph_and_changed_lengths(cuda):
