@@ -317,10 +317,10 @@ __device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t ta, u
       "r"(ta), "l"(db), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
+__device__ __forceinline__ void commit(uint32_t lead, uint32_t bar) {
   asm volatile(
       "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
-      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
       "r"(lead)
       : "memory");
 }
@@ -377,14 +377,17 @@ __device__ __forceinline__ float ex2(float x) {
 
 // A warp's bounded wait, agreed by its lanes, that gives up early when another role has. The
 // ready barrier costs one poll and one vote; the loop is kept short, as every role has several.
-__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ uint32_t try_bar(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
+      : "r"(bar), "r"(parity)
       : "memory");
-  return __all_sync(0xffffffffu, done != 0) != 0;
+  return done;
+}
+__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, try_bar(smem_u32(bar), parity) != 0) != 0;
 }
 constexpr uint32_t kPolls = 1u << 19;  // about 2 s, far beyond any copy or product
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
@@ -791,6 +794,10 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t lead = elect_one();
       auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_warp(bar, parity, abort); };
+      auto at = [&](const void* bar) { return __shfl_sync(0xffffffffu, smem_u32(bar), 0); };
+      const uint32_t full_own = at(&bars->full[s][0]), full_both = at(&bars->full[2][0]), empty = at(&bars->empty[0]);
+      const uint32_t s_full = at(&bars->s_full[s]), s_empty = at(&bars->s_empty[s]);
+      const uint32_t p_full = at(&bars->p_full[2 * s]), pv = at(&bars->pv[2 * s]);
       // stages of the tiles that S and P V use next (K and V alternate in the ring); phases of this
       // stream's own full barriers and of the shared ones, a bit per stage
       uint32_t k_stage = 0u, v_stage = 1u, own = 0u, both = 0u;
@@ -821,35 +828,40 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         const int odd = mode == kSplit ? 0 : 1;  // a tile's first step has (g & odd) == 0, its last odd, or ends the segment
         const uint32_t half0 = mode == kSplit ? s * (kHalf * 128) : 0u;
         const uint64_t qd = desc128(base + qb * S::tile, 16);
-        auto wait_full = [&](uint32_t stage) {
-          const bool full = wait(&bars->full[readers(mode)][stage], ((mode < kSolo ? both : own) >> stage) & 1u);
-          if (mode < kSolo) both ^= 1u << stage;
-          else own ^= 1u << stage;
-          return full;
-        };
+        const bool solo = mode >= kSolo;
+        const uint32_t full = solo ? full_own : full_both;
+        uint32_t bits = solo ? own : both;  // phases of the full barriers of these tiles' readers
         // A tile and a Q buffer are freed by two arrivals: one of each stream that reads it, or
         // both of the only one.
         auto free_tile = [&](uint32_t stage) {
-          commit(lead, &bars->empty[stage]);
-          if (mode >= kSolo) commit(lead, &bars->empty[stage]);
+          commit(lead, empty + 8 * stage);
+          if (solo) commit(lead, empty + 8 * stage);
+          bits ^= 1u << stage;
         };
         auto free_q = [&]() {
-          commit(lead, &bars->q_empty[qb]);
-          if (mode != kSplit) commit(lead, &bars->q_empty[qb]);
+          commit(lead, smem_u32(&bars->q_empty[qb]));
+          if (mode != kSplit) commit(lead, smem_u32(&bars->q_empty[qb]));
+        };
+        // The two barriers that a product waits for are tried together: ready, as they mostly are,
+        // they cost one vote.
+        auto wait2 = [&](uint32_t b0, uint32_t parity0, bool need0, uint32_t b1, uint32_t parity1, bool need1) {
+#pragma unroll 1
+          for (uint32_t i = 0; i < kPolls; ++i) {
+            const uint32_t d0 = need0 ? try_bar(b0, parity0) : 1u, d1 = need1 ? try_bar(b1, parity1) : 1u;
+            if (__all_sync(0xffffffffu, (d0 & d1) != 0)) return true;
+            if (__any_sync(0xffffffffu, *abort)) return false;
+          }
+          *abort = 1;
+          return false;
         };
         // S of step g + 1 is begun before P V of step g
 #pragma unroll 1
         for (int g = -1; g < steps; ++g) {
           if (g + 1 < steps) {
             const int x = g + 1;
-            if ((x & odd) == 0 && !wait_full(k_stage)) {
-              ok = false;
-              break;
-            }
-            if (n_s > 0 && !wait(&bars->s_empty[s], (n_s - 1) & 1u)) {  // the last S has been read
-              ok = false;
-              break;
-            }
+            // the tile is there and the last S has been read
+            ok = wait2(full + 8 * k_stage, (bits >> k_stage) & 1u, (x & odd) == 0, s_empty, (n_s - 1) & 1u, n_s > 0);
+            if (!ok) break;
             tc_fence_after();
             const uint32_t d = tm + 256 * s;
             const uint64_t kd = desc128(base + S::ring + k_stage * S::tile + half0 + (x & odd) * (kHalf * 128), 16);
@@ -858,7 +870,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
               mma_ss(lead, d, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
             }
-            commit(lead, &bars->s_full[s]);
+            commit(lead, s_full);
             ++n_s;
             if ((x & odd) == odd || x == steps - 1) {
               free_tile(k_stage);
@@ -867,15 +879,13 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
             if (x == steps - 1) free_q();
           }
           if (g >= 0) {
-            if ((g & odd) == 0 && !wait_full(v_stage)) {
-              ok = false;
-              break;
+            if (g == 0 && n_seg > 0) {  // the last segment's O has been read
+              ok = wait(&bars->o_free[s], (n_seg - 1) & 1u);
+              if (!ok) break;
             }
-            if (!wait(&bars->p_full[2 * s + (n_pv & 1u)], (n_pv >> 1) & 1u) ||
-                (g == 0 && n_seg > 0 && !wait(&bars->o_free[s], (n_seg - 1) & 1u))) {  // the last segment's O has been read
-              ok = false;
-              break;
-            }
+            ok = wait2(full + 8 * v_stage, (bits >> v_stage) & 1u, (g & odd) == 0, p_full + 8 * (n_pv & 1u),
+                       (n_pv >> 1) & 1u, true);
+            if (!ok) break;
             tc_fence_after();
             const uint32_t d = tm + 256 * s + kO, p = tm + 256 * s + kP + 32 * (n_pv & 1u);
             const uint64_t vd =
@@ -883,7 +893,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
 #pragma unroll
             for (int k = 0; k < kHalf / 16; ++k)
               mma_ts(lead, d, p + k * 8, vd + k * (2048 >> 4), kIdescO, (g > 0 || k > 0) ? 1u : 0u);
-            commit(lead, &bars->pv[2 * s + (n_pv & 1u)]);
+            commit(lead, pv + 8 * (n_pv & 1u));
             ++n_pv;
             if ((g & odd) == odd || g == steps - 1) {
               free_tile(v_stage);
@@ -894,15 +904,17 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         if (!ok) break;
         ++n_seg;
         if (mode == kSplit && steps < n) {  // the last tile has no keys for this stream: seen and freed
-          ok = wait_full(k_stage) && wait_full(v_stage);
+          ok = wait2(full + 8 * k_stage, (bits >> k_stage) & 1u, true, full + 8 * v_stage, (bits >> v_stage) & 1u, true);
           free_tile(k_stage);
           free_tile(v_stage);
           next_tile(k_stage);
           next_tile(v_stage);
         }
+        if (solo) own = bits;
+        else both = bits;
       }
       // nothing may be in flight when the columns are released
-      commit(lead, &bars->done);
+      commit(lead, smem_u32(&bars->done));
       mbar_wait_bounded(&bars->done, 0u, kPolls);
     }
     __syncwarp();
