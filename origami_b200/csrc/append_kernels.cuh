@@ -12,12 +12,19 @@
 //
 // Bound: bytes. Every element is read once and written once and nothing else scales with the
 // row, so the design only has to keep enough loads in flight and spend few instructions:
-// a lane holds 16 elements of a head as two 8-element chunks that contain both members of
-// each of its pairs (chunks c and c + R/16 for halves, 2c and 2c + 1 interleaved), so the
-// rotation needs no exchange between lanes, the norm is log2(lanes per head) shuffles, and
-// the 8 (cos, sin) and the weights a lane needs are loaded once for all the heads it walks of
-// its token. A walker's key and value rows and its first query rows are all requested before
-// the first is used.
+// - a lane holds 16 elements of a head as two 8-element chunks that contain both members of
+//   each of its pairs (chunks c and c + R/16 for halves, 2c and 2c + 1 interleaved), so the
+//   rotation needs no exchange between lanes and the norm is log2(lanes per head) shuffles;
+//   chunks of 4 halve the registers but double the instructions (147 us instead of 98 for
+//   16384 tokens of 32 + 8 heads of 128, both with one token per walker);
+// - a walker steps through tokens with a fixed set of heads: addresses, weights (fp32, in shared
+//   memory) and roles are set up once, the next token's position and slot are loaded a token
+//   ahead, and a token's key, value and first query rows and its table row are all requested
+//   before the first is used;
+// - fp32 arithmetic in pairs (f32x2).
+// Measured on bf16, halves, with norm: 16384 tokens of 32 query and 8 KV heads of 128, 344 MB,
+// 72 us (4.8 TB/s, 0.74 of the copy rate); append of 32768 such tokens, 822 MB, 154 us (5.3
+// TB/s, 0.83). What remains is latency at 16 warps an SM: a third block (80 registers) spills.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -60,9 +67,7 @@ struct AppendArgs {
 namespace app {
 
 constexpr int kF16 = 1, kBF16 = 2, kF32 = 3;
-// Query heads a lane has in flight (beside a key and a value head).
-template <typename T>
-__host__ __device__ constexpr int unroll() { return sizeof(T) == 4 ? 1 : 2; }
+constexpr int kUnroll = 2;  // query heads a lane has in flight (beside a key and a value head)
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -194,16 +199,18 @@ struct Place {
   int64_t position;
   bool rotates;       // false: position outside the table, no row of the token is written
 };
-__device__ __forceinline__ Place place_of(const AppendArgs& a, int64_t t, uint32_t& skipped) {
-  Place p{-1, 0, true};
+// What the lists hold for a token; loaded a token ahead by the kernel that steps through them.
+struct Listed {
+  int64_t slot, position;
+  __device__ __forceinline__ Listed(const AppendArgs& a, int64_t t)
+      : slot(a.slots ? index_at(a.slots, a.slots64, t) : -1), position(a.positions ? index_at(a.positions, a.positions64, t) : 0) {}
+};
+__device__ __forceinline__ Place place_of(const AppendArgs& a, const Listed& listed, uint32_t& skipped) {
+  Place p{-1, listed.position, true};
   skipped = 0;
-  int64_t slot = -1;
-  if (a.slots) slot = index_at(a.slots, a.slots64, t);
+  const int64_t slot = listed.slot;
   const bool in_cache = slot >= 0 && slot < a.num_slots;
-  if (a.positions) {
-    p.position = index_at(a.positions, a.positions64, t);
-    p.rotates = p.position >= 0 && p.position < a.max_positions;
-  }
+  if (a.positions) p.rotates = p.position >= 0 && p.position < a.max_positions;
   if (in_cache)
   {
     int64_t block;
@@ -231,7 +238,7 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int64_t t, uint32
 template <typename TI, typename TC, bool FULL>
 __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ AppendArgs a) {
   using namespace app;
-  constexpr int U = unroll<TI>();
+  constexpr int U = kUnroll;
   __shared__ __align__(16) float w_sm[2][512];
   const int lph = 1 << a.lanes_log2;
   const int lane = threadIdx.x & (lph - 1);
@@ -318,12 +325,20 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
     }
   };
   // uniform trip counts: the walkers of a warp shuffle together
-#pragma unroll 1
   // (walkers beyond the last whole token of a pass have none)
-  for (int64_t t = first < a.step ? first : a.tokens; __any_sync(0xffffffffu, t < a.tokens); t += a.step) {
+  int64_t t = first < a.step ? first : a.tokens;
+  Listed listed(a, min64(t, a.tokens - 1));
+#pragma unroll 1
+  for (; __any_sync(0xffffffffu, t < a.tokens); t += a.step) {
     const bool live = t < a.tokens;
     // rows that a walker does not have are read as its neighbours' and not stored
     const int64_t tr = live ? t : a.tokens - 1;
+    Place pl{-1, 0, false};
+    if (live) {
+      uint32_t skipped;
+      pl = place_of(a, listed, skipped);
+      if (skipped && g == 0 && lane == 0 && a.err) atomicAdd(a.err, skipped);
+    }
     Raw8<TI> xk[2], xv[2], xq[U][2];
     if (a.k.heads > 0) fetch(a.k.in, tr * a.k.in_token + k_in, xk);
     if (a.v.heads > 0) fetch(a.v.in, tr * a.v.in_token + v_in, xv);
@@ -332,17 +347,12 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
 #pragma unroll
       for (int j = 0; j < U; ++j) fetch(a.q.in, q_at + min64(q0 + j, q_last) * a.q.in_head, xq[j]);
     }
-    Place pl{-1, 0, false};
-    if (live) {
-      uint32_t skipped;
-      pl = place_of(a, t, skipped);
-      if (skipped && g == 0 && lane == 0 && a.err) atomicAdd(a.err, skipped);
-    }
     if (pl.rotates && turns && (has_k || q0 < q1)) {
       const int64_t row = pl.position * a.table_stride + 8 * lane;
       small8(a.table, a.table_dtype, row, co);
       small8(a.table, a.table_dtype, row + (a.R >> 1), si);
     }
+    listed = Listed(a, min64(t + a.step, a.tokens - 1));
     TC* cache_row = static_cast<TC*>(a.cache) + pl.cache_row;
     if (a.k.heads > 0) {
       float f[16];
@@ -391,7 +401,7 @@ __global__ void __launch_bounds__(256) append_rows_any(const __grid_constant__ A
   const HeadRows& r = is_q ? a.q : is_k ? a.k : a.v;
   const int h = is_q ? u : is_k ? u - a.q.heads : u - a.q.heads - a.k.heads;
   uint32_t skipped;
-  const Place pl = place_of(a, t, skipped);
+  const Place pl = place_of(a, Listed(a, t), skipped);
   if (u == 0 && lane == 0 && skipped && a.err) atomicAdd(a.err, skipped);
   if (!pl.rotates || (!r.out && pl.cache_row < 0)) return;
   const TI* x = static_cast<const TI*>(r.in) + t * r.in_token + h * r.in_head;
