@@ -407,11 +407,13 @@ int32_t origami_append_kv(const origami_head_rows* key, const origami_head_rows*
  * zero K and V (the key still takes part in the softmax with score 0); query tokens outside
  * [query_start[0], query_start[requests]) are left as they are in output and lse. The lists
  * are device int32; lengths are clamped to the tables (suffix_lens to suffix_width *
- * block_size, query_start to [0, tokens]).
+ * block_size, query_start to [0, tokens]). If query_start decreases anywhere, nothing is
+ * written and bit 30 of d_error_flags is set.
  * query, output and cache share a type (F16 or BF16); head_dim is 64 or 128, the query heads
  * of a KV head at most 128. lse (nullable, [tokens, query_heads] contiguous) gets the natural
  * logarithm of each row's sum of exponentials. Keys and values past the last one that any of
- * a request's rows sees are never read.
+ * a request's rows sees are never read. A value that a row does not see but a later row of
+ * its request does meets it with weight zero: if it is infinite or NaN, so becomes the row.
  * d_workspace: origami_shared_prefix_attention_workspace() bytes, 16-byte aligned; its
  * contents need no preparation and mean nothing between calls; calls that share it must not
  * overlap. d_error_flags (nullable) gets bit 31 if a bounded wait inside the kernel ran out.

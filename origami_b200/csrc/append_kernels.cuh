@@ -23,8 +23,8 @@
 //   before the first is used;
 // - fp32 arithmetic in pairs (f32x2).
 // Measured on bf16, halves, with norm: 16384 tokens of 32 query and 8 KV heads of 128, 344 MB,
-// 72 us (4.8 TB/s, 0.74 of the copy rate); append of 32768 such tokens, 822 MB, 154 us (5.3
-// TB/s, 0.83). What remains is latency at 16 warps an SM: a third block (80 registers) spills.
+// 73 us (4.7 TB/s, 0.73 of the copy rate); append of 32768 such tokens, 822 MB, 158 us (5.2
+// TB/s, 0.81). What remains is latency at 16 warps an SM: a third block (80 registers) spills.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -211,8 +211,7 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, const Listed& lis
   const int64_t slot = listed.slot;
   const bool in_cache = slot >= 0 && slot < a.num_slots;
   if (a.positions) p.rotates = p.position >= 0 && p.position < a.max_positions;
-  if (in_cache)
-  {
+  if (in_cache) {
     int64_t block;
     if (((slot | a.block_size) >> 31) == 0) block = static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.block_size);
     else block = slot / a.block_size;

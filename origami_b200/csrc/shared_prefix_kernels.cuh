@@ -21,17 +21,27 @@
 // A CTA: 4 loader warps gather K and V tiles through the block tables into a ring of
 // 128-byte-swizzled tiles, by TMA where a block's rows come in eights (a box per block), else
 // and where a tile ends inside with 16-byte cp.async (rows past the end become zeros, so
-// garbage there cannot reach the products); one warp per stream issues its tcgen05.mma; two softmax
+// garbage there cannot reach the products; all by cp.async: 102 / 150 / 225 us for the three cases
+// measured below); one warp per stream issues its tcgen05.mma; two softmax
 // warpgroups own one stream each, a stream being, in TMEM, 64 keys' scores, two buffers of P and O:
 //   S_s [128 rows x 64 keys] = Q K^T (shared memory operands),
 //   O_s [128 rows x D]      += P V   (P in TMEM, V the N-major B operand).
 // The next scores are begun as soon as a step has read its own, so a stream's chain is its
 // softmax alone. One thread owns one row: the softmax needs no exchange. O is rescaled only when the
-// maximum grew by more than 2^8 (P stays below 2^8, exact in the same relative precision).
+// maximum grew by more than 2^8 (P stays below 2^8, exact in the same relative precision; each
+// time it grows, the batch of 256 takes 256 us instead of 209).
 // With more than 128 rows an item has two row tiles, one per stream, that share each K and V
 // tile ("pair"); with fewer, the streams take one half of each key tile for one row tile and
 // join at the end of the segment ("split"); segments of one tile go to the streams in turn
 // ("solo"), so that one's epilogue runs under the other's work.
+//
+// Measured (cold L2, both launches): 64 requests over 32768 shared keys and up to 1024 own, 32 / 8
+// heads of 128, 282 MB, 35 GFLOP: 86 us; 8 requests over 131072, 64 / 8 heads, 616 MB: 127 us (4.9
+// TB/s, 0.75 of the copy rate, by the ring's stages in flight); 256 requests over 32768, 138 GFLOP:
+// 209 us. There a pair of streams' steps of 64 keys takes about 1850 clocks, its products alone
+// 1304 (Q K^T at N = 64 takes 49 clocks per 16 dims, bound by its shared-memory operands, where
+// N = 128 takes 65), softmax 1027 of ex2: the products' chain bounds. Steps of 128 keys have
+// cheaper products but leave TMEM for one S a stream, with P over it: 223 us.
 #pragma once
 
 #include <cuda.h>
@@ -48,9 +58,14 @@ namespace spa {
 
 constexpr int kThreadsS = 512;  // warps 0-3 / 4-7: softmax of stream 0 / 1; 8-11: loaders; 12 / 14: products of
                                 // stream 0 / 1; 13: scheduler
+constexpr uint32_t kQueryStartFlag = 0x40000000u;  // of d_error_flags: query_start decreases
 constexpr int kTile = 128;      // keys per tile, rows per row tile
 constexpr int kHalf = 64;       // keys per softmax step
-// Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of an item of either kind.
+// Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of
+// an item of either kind (its prologue, epilogue and partial). Chunks (13 requests of up to 300
+// tokens, D 64) / batch of 64 / batch of 256 over 32768 keys, us, cold L2: 86 / 86 / 209 so; a
+// pair's tile at 8: 90 / 100 / 232, at 16: 96 / 84 / 231; items for nothing: 96 / 86 / 272, a
+// pair's at 8: 86 / 90 / 211, a single's at 16: 88 / 92 / 229.
 constexpr int kCostTile = 8, kCostPair = 12, kCostItem = 8, kCostPairItem = 22;
 
 // Shared memory: Q tiles, then the ring of K / V tiles (each [128][D] 16-bit), then scalars.
@@ -91,7 +106,7 @@ struct SharedArgs {
   uint32_t inv_ctas;         // floor(2^32 / ctas)
   float scale_log2;
   // workspace
-  int32_t* head;      // suffix cost of one head
+  int32_t* head;      // suffix cost of one head, -1 if the call is refused
   int32_t* req_cost;  // [requests] suffix cost of the requests before this one
   float* ml;          // [rows][2]
   float* o;           // [rows][D]
@@ -525,8 +540,12 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     const int b0 = min(tid * per, a.requests), b1 = min(b0 + per, a.requests);
     const int used = used_tokens(a);
     int sum = 0;
+    bool falls = false;  // query_start does: requests would share tokens, and their costs have no bound
 #pragma unroll 1
-    for (int b = b0; b < b1; ++b) sum += request_cost(a, Request(a, b));
+    for (int b = b0; b < b1; ++b) {
+      sum += request_cost(a, Request(a, b));
+      falls |= __ldg(a.query_start + b + 1) < __ldg(a.query_start + b);
+    }
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -534,7 +553,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       if (lane >= o) incl += v;
     }
     if (lane == 31) scan[warp] = incl;
-    __syncthreads();
+    const bool refused = __syncthreads_or(falls) != 0;
     int before = lane < kThreadsS / 32 ? scan[lane] : 0, total = before;
     if (lane >= warp) before = 0;
 #pragma unroll
@@ -543,9 +562,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       total += __shfl_xor_sync(0xffffffffu, total, o);
     }
     before = __shfl_sync(0xffffffffu, before, 0);
-    total = __shfl_sync(0xffffffffu, total, 0);
+    total = refused ? 0 : __shfl_sync(0xffffffffu, total, 0);
     const int excl = before + incl - sum;
-    const int wp = prefix_cost(a, used), all_p = wp * a.kv_heads, all = all_p + total * a.kv_heads;
+    const int wp = refused ? 0 : prefix_cost(a, used), all_p = wp * a.kv_heads, all = all_p + total * a.kv_heads;
     const int w0 = share_begin(a, all, cta);
     // the share's first suffix item lies in the run of requests that holds its cost
     const int y = max(w0 - all_p, 0), fh = total > 0 ? y / total : a.kv_heads, rem = total > 0 ? y - fh * total : 0;
@@ -559,9 +578,10 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
         deal_sm->b = deal_sm->tile = 0;
         deal_sm->start = all_p;
       }
-      if (cta == 0) *a.head = total;
+      if (cta == 0) *a.head = refused ? -1 : total;
+      if (cta == 0 && refused && a.err) atomicOr(a.err, kQueryStartFlag);
     }
-    if ((sum > 0 && rem >= excl && rem < excl + sum) || cta == 0) {
+    if (!refused && ((sum > 0 && rem >= excl && rem < excl + sum) || cta == 0)) {
       int at = excl;
 #pragma unroll 1
       for (int b = b0; b < b1; ++b) {
@@ -1137,7 +1157,10 @@ __global__ void __launch_bounds__(256, AHEAD > 8 ? 2 : 3) merge_partials(const _
   // the request: token t itself in a step of one token each, else by bisection
   int b = clamp32(t, 0, a.requests - 1);
   const int first = __ldg(a.query_start), lo0 = __ldg(a.query_start + b), hi0 = __ldg(a.query_start + b + 1);
-  if (t >= used || t < first) return;
+  if (t >= used || t < first) {  // (a launch that ends before its wait could let the stream run ahead of the first kernel)
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    return;
+  }
   if (t < lo0 || t >= hi0) {
     int lo = 0, hi = a.requests;  // query_start[lo] <= t < query_start[hi]
     while (hi - lo > 1) {
@@ -1158,6 +1181,7 @@ __global__ void __launch_bounds__(256, AHEAD > 8 ? 2 : 3) merge_partials(const _
   const int wp = prefix_cost(a, used), per = prefix_item_tokens(a, used), pi = t / per;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int ws = __ldcg(a.head);
+  if (ws < 0) return;
   before += __ldcg(a.req_cost + b);
   const int all = (wp + ws) * a.kv_heads;
   const float shares = static_cast<float>(a.ctas) / static_cast<float>(all);

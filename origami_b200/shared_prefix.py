@@ -62,11 +62,13 @@ def shared_prefix_attention(query: torch.Tensor, kv_layer: torch.Tensor, query_s
     alone). All int32 on the device. query, out and kv_layer share a type (bf16 or fp16) and
     D is 64 or 128; softmax_scale defaults to D ** -0.5. lse [T, Hq] float32, optional,
     receives each row's log of the sum of exponentials. A row without keys gives zeros and
-    -inf; a block id outside the cache reads as zero keys and values that still take part.
+    -inf; a block id outside the cache reads as zero keys and values that still take part. A
+    value that a row does not see but a later row of its request does meets it with weight
+    zero: if it is infinite or NaN, so becomes the row.
 
     workspace: a uint8 tensor of workspace_bytes(...) bytes, allocated per call when omitted;
     calls that share one must not overlap. error_flags (int32): bit 31 is set if a bounded
-    wait inside the kernel ran out."""
+    wait inside the kernel ran out, bit 30 if query_start decreases (nothing is written then)."""
     index = _device_index(query, "query")
     if query.dim() != 3:
         raise ValueError(f"query must have shape [tokens, heads, head_dim], got {tuple(query.shape)}")

@@ -242,6 +242,19 @@ def test_tokens_before_the_first_request_and_empty_tables(cuda):
     assert not out.any()
 
 
+def test_query_start_that_falls_or_is_empty_writes_nothing(cuda):
+    x = Batch(cuda, [2, 1, 1], [30, 9, 200], 70, 4, 2, 64, 16, BF16, seed=16)
+    flags = torch.zeros(1, dtype=torch.int32, device=cuda)
+    want, lse = x.run(), torch.full((4, 4), 5.0, device=cuda)
+    ws = torch.empty(shared_prefix.workspace_bytes(4, 4, 2, 64, 3, cuda), dtype=torch.uint8, device=cuda)
+    for starts, flag in (([0, 3, 2, 4], 1 << 30), ([4, 0, 4, 0], 1 << 30), ([0, 0, 0, 0], 0)):
+        out = torch.full_like(x.q, 7.0)
+        flags.zero_()
+        x.run(query_start=torch.tensor(starts, dtype=torch.int32, device=cuda), out=out, lse=lse, error_flags=flags, workspace=ws)
+        assert bool((out == 7.0).all()) and bool((lse == 5.0).all()) and int(flags) == flag, starts
+        assert torch.equal(x.run(workspace=ws), want)
+
+
 def test_calls_that_share_a_workspace_in_turn(cuda):
     """Other shapes, and a captured call, over the workspace another call left behind."""
     x = Batch(cuda, [1] * 3, [20, 300, 4], 500, 8, 2, 128, 16, BF16, seed=14)
