@@ -53,7 +53,7 @@ Workspace plan(int64_t tokens, int64_t query_heads, int64_t kv_heads, int64_t he
   w.req_cost = kAlign;
   w.ml = w.req_cost + round_up(requests * 4, kAlign);
   w.o = w.ml + round_up(rows * 8, kAlign);
-  w.bytes = w.o + round_up(rows * head_dim * 4, kAlign);
+  w.bytes = w.o + round_up(rows * head_dim * 4, kAlign) + 16;  // 16: to a 32-byte boundary, for whole-sector stores
   return w;
 }
 
@@ -234,7 +234,7 @@ int32_t origami_shared_prefix_attention(
   // issue slots on (86 us for 2100 tokens of 16 heads that take 115 with a warp per row).
   a.merge_rows = static_cast<int32_t>(std::clamp<int64_t>(tokens * a.q_heads / (16 * sms), 1, a.group));
   a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
-  uint8_t* ws = static_cast<uint8_t*>(d_workspace);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<int64_t>(d_workspace), 32));
   a.head = reinterpret_cast<int32_t*>(ws);
   a.req_cost = reinterpret_cast<int32_t*>(ws + w.req_cost);
   a.ml = reinterpret_cast<float*>(ws + w.ml);

@@ -262,6 +262,7 @@ def test_calls_that_share_a_workspace_in_turn(cuda):
     need = max(shared_prefix.workspace_bytes(3, 8, 2, 128, 3, cuda), shared_prefix.workspace_bytes(6, 32, 2, 64, 2, cuda))
     ws = torch.empty(need, dtype=torch.uint8, device=cuda)
     a, b = x.run(), y.run()
+    assert torch.equal(x.run(workspace=torch.empty(need + 16, dtype=torch.uint8, device=cuda)[16:]), a)  # 16-byte aligned
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         ga = x.run(workspace=ws)
