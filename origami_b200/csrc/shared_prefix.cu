@@ -39,7 +39,7 @@ int32_t check_shape(int64_t tokens, int64_t query_heads, int64_t kv_heads, int64
   if (head_dim != 64 && head_dim != 128)
     return fail(ORIGAMI_ERR_UNSUPPORTED, "shared-prefix attention supports head_dim 64 and 128");
   if (requests <= 0) return fail(ORIGAMI_ERR_INVALID, "at least one request is needed");
-  if (requests > (1 << 24) || tokens > (1 << 24) || query_heads > (1 << 15))
+  if (requests > (1 << 24) || tokens > (1 << 24) || query_heads > (1 << 15) || tokens * query_heads > (1 << 29))
     return fail(ORIGAMI_ERR_UNSUPPORTED, "too many query rows");
   return ORIGAMI_OK;
 }
@@ -85,7 +85,7 @@ int32_t launch(const origami::SharedArgs& a, cudaStream_t st) {
                         "shared_prefix_attention launch", a);
   if (rc) return rc;
   const int64_t warps = static_cast<int64_t>(a.tokens) * a.kv_heads * ((a.group + a.merge_rows - 1) / a.merge_rows);
-  auto* merge = a.merge_rows == 1 ? &origami::merge_partials<QT, D, 16> : &origami::merge_partials<QT, D, 8>;
+  auto* merge = a.merge_rows == 1 ? &origami::merge_partials<QT, D, false> : &origami::merge_partials<QT, D, true>;
   return launch_dependent(merge, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st, "merge_partials launch", a);
 }
 
@@ -229,10 +229,11 @@ int32_t origami_shared_prefix_attention(
   a.q_vec = rows_vec(query);
   a.o_vec = rows_vec(output);
   a.ctas = sms;
-  // One row a warp while the rows are few (their latency counts: 127 us for 8 requests over 131072 keys
-  // that take 152 with a warp per group), more when their lists' lookup would be what an SM spends its
-  // issue slots on (86 us for 2100 tokens of 16 heads that take 115 with a warp per row).
-  a.merge_rows = static_cast<int32_t>(std::clamp<int64_t>(tokens * a.q_heads / (16 * sms), 1, a.group));
+  // One row a warp while the rows are few (their latency counts: twice as many rows a warp take the
+  // batch of 64 over 32768 keys from 86 to 94 us), more when their lists' lookup would be what an SM
+  // spends its issue slots on (half as many: the batch of 256 211 us instead of 205; one each:
+  // chunks of 2100 tokens of 16 heads 115 instead of 86).
+  a.merge_rows = static_cast<int32_t>(std::clamp<int64_t>(tokens * a.q_heads / (8 * sms), 1, a.group));
   a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   uint8_t* ws = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<int64_t>(d_workspace), 32));
   a.head = reinterpret_cast<int32_t*>(ws);

@@ -1127,23 +1127,23 @@ namespace spa {
 struct Parts {
   Item it;
   int32_t first, count, stride;
-  int64_t row0;
+  int32_t row0;  // (the host keeps partial rows below 2^31)
   __device__ __forceinline__ Parts(const SharedArgs& a, const Item& item, int t, int all, float shares) : it(item) {
     // (float: off by less than one share)
     first = max(static_cast<int>(static_cast<float>(it.start) * shares) - 2, 0);
     const int last = min(static_cast<int>(static_cast<float>(it.start + it.cost()) * shares) + 2, a.ctas - 1);
     count = it.kend > 0 ? last - first + 1 : 0;
     stride = it.b < 0 ? a.item_rows_p : a.item_rows_s;
-    row0 = partial_base(a, it, first) + static_cast<int64_t>(t - it.tok0) * a.group;
+    row0 = static_cast<int32_t>(partial_base(a, it, first)) + (t - it.tok0) * a.group;
   }
 };
 
 }  // namespace spa
 
-// AHEAD: partials' loads in flight; 16 while a warp has one row and latency counts (a batch of
-// 64: 90 -> 88 us), else 8, which leaves room for a third block.
-template <typename QT, int D, int AHEAD>
-__global__ void __launch_bounds__(256, AHEAD > 8 ? 2 : 3) merge_partials(const __grid_constant__ SharedArgs a) {
+// MANY: several rows a warp.
+template <typename QT, int D, bool MANY>
+__global__ void __launch_bounds__(256, 2) merge_partials(const __grid_constant__ SharedArgs a) {
+  constexpr int kAhead = 16;  // partials' loads in flight (8: 90 us for 88 in a batch of 64)
   using namespace spa;
   constexpr int kPer = D / 32;  // dims per lane
   const int lane = threadIdx.x & 31;
@@ -1189,19 +1189,105 @@ __global__ void __launch_bounds__(256, AHEAD > 8 ? 2 : 3) merge_partials(const _
   const Parts suf(a, suffix_item(a, r, h, b, tile, a.kv_heads * wp + h * ws + before), t, all, shares);
   const int parts = pre.count + suf.count;
   // partial row of the token's first row in partial i of the list, -1 where the share holds none
-  auto place = [&](int i) -> int64_t {
+  auto place = [&](int i) -> int {
     if (i >= parts) return -1;
     const bool p = i < pre.count;
     const Item& it = p ? pre.it : suf.it;
     const int k = p ? i : i - pre.count, c = (p ? pre.first : suf.first) + k;
     if (it.tile_at(share_begin(a, all, c + 1)) <= it.tile_at(share_begin(a, all, c))) return -1;
-    return (p ? pre.row0 : suf.row0) + static_cast<int64_t>(k) * (p ? pre.stride : suf.stride);
+    return (p ? pre.row0 : suf.row0) + k * (p ? pre.stride : suf.stride);
   };
-  const int64_t mine = place(lane);
-  auto load_ml = [&](int64_t row) {
+  const int mine = place(lane);
+  auto load_ml = [&](int row) {
     return row < 0 ? make_float2(-INFINITY, 0.f) : __ldcg(reinterpret_cast<const float2*>(a.ml) + row);
   };
   const int g_end = min(g0 + a.merge_rows, a.group);
+  uint16_t* out_t = a.output + static_cast<int64_t>(t) * a.o_token + static_cast<int64_t>(h) * a.group * a.o_head + lane * kPer;
+  auto put = [&](int g, const float* f) {
+    uint16_t* out = out_t + g * a.o_head;
+    uint32_t packed[kPer / 2];
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) packed[i] = pack2<QT>(f[2 * i], f[2 * i + 1]);
+    if (a.o_vec) {
+      if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(packed[0], packed[1]);
+      else *reinterpret_cast<uint32_t*>(out) = packed[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) out[i] = static_cast<uint16_t>(packed[i / 2] >> (16 * (i & 1)));
+    }
+  };
+  auto put_lse = [&](int g, float m, float l) {
+    a.lse[static_cast<int64_t>(t) * a.q_heads + h * a.group + g] =
+        l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  };
+  const float* o_lane = a.o + lane * kPer;
+  auto load_o = [&](int row, float (&v)[kPer]) {
+    const float* p = o_lane + static_cast<int64_t>(row) * D;
+    if constexpr (kPer == 4) {
+      const float4 f = __ldcg(reinterpret_cast<const float4*>(p));
+      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else {
+      const float2 f = __ldcg(reinterpret_cast<const float2*>(p));
+      v[0] = f.x, v[1] = f.y;
+    }
+  };
+  // At most four partials, as mostly in a large batch: eight rows' weights at once, a lane for one
+  // row's one partial (chunks of 2100 tokens x 16 heads: 86 -> 74 us, both launches).
+  unsigned held = MANY ? __ballot_sync(0xffffffffu, mine >= 0) : 0u;
+  if (MANY && parts <= 32 && __popc(held) <= 4) {
+    int rows[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = __shfl_sync(0xffffffffu, mine, held ? __ffs(held) - 1 : 0);
+      rows[i] = held ? row : -1;
+      held &= held - 1;
+    }
+    const int part = lane & 3;
+    const int my_row = part == 0 ? rows[0] : part == 1 ? rows[1] : part == 2 ? rows[2] : rows[3];
+#pragma unroll 1
+    for (int gb = g0; gb < g_end; gb += 8) {
+      const int my_g = gb + (lane >> 2);
+      const float2 ml = load_ml(my_g < g_end && my_row >= 0 ? my_row + my_g : -1);
+      float m = fmaxf(ml.x, __shfl_xor_sync(0xffffffffu, ml.x, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      float wgt = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+      float l = wgt * ml.y;
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      // l > 0 wherever a key has weight; NaN stays NaN
+      wgt *= l == 0.f ? 0.f : 1.f / l;
+      const unsigned live = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+      if (a.lse && part == 0 && my_g < g_end) put_lse(my_g, m, l);
+      constexpr int kRows = kAhead / 4;  // rows in flight
+#pragma unroll 1
+      for (int r = 0; r < min(8, g_end - gb); r += kRows) {
+        float v[kRows][4][kPer];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[u][i][e] = 0.f;
+            if ((live >> (4 * (r + u) + i)) & 1u) load_o(rows[i] + gb + r + u, v[u][i]);
+          }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          float acc[kPer];
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float w = __shfl_sync(0xffffffffu, wgt, (4 * (r + u) + i) & 31);
+            // (a NaN of the sum reaches the row through the weights)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) acc[e] = fmaf(v[u][i][e], w, acc[e]);
+          }
+          if (gb + r + u < g_end) put(gb + r + u, acc);
+        }
+      }
+    }
+    return;
+  }
   float2 ml_next = load_ml(mine < 0 ? mine : mine + g0);
 #pragma unroll 1
   for (int g = g0; g < g_end; ++g) {
@@ -1212,7 +1298,7 @@ __global__ void __launch_bounds__(256, AHEAD > 8 ? 2 : 3) merge_partials(const _
     for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
 #pragma unroll 1
     for (int i0 = 0; i0 < parts; i0 += 32) {
-      const int64_t row = i0 == 0 ? mine : place(i0 + lane);
+      const int row = i0 == 0 ? mine : place(i0 + lane);
       const float2 ml = i0 == 0 ? ml_mine : load_ml(row < 0 ? row : row + g);
       float mn = fmaxf(m, ml.x);
 #pragma unroll
@@ -1231,21 +1317,15 @@ __global__ void __launch_bounds__(256, AHEAD > 8 ? 2 : 3) merge_partials(const _
       }
       unsigned live = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
       while (live) {
-        float v[AHEAD][kPer], wv[AHEAD];
+        float v[kAhead][kPer], wv[kAhead];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
+        for (int u = 0; u < kAhead; ++u) {
           const int src = live ? __ffs(live) - 1 : 0;
           const float w = __shfl_sync(0xffffffffu, wgt, src);
-          const float* p = a.o + (__shfl_sync(0xffffffffu, row, src) + g) * D + lane * kPer;
+          const int at = __shfl_sync(0xffffffffu, row, src) + g;
           wv[u] = live ? w : 0.f;
           if (live) {
-            if constexpr (kPer == 4) {
-              const float4 f = __ldcg(reinterpret_cast<const float4*>(p));
-              v[u][0] = f.x, v[u][1] = f.y, v[u][2] = f.z, v[u][3] = f.w;
-            } else {
-              const float2 f = __ldcg(reinterpret_cast<const float2*>(p));
-              v[u][0] = f.x, v[u][1] = f.y;
-            }
+            load_o(at, v[u]);
           } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) v[u][i] = 0.f;
@@ -1253,27 +1333,17 @@ __global__ void __launch_bounds__(256, AHEAD > 8 ? 2 : 3) merge_partials(const _
           live &= live - 1;
         }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
+        for (int u = 0; u < kAhead; ++u)
 #pragma unroll
           for (int i = 0; i < kPer; ++i) acc[i] = fmaf(v[u][i], wv[u], acc[i]);
       }
     }
     // l > 0 wherever a key has weight; NaN stays NaN
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t qh = static_cast<int64_t>(h) * a.group + g;
-    uint16_t* out = a.output + static_cast<int64_t>(t) * a.o_token + qh * a.o_head + lane * kPer;
-    uint32_t packed[kPer / 2];
 #pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) packed[i] = pack2<QT>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-    if (a.o_vec) {
-      if constexpr (kPer == 4) *reinterpret_cast<uint2*>(out) = make_uint2(packed[0], packed[1]);
-      else *reinterpret_cast<uint32_t*>(out) = packed[0];
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) out[i] = static_cast<uint16_t>(packed[i / 2] >> (16 * (i & 1)));
-    }
-    if (a.lse && lane == 0)
-      a.lse[static_cast<int64_t>(t) * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    for (int i = 0; i < kPer; ++i) acc[i] *= inv;
+    put(g, acc);
+    if (a.lse && lane == 0) put_lse(g, m, l);
   }
 }
 
