@@ -154,16 +154,19 @@ int32_t launch(origami::AppendArgs& a, cudaStream_t st) {
     const int64_t resident = static_cast<int64_t>(sms) * 512;
     a.groups = a.tokens * total << a.lanes_log2 <= resident ? total : std::max(a.k.heads, (a.q.heads + 3) / 4);
     const bool full = a.D == 16 << a.lanes_log2;
-    auto* fn = full ? &origami::append_rows<TI, TC, true> : &origami::append_rows<TI, TC, false>;
+    const bool stream = a.groups != total;
+    auto* fn = stream ? (full ? &origami::append_rows<TI, TC, true, true> : &origami::append_rows<TI, TC, false, true>)
+                      : (full ? &origami::append_rows<TI, TC, true, false> : &origami::append_rows<TI, TC, false, false>);
+    const int smem = stream ? origami::app::kStreamSmem<TI> : 0;
     int slots = 0;
-    const int32_t rc = persistent_slots(reinterpret_cast<const void*>(fn), 0, slots);
+    const int32_t rc = persistent_slots(reinterpret_cast<const void*>(fn), smem, slots);
     if (rc) return rc;
     const int64_t per_cta = 256 >> a.lanes_log2;  // walkers
     const int64_t needed = (a.tokens * a.groups + per_cta - 1) / per_cta;
-    // as many CTAs as fit at once, but at least one token's walkers; whole tokens per pass
-    const int64_t ctas = std::min(needed, std::max<int64_t>(slots, (a.groups + per_cta - 1) / per_cta));
+    // as many CTAs as fit at once, but at least one token's walkers (without steps: all); whole tokens per pass
+    const int64_t ctas = stream ? std::min(needed, std::max<int64_t>(slots, (a.groups + per_cta - 1) / per_cta)) : needed;
     a.step = static_cast<int32_t>(ctas * per_cta / a.groups);
-    fn<<<static_cast<unsigned>(ctas), 256, 0, st>>>(a);
+    fn<<<static_cast<unsigned>(ctas), 256, smem, st>>>(a);
     return after_launch("append_rows launch");
   }
   const int64_t ctas = (a.tokens * total + 7) / 8;

@@ -19,8 +19,8 @@
 //   16384 tokens of 32 + 8 heads of 128, both with one token per walker);
 // - a walker steps through tokens with a fixed set of heads: addresses, weights (fp32, in shared
 //   memory) and roles are set up once, the next token's position and slot are loaded a token
-//   ahead, and a token's key, value and first query rows and its table row are all requested
-//   before the first is used;
+//   ahead, its rows (16-bit: of two tokens) copied to shared memory by cp.async, each row's place
+//   refilled as soon as it has been read, so that a walker never waits with nothing requested;
 // - fp32 arithmetic in pairs (f32x2).
 // Measured on bf16, halves, with norm: 16384 tokens of 32 query and 8 KV heads of 128, 344 MB,
 // 73 us (4.7 TB/s, 0.73 of the copy rate); append of 32768 such tokens, 822 MB, 158 us (5.2
@@ -67,7 +67,13 @@ struct AppendArgs {
 namespace app {
 
 constexpr int kF16 = 1, kBF16 = 2, kF32 = 3;
-constexpr int kUnroll = 2;  // query heads a lane has in flight (beside a key and a value head)
+// Rows of a token that a walker of the streaming form has at most (key, value, query heads), and
+// the tokens that it has requested ahead, in shared memory: 96 KB a CTA.
+constexpr int kQueryRows = 4, kWalkerRows = 2 + kQueryRows;
+template <typename TI>
+constexpr int kAhead = sizeof(TI) == 4 ? 1 : 2;
+template <typename TI>
+constexpr int kStreamSmem = kAhead<TI> * kWalkerRows * 256 * 16 * static_cast<int>(sizeof(TI));
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -228,28 +234,26 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, const Listed& lis
 
 }  // namespace app
 
-// Fast kernel: D % 8 == 0, 16-byte rows, R % 16 == 0. 1 << lanes_log2 lanes per head; `groups`
-// such walkers share a token's heads: walker g takes its part of the query heads, key head g
-// and value head groups - 1 - g; or, in a step of few tokens (groups = all heads), one head.
-// A walker keeps its g and steps through the tokens, so that all but the rows, the position
-// and the slot is set up once (the weights in shared memory, in fp32). FULL: every lane has
-// both chunks (D is 16 << lanes_log2).
-template <typename TI, typename TC, bool FULL>
+// Fast kernel: D % 8 == 0, 16-byte rows, R % 16 == 0. 1 << lanes_log2 lanes ("a walker") per
+// head. STREAM: `groups` walkers share a token's heads, walker g taking up to kQueryRows query
+// heads, key head g and value head groups - 1 - g, and step through the tokens, so that all but
+// the rows, the position and the slot is set up once (the weights in shared memory, in fp32).
+// Else a walker for each head of each token. FULL: every lane has both chunks (D is 16 <<
+// lanes_log2).
+template <typename TI, typename TC, bool FULL, bool STREAM>
 __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ AppendArgs a) {
   using namespace app;
-  constexpr int U = kUnroll;
   __shared__ __align__(16) float w_sm[2][512];
   const int lph = 1 << a.lanes_log2;
   const int lane = threadIdx.x & (lph - 1);
   const int walker = static_cast<int>((blockIdx.x * blockDim.x + threadIdx.x) >> a.lanes_log2);
   const int first = walker / a.groups, g = walker - first * a.groups;
   // this walker's heads
-  const bool single = a.groups == a.q.heads + a.k.heads + a.v.heads;
-  const int kh = single ? g - a.q.heads : g;
-  const int vh = single ? g - a.q.heads - a.k.heads : a.groups - 1 - g;
+  const int kh = STREAM ? g : g - a.q.heads;
+  const int vh = STREAM ? a.groups - 1 - g : g - a.q.heads - a.k.heads;
   const bool has_k = kh >= 0 && kh < a.k.heads, has_v = vh >= 0 && vh < a.v.heads;
-  const int q_per = single ? (a.q.heads > 0 ? 1 : 0) : (a.q.heads + a.groups - 1) / a.groups;
-  const int q0 = single ? g : g * q_per, q1 = min(q0 + q_per, a.q.heads);
+  const int q_per = STREAM ? (a.q.heads + a.groups - 1) / a.groups : 1;
+  const int q0 = g * q_per, q1 = min(q0 + q_per, a.q.heads);
 
   // this lane's two chunks; D / 8 may be odd (the last lane then has one)
   const bool split = !a.interleaved && lane < (a.R >> 4);
@@ -258,18 +262,11 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
   // pairs 8 lane .. 8 lane + 7 in both arrangements
   const bool turns = a.positions && 16 * lane < a.R;
   const int64_t k_in = (has_k ? kh : 0) * a.k.in_head, v_in = (has_v ? vh : 0) * a.v.in_head;
-  const int64_t q_last = a.q.heads - 1;
   for (int i = threadIdx.x; i < a.D; i += blockDim.x) {
     if (a.q.weight) w_sm[0][i] = small_at(a.q.weight, a.q.weight_dtype, i);
     if (a.k.weight) w_sm[1][i] = small_at(a.k.weight, a.k.weight_dtype, i);
   }
   __syncthreads();
-  auto fetch = [&](const void* in, int64_t at, Raw8<TI> (&x)[2]) {
-    const TI* p = static_cast<const TI*>(in) + at;
-    if (!FULL) x[0] = x[1] = Raw8<TI>{};
-    if (has0) x[0] = load8(p + e0);
-    if (has1) x[1] = load8(p + e1);
-  };
   auto put = [&](auto* o, const float (&f)[16]) {
     using T = std::remove_reference_t<decltype(*o)>;
     if (has0) store8(o + e0, pack8<T>(f));
@@ -279,7 +276,7 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
 #pragma unroll
   for (int i = 0; i < 8; ++i) co[i] = 1.f, si[i] = 0.f;
   // norm and rotation of one head's 16 elements (the whole warp takes part in the shuffles)
-  auto turn = [&](const float* w, bool norm, const Raw8<TI> (&x)[2], float (&f)[16]) {
+  auto turn = [&](const float* w, bool norm, bool scale, bool rotate, const Raw8<TI> (&x)[2], float (&f)[16]) {
     unpack8(x[0], f);
     unpack8(x[1], f + 8);
     if (norm) {
@@ -298,14 +295,14 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
       const uint64_t inv2 = pair2(inv, inv);
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        if (i < 8 ? has0 : has1) {
+        if (scale && (i < 8 ? has0 : has1)) {
           const float4 v = *reinterpret_cast<const float4*>(w + (i < 8 ? e0 + i : e1 + i - 8));
           split2(mul2(mul2(pair2(f[i], f[i + 1]), inv2), pair2(v.x, v.y)), f[i], f[i + 1]);
           split2(mul2(mul2(pair2(f[i + 2], f[i + 3]), inv2), pair2(v.z, v.w)), f[i + 2], f[i + 3]);
         }
       }
     }
-    if (!turns) return;
+    if (!turns || !rotate) return;
     if (a.interleaved) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -323,66 +320,125 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
       }
     }
   };
-  // uniform trip counts: the walkers of a warp shuffle together
   // (walkers beyond the last whole token of a pass have none)
   int64_t t = first < a.step ? first : a.tokens;
   Listed listed(a, min64(t, a.tokens - 1));
-#pragma unroll 1
-  for (; __any_sync(0xffffffffu, t < a.tokens); t += a.step) {
-    const bool live = t < a.tokens;
-    // rows that a walker does not have are read as its neighbours' and not stored
-    const int64_t tr = live ? t : a.tokens - 1;
-    Place pl{-1, 0, false};
-    if (live) {
-      uint32_t skipped;
-      pl = place_of(a, listed, skipped);
-      if (skipped && g == 0 && lane == 0 && a.err) atomicAdd(a.err, skipped);
+  auto table = [&](const Listed& at, float (&c)[8], float (&s)[8]) {
+    if (turns && at.position >= 0 && at.position < a.max_positions) {
+      const int64_t row = at.position * a.table_stride + 8 * lane;
+      small8(a.table, a.table_dtype, row, c);
+      small8(a.table, a.table_dtype, row + (a.R >> 1), s);
     }
-    Raw8<TI> xk[2], xv[2], xq[U][2];
-    if (a.k.heads > 0) fetch(a.k.in, tr * a.k.in_token + k_in, xk);
-    if (a.v.heads > 0) fetch(a.v.in, tr * a.v.in_token + v_in, xv);
-    const int64_t q_at = tr * a.q.in_token;
-    if (a.q.heads > 0) {
+  };
+  if constexpr (STREAM) {
+    // Row r of a token: 0 the key, 1 the value, then query heads. A lane requests the 16-byte
+    // pieces of its own chunks into its own places of shared memory and reads no other's, so
+    // nothing but its own copies' groups (one a row, in order) has to be waited for.
+    extern __shared__ __align__(16) uint8_t stream_sm[];
+    constexpr int kHalfPieces = static_cast<int>(sizeof(TI)) / 2, kPer16 = 16 / static_cast<int>(sizeof(TI));
+    uint8_t* mine = stream_sm + threadIdx.x * 16;
+    auto request = [&](int stage, int r, int64_t at_t) {
+      const bool want = at_t < a.tokens && (r == 0 ? has_k : r == 1 ? has_v : q0 + r - 2 < q1);
+      if (want) {
+        const HeadRows& rows = r == 0 ? a.k : r == 1 ? a.v : a.q;
+        const TI* p = static_cast<const TI*>(rows.in) + at_t * rows.in_token +
+                      (r == 0 ? k_in : r == 1 ? v_in : (q0 + r - 2) * a.q.in_head);
+        uint8_t* dst = mine + (stage * kWalkerRows + r) * 2 * kHalfPieces * 4096;
 #pragma unroll
-      for (int j = 0; j < U; ++j) fetch(a.q.in, q_at + min64(q0 + j, q_last) * a.q.in_head, xq[j]);
-    }
-    if (pl.rotates && turns && (has_k || q0 < q1)) {
-      const int64_t row = pl.position * a.table_stride + 8 * lane;
-      small8(a.table, a.table_dtype, row, co);
-      small8(a.table, a.table_dtype, row + (a.R >> 1), si);
-    }
-    listed = Listed(a, min64(t + a.step, a.tokens - 1));
-    TC* cache_row = static_cast<TC*>(a.cache) + pl.cache_row;
-    if (a.k.heads > 0) {
+        for (int c = 0; c < kHalfPieces; ++c) {
+          if (has0) cp_async16(dst + c * 4096, p + e0 + c * kPer16);
+          if (has1) cp_async16(dst + (kHalfPieces + c) * 4096, p + e1 + c * kPer16);
+        }
+      }
+      asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+    auto take = [&](int stage, int r, Raw8<TI> (&x)[2]) {
+      asm volatile("cp.async.wait_group %0;\n" ::"n"(kAhead<TI> * kWalkerRows - 1) : "memory");
+      const uint8_t* src = mine + (stage * kWalkerRows + r) * 2 * kHalfPieces * 4096;
+      if (!FULL) x[0] = x[1] = Raw8<TI>{};
+#pragma unroll
+      for (int c = 0; c < kHalfPieces; ++c) {
+        if (has0) x[0].w[c] = *reinterpret_cast<const uint4*>(src + c * 4096);
+        if (has1) x[1].w[c] = *reinterpret_cast<const uint4*>(src + (kHalfPieces + c) * 4096);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead<TI>; ++i)
+#pragma unroll
+      for (int r = 0; r < kWalkerRows; ++r) request(i, r, t + i * a.step);
+    Listed next(a, min64(t + a.step, a.tokens - 1));
+    table(listed, co, si);
+    int stage = 0;
+#pragma unroll 1
+    for (; __any_sync(0xffffffffu, t < a.tokens); t += a.step) {
+      Place pl{-1, 0, false};
+      if (t < a.tokens) {
+        uint32_t skipped;
+        pl = place_of(a, listed, skipped);
+        if (skipped && g == 0 && lane == 0 && a.err) atomicAdd(a.err, skipped);
+      }
+      float co_next[8], si_next[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) co_next[i] = 1.f, si_next[i] = 0.f;
+      table(next, co_next, si_next);
+      listed = next;
+      next = Listed(a, min64(t + 2 * static_cast<int64_t>(a.step), a.tokens - 1));
+      const int64_t later = t + kAhead<TI> * static_cast<int64_t>(a.step);
+      TC* cache_row = static_cast<TC*>(a.cache) + pl.cache_row;
+      Raw8<TI> x[2];
       float f[16];
-      turn(w_sm[1], a.k.weight != nullptr, xk, f);
+      take(stage, 0, x);
+      turn(w_sm[1], a.k.weight != nullptr, true, true, x, f);
       if (has_k && pl.rotates) {
         if (a.k.out) put(static_cast<TI*>(a.k.out) + t * a.k.out_token + kh * a.k.out_head, f);
         else if (pl.cache_row >= 0) put(cache_row + static_cast<int64_t>(kh) * a.D, f);
       }
-    }
-    if (has_v && pl.rotates && pl.cache_row >= 0) {
-      float f[16];
-      unpack8(xv[0], f);
-      unpack8(xv[1], f + 8);
-      put(cache_row + a.kv_stride + static_cast<int64_t>(vh) * a.D, f);
-    }
-    TI* out = static_cast<TI*>(a.q.out) + t * a.q.out_token + q0 * a.q.out_head;
+      request(stage, 0, later);
+      if (a.v.heads > 0) {
+        take(stage, 1, x);
+        unpack8(x[0], f);
+        unpack8(x[1], f + 8);
+        if (has_v && pl.rotates && pl.cache_row >= 0) put(cache_row + a.kv_stride + static_cast<int64_t>(vh) * a.D, f);
+      }
+      request(stage, 1, later);
+      TI* out = static_cast<TI*>(a.q.out) + t * a.q.out_token + q0 * a.q.out_head;
 #pragma unroll 1
-    for (int i0 = 0; i0 < q_per; i0 += U) {
-      if (i0 > 0) {
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-          fetch(a.q.in, q_at + min64(q0 + i0 + j, q_last) * a.q.in_head, xq[j]);
+      for (int j = 0; j < kQueryRows; ++j) {
+        if (j < q_per) {
+          take(stage, 2 + j, x);
+          turn(w_sm[0], a.q.weight != nullptr, true, true, x, f);
+          if (q0 + j < q1 && pl.rotates) put(out + j * a.q.out_head, f);
+        }
+        request(stage, 2 + j, later);
       }
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        float f[16];
-        turn(w_sm[0], a.q.weight != nullptr, xq[j], f);
-        if (q0 + i0 + j < q1 && pl.rotates) put(out + (i0 + j) * a.q.out_head, f);
-      }
+      for (int i = 0; i < 8; ++i) co[i] = co_next[i], si[i] = si_next[i];
+      if (++stage == kAhead<TI>) stage = 0;
     }
+    return;
   }
+  // One head of one token a walker, in one pass.
+  const bool live = t < a.tokens, is_q = q0 < q1;
+  Place pl{-1, 0, false};
+  if (live) {
+    uint32_t skipped;
+    pl = place_of(a, listed, skipped);
+    if (skipped && g == 0 && lane == 0 && a.err) atomicAdd(a.err, skipped);
+  }
+  const HeadRows& rows = is_q ? a.q : has_k ? a.k : a.v;
+  const int64_t head = is_q ? q0 : has_k ? kh : vh;
+  Raw8<TI> x[2] = {Raw8<TI>{}, Raw8<TI>{}};
+  if (live) {
+    const TI* p = static_cast<const TI*>(rows.in) + t * rows.in_token + head * rows.in_head;
+    if (has0) x[0] = load8(p + e0);
+    if (has1) x[1] = load8(p + e1);
+  }
+  if (is_q || has_k) table(listed, co, si);
+  float f[16];
+  turn(w_sm[is_q ? 0 : 1], a.q.weight || a.k.weight, rows.weight != nullptr, is_q || has_k, x, f);
+  if (!pl.rotates) return;
+  if (rows.out) put(static_cast<TI*>(rows.out) + t * rows.out_token + head * rows.out_head, f);
+  else if (pl.cache_row >= 0) put(static_cast<TC*>(a.cache) + pl.cache_row + (has_k ? 0 : a.kv_stride) + head * a.D, f);
 }
 
 // Any head_dim, any even R, element-aligned rows: one warp per row, a lane reads and writes
