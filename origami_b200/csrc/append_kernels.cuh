@@ -19,12 +19,13 @@
 //   16384 tokens of 32 + 8 heads of 128, both with one token per walker);
 // - a walker steps through tokens with a fixed set of heads: addresses, weights (fp32, in shared
 //   memory) and roles are set up once, the next token's position and slot are loaded a token
-//   ahead, its rows (16-bit: of two tokens) copied to shared memory by cp.async, each row's place
-//   refilled as soon as it has been read, so that a walker never waits with nothing requested;
+//   ahead, its rows copied to shared memory by cp.async, each row's place refilled as soon as it
+//   has been read, so that a walker never waits with nothing requested (16384 tokens: 72 us with
+//   loads into registers, 68 so, 72 with two tokens ahead; all cold L2);
 // - fp32 arithmetic in pairs (f32x2).
 // Measured on bf16, halves, with norm: 16384 tokens of 32 query and 8 KV heads of 128, 344 MB,
-// 73 us (4.7 TB/s, 0.73 of the copy rate); append of 32768 such tokens, 822 MB, 158 us (5.2
-// TB/s, 0.81). What remains is latency at 16 warps an SM: a third block (80 registers) spills.
+// 67 us (5.1 TB/s, 0.80 of the copy rate); append of 32768 such tokens, 822 MB, 146 us (5.6
+// TB/s, 0.87).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -68,12 +69,10 @@ namespace app {
 
 constexpr int kF16 = 1, kBF16 = 2, kF32 = 3;
 // Rows of a token that a walker of the streaming form has at most (key, value, query heads), and
-// the tokens that it has requested ahead, in shared memory: 96 KB a CTA.
+// the shared memory for one token's of each: 48 KB a CTA of 16-bit rows, 96 KB of fp32.
 constexpr int kQueryRows = 4, kWalkerRows = 2 + kQueryRows;
 template <typename TI>
-constexpr int kAhead = sizeof(TI) == 4 ? 1 : 2;
-template <typename TI>
-constexpr int kStreamSmem = kAhead<TI> * kWalkerRows * 256 * 16 * static_cast<int>(sizeof(TI));
+constexpr int kStreamSmem = kWalkerRows * 256 * 16 * static_cast<int>(sizeof(TI));
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -337,13 +336,13 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
     extern __shared__ __align__(16) uint8_t stream_sm[];
     constexpr int kHalfPieces = static_cast<int>(sizeof(TI)) / 2, kPer16 = 16 / static_cast<int>(sizeof(TI));
     uint8_t* mine = stream_sm + threadIdx.x * 16;
-    auto request = [&](int stage, int r, int64_t at_t) {
+    auto request = [&](int r, int64_t at_t) {
       const bool want = at_t < a.tokens && (r == 0 ? has_k : r == 1 ? has_v : q0 + r - 2 < q1);
       if (want) {
         const HeadRows& rows = r == 0 ? a.k : r == 1 ? a.v : a.q;
         const TI* p = static_cast<const TI*>(rows.in) + at_t * rows.in_token +
                       (r == 0 ? k_in : r == 1 ? v_in : (q0 + r - 2) * a.q.in_head);
-        uint8_t* dst = mine + (stage * kWalkerRows + r) * 2 * kHalfPieces * 4096;
+        uint8_t* dst = mine + r * 2 * kHalfPieces * 4096;
 #pragma unroll
         for (int c = 0; c < kHalfPieces; ++c) {
           if (has0) cp_async16(dst + c * 4096, p + e0 + c * kPer16);
@@ -352,9 +351,9 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
       }
       asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
-    auto take = [&](int stage, int r, Raw8<TI> (&x)[2]) {
-      asm volatile("cp.async.wait_group %0;\n" ::"n"(kAhead<TI> * kWalkerRows - 1) : "memory");
-      const uint8_t* src = mine + (stage * kWalkerRows + r) * 2 * kHalfPieces * 4096;
+    auto take = [&](int r, Raw8<TI> (&x)[2]) {
+      asm volatile("cp.async.wait_group %0;\n" ::"n"(kWalkerRows - 1) : "memory");
+      const uint8_t* src = mine + r * 2 * kHalfPieces * 4096;
       if (!FULL) x[0] = x[1] = Raw8<TI>{};
 #pragma unroll
       for (int c = 0; c < kHalfPieces; ++c) {
@@ -363,12 +362,9 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
       }
     };
 #pragma unroll
-    for (int i = 0; i < kAhead<TI>; ++i)
-#pragma unroll
-      for (int r = 0; r < kWalkerRows; ++r) request(i, r, t + i * a.step);
+    for (int r = 0; r < kWalkerRows; ++r) request(r, t);
     Listed next(a, min64(t + a.step, a.tokens - 1));
     table(listed, co, si);
-    int stage = 0;
 #pragma unroll 1
     for (; __any_sync(0xffffffffu, t < a.tokens); t += a.step) {
       Place pl{-1, 0, false};
@@ -383,37 +379,35 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
       table(next, co_next, si_next);
       listed = next;
       next = Listed(a, min64(t + 2 * static_cast<int64_t>(a.step), a.tokens - 1));
-      const int64_t later = t + kAhead<TI> * static_cast<int64_t>(a.step);
       TC* cache_row = static_cast<TC*>(a.cache) + pl.cache_row;
       Raw8<TI> x[2];
       float f[16];
-      take(stage, 0, x);
+      take(0, x);
       turn(w_sm[1], a.k.weight != nullptr, true, true, x, f);
       if (has_k && pl.rotates) {
         if (a.k.out) put(static_cast<TI*>(a.k.out) + t * a.k.out_token + kh * a.k.out_head, f);
         else if (pl.cache_row >= 0) put(cache_row + static_cast<int64_t>(kh) * a.D, f);
       }
-      request(stage, 0, later);
+      request(0, t + a.step);
       if (a.v.heads > 0) {
-        take(stage, 1, x);
+        take(1, x);
         unpack8(x[0], f);
         unpack8(x[1], f + 8);
         if (has_v && pl.rotates && pl.cache_row >= 0) put(cache_row + a.kv_stride + static_cast<int64_t>(vh) * a.D, f);
       }
-      request(stage, 1, later);
+      request(1, t + a.step);
       TI* out = static_cast<TI*>(a.q.out) + t * a.q.out_token + q0 * a.q.out_head;
 #pragma unroll 1
       for (int j = 0; j < kQueryRows; ++j) {
         if (j < q_per) {
-          take(stage, 2 + j, x);
+          take(2 + j, x);
           turn(w_sm[0], a.q.weight != nullptr, true, true, x, f);
           if (q0 + j < q1 && pl.rotates) put(out + j * a.q.out_head, f);
         }
-        request(stage, 2 + j, later);
+        request(2 + j, t + a.step);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) co[i] = co_next[i], si[i] = si_next[i];
-      if (++stage == kAhead<TI>) stage = 0;
     }
     return;
   }
