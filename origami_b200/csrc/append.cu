@@ -145,14 +145,14 @@ int32_t launch(origami::AppendArgs& a, cudaStream_t st) {
     const int lanes = (a.D / 8 + 1) / 2;
     while ((1 << a.lanes_log2) < lanes) ++a.lanes_log2;
     // One walker per head while that many threads fit the device at once (the step of a few
-    // tokens is bound by latency); else four query heads a walker beside a key and a value head
-    // (two of them took 180 us for the 32768-token append that four take 160 for, eight the same).
+    // tokens is bound by latency); else kQueryRows query heads a walker beside a key and a value
+    // head (two of them took 162 us for the 32768-token append that four take 139 for, cold L2).
     int sms = 0, dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
     const int64_t resident = static_cast<int64_t>(sms) * 512;
-    a.groups = a.tokens * total << a.lanes_log2 <= resident ? total : std::max(a.k.heads, (a.q.heads + 3) / 4);
+    a.groups = a.tokens * total << a.lanes_log2 <= resident ? total : std::max(a.k.heads, (a.q.heads + origami::app::kQueryRows - 1) / origami::app::kQueryRows);
     const bool full = a.D == 16 << a.lanes_log2;
     const bool stream = a.groups != total;
     auto* fn = stream ? (full ? &origami::append_rows<TI, TC, true, true> : &origami::append_rows<TI, TC, false, true>)

@@ -20,7 +20,7 @@
 // - a walker steps through tokens with a fixed set of heads: addresses, weights (fp32, in shared
 //   memory) and roles are set up once, the next token's position and slot are loaded a token
 //   ahead, its rows copied to shared memory by cp.async, each row's place refilled as soon as it
-//   has been read, so that a walker never waits with nothing requested (16384 tokens: 72 us with
+//   has been read, so that a walker never waits with nothing requested (16384 tokens: 78 us with
 //   loads into registers, 68 so, 72 with two tokens ahead; all cold L2);
 // - fp32 arithmetic in pairs (f32x2).
 // Measured on bf16, halves, with norm: 16384 tokens of 32 query and 8 KV heads of 128, 344 MB,
