@@ -24,8 +24,8 @@
 //   loads into registers, 68 so, 72 with two tokens ahead; all cold L2);
 // - fp32 arithmetic in pairs (f32x2).
 // Measured on bf16, halves, with norm: 16384 tokens of 32 query and 8 KV heads of 128, 344 MB,
-// 67 us (5.1 TB/s, 0.80 of the copy rate); append of 32768 such tokens, 822 MB, 146 us (5.6
-// TB/s, 0.87).
+// 64 to 67 us (5.1 to 5.4 TB/s, 0.80 to 0.84 of the copy rate); append of 32768 such tokens, 822
+// MB, 141 to 147 us (5.6 to 5.8 TB/s, 0.87 to 0.90).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -38,7 +38,7 @@
 // Measured (cold L2, both launches): 64 requests over 32768 shared keys and up to 1024 own, 32 / 8
 // heads of 128, 282 MB, 35 GFLOP: 86 us; 8 requests over 131072, 64 / 8 heads, 616 MB: 127 us (4.9
 // TB/s, 0.75 of the copy rate, by the ring's stages in flight); 256 requests over 32768, 138 GFLOP:
-// 209 us. There a pair of streams' steps of 64 keys takes about 1850 clocks, its products alone
+// 205 us. There a pair of streams' steps of 64 keys takes about 1850 clocks, its products alone
 // 1304 (Q K^T at N = 64 takes 49 clocks per 16 dims, bound by its shared-memory operands, where
 // N = 128 takes 65), softmax 1027 of ex2: the products' chain bounds. Steps of 128 keys have
 // cheaper products but leave TMEM for one S a stream, with P over it: 223 us.
