@@ -178,7 +178,7 @@ def append_kv(kv_layer: torch.Tensor, key: torch.Tensor, value: torch.Tensor, sl
     kv_layer is a paged cache layer in either layout of `layer.cache_layout`, bf16 or fp16;
     key, value and query share a type (bf16, fp16 or fp32). A token with slot -1 gets no
     cache row; its query is still written. Slots must differ from one another. query_out may
-    be query itself."""
+    be query itself; no other input may share memory with an output or the cache."""
     index = _device_index(kv_layer, "the paged KV cache")
     desc = paged_desc(kv_layer)
     cache_dtype = _DTYPE.get(kv_layer.dtype)

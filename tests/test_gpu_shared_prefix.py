@@ -128,6 +128,11 @@ CASES = [  # new, suffix, prefix, Hq, Hk, D, block size
     ([1, 2, 1], [200, 129, 31], 517, 8, 2, 64, 24),
     ([1] * 50, [1 + 13 * i for i in range(50)], 1025, 16, 4, 128, 64),
     ([3, 1], [700, 300], 900, 8, 2, 64, 256),
+    # thousands of rows: several a warp in the join, of few partials each and of many, some without a key
+    ([200, 193, 7], [150, 193, 60], 0, 6, 2, 128, 16),
+    ([300, 300], [300, 350], 100, 24, 2, 64, 16),
+    ([20], [25], 12000, 128, 1, 64, 16),
+    ([64] * 6, [64 + i for i in range(6)], 700, 32, 4, 128, 16),
 ]
 
 
@@ -146,6 +151,8 @@ def test_against_the_formula(cuda, case, dtype):
                     device=cuda)
     again = x.run(softmax_scale=D ** -0.5, workspace=ws)
     assert torch.equal(out, again)
+    odd = torch.empty(out.numel() + 1, dtype=dtype, device=cuda)[1:].view_as(out)  # an output at an odd element
+    assert torch.equal(x.run(out=odd), out)
 
 
 @pytest.mark.parametrize("k_std", [0.01, 8.0, 40.0])
