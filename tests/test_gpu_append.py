@@ -77,6 +77,10 @@ SHAPES = [  # T, Hq, Hk, D, R, interleaved
     (6, 3, 3, 1, 0, False),
     (2, 1, 1, 2, 2, True),
     (5000, 4, 1, 64, 32, True),
+    # a walker steps through several tokens, the last pass being partial
+    (4001, 28, 4, 128, 128, False),
+    (12000, 5, 2, 96, 48, False),
+    (9600, 3, 5, 40, 16, True),    # more key heads than the query heads' walkers
 ]
 
 
@@ -132,6 +136,9 @@ def flat_slots(cache, kv_first):
     (23, 3, 1, 96, 48, False, 1),
     (10, 2, 2, 80, 0, False, 7),
     (12, 3, 3, 7, 6, True, 3),
+    (4001, 28, 4, 128, 128, False, 16),
+    (20011, 0, 2, 64, 32, False, 5),
+    (12000, 5, 1, 72, 0, False, 8),
 ])
 def test_append(cuda, T, Hq, Hk, D, R, interleaved, bs, dtype, cache_dtype, kv_first):
     q, k, v = make(T, max(Hq, 1), Hk, D, dtype, cuda, T % 2 == 1, T + D)
@@ -180,6 +187,36 @@ def test_bad_slots_and_positions_are_skipped_and_counted(cuda, D):
     assert torch.equal(flat[1][3], v[0])
     flat[:, 3] = 0
     assert not flat.any()
+
+
+def test_skipped_and_padded_tokens_between_others_of_a_long_step(cuda):
+    T, Hq, Hk, D, bs = 12007, 5, 2, 64, 16
+    q, k, v = make(T, Hq, Hk, D, BF16, cuda, True, 8)
+    blocks = T // bs + 1
+    cache = torch.full((blocks, 2, bs, Hk, D), 3.0, dtype=BF16, device=cuda)
+    i = torch.arange(T, device=cuda)
+    slots = torch.randperm(blocks * bs, generator=torch.Generator().manual_seed(1))[:T].to(cuda)
+    padded, outside, bad = i % 7 == 2, i % 11 == 3, i % 13 == 4
+    slots[outside] = blocks * bs + 5
+    slots[padded] = -1
+    outside &= ~padded
+    pos = i % 100
+    pos[bad] = 100
+    table = table_for(D, 100, F32, cuda)
+    out = torch.full_like(q, 9.0)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    append.append_kv(cache, k, v, slots, query=q, positions=pos, cos_sin=table, query_out=out, error_count=err)
+    written = ~(padded | outside | bad)
+    assert int(err) == int(bad.sum()) * Hq + int((outside | (bad & ~padded)).sum()) * 2 * Hk
+    want, allow = expected(q, None, pos.clamp(max=99), table, False)
+    assert_rows(out[~bad], want[~bad], allow[~bad], BF16)
+    assert bool((out[bad] == 9.0).all())
+    flat = flat_slots(cache, False)
+    want, allow = expected(k, None, pos.clamp(max=99), table, False)
+    assert_rows(flat[0][slots[written]], want[written], allow[written], BF16)
+    assert torch.equal(flat[1][slots[written]], v[written])
+    flat[:, slots[written]] = 3.0
+    assert bool((flat == 3.0).all())
 
 
 def test_non_finite_rows_stay_in_their_rows(cuda):
