@@ -8,7 +8,8 @@
 // the joins are fp32; the probabilities are rounded to the type of V for the product (the
 // tensor cores take both operands in one type; half a step, 2^-8 bf16 / 2^-11 fp16, of each
 // probability at most, which averages over the keys: measured against 64 bits, 2.2e-3 of the
-// output's norm in bf16 where the output's own rounding is 1.7e-3).
+// output's norm in bf16 where the output's own rounding is 1.7e-3). In fp16 that holds down to
+// 2^-23 of the piece's largest probability; smaller ones are off by up to 2^-34 of it each.
 //
 // Work. The prefix is one attention problem per KV head whose rows are the new tokens of ALL
 // requests x the query heads of the group: its K and V are read once for every 128 or 256
@@ -28,8 +29,8 @@
 //   O_s [128 rows x D]      += P V   (P in TMEM, V the N-major B operand).
 // The next scores are begun as soon as a step has read its own, so a stream's chain is its
 // softmax alone. One thread owns one row: the softmax needs no exchange. O is rescaled only when the
-// maximum grew by more than 2^8 (P stays below 2^8, exact in the same relative precision; each
-// time it grows, the batch of 256 takes 256 us instead of 209).
+// maximum grew by more than a few powers of two (`Reference`; each time it grows, the batch of 256
+// takes 256 us instead of 209).
 // With more than 128 rows an item has two row tiles, one per stream, that share each K and V
 // tile ("pair"); with fewer, the streams take one half of each key tile for one row tile and
 // join at the end of the segment ("split"); segments of one tile go to the streams in turn
@@ -67,6 +68,18 @@ constexpr int kHalf = 64;       // keys per softmax step
 // pair's tile at 8: 90 / 100 / 232, at 16: 96 / 84 / 231; items for nothing: 96 / 86 / 272, a
 // pair's at 8: 86 / 90 / 211, a single's at 16: 88 / 92 / 229.
 constexpr int kCostTile = 8, kCostPair = 12, kCostItem = 8, kCostPairItem = 22;
+// The probabilities as the products take them: p = 2^(s log2(e) - m), where the reference m lies
+// `up` below the largest score (in powers of two) when it is set and follows it once the largest
+// has grown by more than `grow`, so that p stays below 2^(up + grow). fp16 ends at 2^16 and loses
+// bits below 2^-14: the largest begins at 2^9 there, which puts that end 23 bits below it (with
+// `up` 0, keys 17 nats behind one that stands out came to nothing in the products). Of the range,
+// growth by 2^6 costs nothing (batch of 64 / of 256 in fp16: 88 / 205 us, with 8 88 / 209), by 2^4
+// 94 / 217, by 2^2 100 / 227.
+template <bool BF16>
+struct Reference {
+  static constexpr float up = BF16 ? 0.f : 9.f, grow = BF16 ? 8.f : 6.f;
+  static_assert(BF16 || up + grow <= 15.f, "fp16 holds p");
+};
 
 // Shared memory: Q tiles, then the ring of K / V tiles (each [128][D] 16-bit), then scalars.
 template <int D>
@@ -489,6 +502,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
   static_assert(sizeof(Bars) + 8 + sizeof(Deal) + kSegments * sizeof(Segment) <= 1024, "scalars fit");
   static_assert(S::bytes <= 227 * 1024, "shared memory of one SM");
   constexpr bool kBf16 = attn::is_bf16<QT>();
+  using Ref = Reference<kBf16>;
   constexpr uint32_t kIdescS = attn::instr_desc(kBf16, kHalf);
   constexpr uint32_t kIdescO = attn::instr_desc(kBf16, D) | (1u << 16);  // B (V) is N-major
   constexpr uint32_t kP = 64, kO = 128;  // of stream s: S at column 256 s, P at + 64 and + 96, O at + 128
@@ -992,10 +1006,12 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
           }
           mx[0] = max3(mx[0], __uint_as_float(x[kHalf - 4]), __uint_as_float(x[kHalf - 3]));
           mx[1] = max3(mx[1], __uint_as_float(x[kHalf - 2]), __uint_as_float(x[kHalf - 1]));
-          const float mt = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
-          const bool grow = row < rows && (mt > m + 8.f || (m == -INFINITY && mt > -INFINITY));
+          // directed roundings: no score lies above mt, no reference more than up + grow below one
+          const float mt = __fmul_ru(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), a.scale_log2);
+          const float ref = __fsub_ru(mt, Ref::up);
+          const bool grow = row < rows && (mt > __fadd_rd(m, Ref::up + Ref::grow) || (m == -INFINITY && mt > -INFINITY));
           if (__any_sync(0xffffffffu, grow)) {
-            const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - mt)) : 1.f;
+            const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - ref)) : 1.f;
             if (i > 0) {  // O is at rest once the product of the step before has ended
               const uint32_t last = count - 1;
               ok = wait_warp(&bars->pv[2 * s + (last & 1u)], (last >> 1) & 1u, abort);
@@ -1011,7 +1027,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
               }
             }
             l *= alpha;
-            m = grow ? mt : m;
+            m = grow ? ref : m;
           }
           // P's buffer is free: S of this step was begun after the product of two steps before,
           // and its barrier tells that all products begun before it have ended

@@ -381,3 +381,43 @@ def test_step_over_a_restored_prefix(cuda):
         written = cache[:, ids[nb:].to(cuda), step]
         x.skv = [torch.cat([kv_b, written[:, b:b + 1]], 1) for b, kv_b in enumerate(x.skv)]
         x.check(x.run())
+
+
+@pytest.mark.parametrize("nats", [10.0, 14.0, 16.0, 17.0, 17.5, 19.0])
+@pytest.mark.parametrize("spread", [0.0, 0.5])
+def test_fp16_keys_far_below_one_that_stands_out(cuda, nats, spread):
+    """An attention sink: the first key's score lies `nats` above all others and its value is zero, so that
+    the row is made of the others' small probabilities alone; many heads, so that a CTA has it beside most
+    of them. Beside the tolerance above: the kernel's fp16 probabilities have their largest at 2^9 or more,
+    so one below 2^-14 is off by at most half of the smallest step, 2^-25: 2^-34 of |v| a key."""
+    H, g, N, D = 80, 2, 4100, 64
+    x = Batch(cuda, [1, 1], [1, 40], N, H * g, H, D, 16, F16, seed=21)
+    x.q.zero_()
+    x.q[..., 0] = 1
+    for kv in [x.pkv, *x.skv]:
+        kv[0] = 0
+        kv[0, ..., 0] = torch.randn(kv.shape[1:3], device=cuda) * spread * D ** 0.5
+        kv[1] += 1  # values that do not cancel
+    x.pkv[0, 0, :, 0] = nats * D ** 0.5
+    x.pkv[1, 0] = 0
+    x.write(x.pkv, x.prefix_blocks)
+    for b, kv in enumerate(x.skv):
+        x.write(kv, x.suffix_blocks[b])
+    out = x.run().double()
+    u = torch.finfo(F16).eps / 2
+    for b, kv in enumerate(x.skv):
+        k, v = (t.double().transpose(0, 1) for t in torch.cat([x.pkv, kv], 1))  # [H, N, D]
+        p = torch.softmax(k[..., 0] * D ** -0.5, -1)
+        want, A = ((p[:, None] @ t)[:, 0].repeat_interleave(g, 0) for t in (v, v.abs()))
+        err = nats * (D / 8) * 2.0 ** -22 + 2.0 ** -22 * (1 + nats)
+        tol = (u + 2 * err + (k.shape[1] / 8 + 64) * 2.0 ** -23) * A + u * want.abs() + 2.0 ** -25
+        tol += 2.0 ** -34 * v.abs().sum(1).repeat_interleave(g, 0)
+        off = (out[b] - want).abs()
+        assert bool((off <= tol).all()), (b, float((off / want.abs()).max()), float((off - tol).max()))
+
+
+@pytest.mark.parametrize("k_std", [0.01, 8.0, 40.0])
+def test_flat_and_peaked_scores_fp16(cuda, k_std):
+    x = Batch(cuda, [1] * 20, [30 + 17 * i for i in range(20)], 3000, 16, 2, 128, 16, F16, seed=3, k_std=k_std)
+    lse = torch.empty(20, 16, dtype=torch.float32, device=cuda)
+    x.check(x.run(lse=lse), lse)
