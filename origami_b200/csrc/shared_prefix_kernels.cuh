@@ -162,8 +162,17 @@ __device__ __forceinline__ int share_begin(const SharedArgs& a, int all, int c) 
   return c >= a.ctas ? all : static_cast<int>(__umulhi(static_cast<uint32_t>(all), static_cast<uint32_t>(c) * a.inv_ctas));
 }
 __device__ __forceinline__ int clamp32(int v, int lo, int hi) { return min(max(v, lo), hi); }
+// An entry of the device lists, or of the costs that the first kernel leaves for the join. The
+// kernel before on the stream may still be writing them when this one starts, so the load has to
+// stay behind the dependent wait: one through the read-only path, which asks for data that nobody
+// writes while the kernel lives, may be moved ahead of it.
+__device__ __forceinline__ int list_at(const int32_t* p) {
+  int v;
+  asm volatile("ld.global.s32 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ int used_tokens(const SharedArgs& a) {
-  return clamp32(__ldg(a.query_start + a.requests), 0, a.tokens);
+  return clamp32(list_at(a.query_start + a.requests), 0, a.tokens);
 }
 __device__ __forceinline__ int prefix_item_tokens(const SharedArgs& a, int used) {
   return used > a.tile_tokens ? 2 * a.tile_tokens : a.tile_tokens;
@@ -189,12 +198,20 @@ __device__ __forceinline__ int prefix_cost(const SharedArgs& a, int used) {
 
 struct Request {
   int32_t begin, n, len;
-  __device__ __forceinline__ Request(const SharedArgs& a, int b) {
-    begin = clamp32(__ldg(a.query_start + b), 0, a.tokens);
-    n = clamp32(__ldg(a.query_start + b + 1), begin, a.tokens) - begin;
-    len = clamp32(__ldg(a.suffix_lens + b), 0, a.suffix_cap);
-  }
 };
+__device__ __forceinline__ Request request_at(const SharedArgs& a, int b, bool& falls) {
+  const int begin = list_at(a.query_start + b), end = list_at(a.query_start + b + 1), len = list_at(a.suffix_lens + b);
+  Request r;
+  r.begin = clamp32(begin, 0, a.tokens);
+  r.n = clamp32(end, r.begin, a.tokens) - r.begin;
+  r.len = clamp32(len, 0, a.suffix_cap);
+  falls = end < begin;
+  return r;
+}
+__device__ __forceinline__ Request request_at(const SharedArgs& a, int b) {
+  bool falls;
+  return request_at(a, b, falls);
+}
 __device__ __forceinline__ Item suffix_item(const SharedArgs& a, const Request& r, int h, int b, int tile, int start) {
   Item it;
   it.start = start;
@@ -235,7 +252,7 @@ struct Walk {
   int ph, ptok;    // next prefix item: head and first token
   bool in_prefix;
   Request r;
-  __device__ __forceinline__ Walk(const SharedArgs& args, const Deal& deal) : a(args), d(deal), r(args, deal.b) {
+  __device__ __forceinline__ Walk(const SharedArgs& args, const Deal& deal) : a(args), d(deal), r(request_at(args, deal.b)) {
     in_prefix = d.w0 < d.wp * a.kv_heads;
     h = d.h;
     b = d.b;
@@ -264,7 +281,7 @@ struct Walk {
         if (ph >= a.kv_heads) {
           in_prefix = false;
           h = b = tile = 0;
-          r = Request(a, 0);
+          r = request_at(a, 0);
         }
       } else {
         // past the last head there is nothing (requests without any tile cost nothing)
@@ -275,7 +292,7 @@ struct Walk {
             b = 0;
             ++h;
           }
-          r = Request(a, b);
+          r = request_at(a, b);
           continue;
         }
         it = suffix_item(a, r, h, b, tile, next);
@@ -557,8 +574,9 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
     bool falls = false;  // query_start does: requests would share tokens, and their costs have no bound
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
-      sum += request_cost(a, Request(a, b));
-      falls |= __ldg(a.query_start + b + 1) < __ldg(a.query_start + b);
+      bool here;
+      sum += request_cost(a, request_at(a, b, here));
+      falls |= here;
     }
     int incl = sum;
 #pragma unroll
@@ -599,7 +617,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       int at = excl;
 #pragma unroll 1
       for (int b = b0; b < b1; ++b) {
-        const Request r(a, b);
+        const Request r = request_at(a, b);
         const int c = request_cost(a, r);
         if (cta == 0) a.req_cost[b] = at;
         if (c > 0 && rem >= at && rem < at + c) {
@@ -680,7 +698,7 @@ __global__ void __launch_bounds__(spa::kThreadsS, 1) shared_prefix_attention(con
       auto row_of = [&](int key) -> int {
         if (key >= seg.kend) return -1;
         const uint32_t page = static_cast<uint32_t>(key) / static_cast<uint32_t>(a.block_size);
-        const int pb = __ldg(table + page);
+        const int pb = list_at(table + page);
         return pb < 0 || pb >= a.num_blocks ? -1 : pb * a.block_rows + (key - static_cast<int>(page) * a.block_size);
       };
       int key = seg.t0 * kTile + 32 * lw + lane;
@@ -1167,38 +1185,37 @@ __global__ void __launch_bounds__(256, 2) merge_partials(const __grid_constant__
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int t = static_cast<int>(unit / per_token), in_token = static_cast<int>(unit - static_cast<int64_t>(t) * per_token);
   const int h = in_token / per_head, g0 = (in_token - h * per_head) * a.merge_rows;
-  // The lists are this launch's inputs as much as the first kernel's, which had waited for what
-  // wrote them before it let this one start: read ahead of the wait for its partials.
-  const int used = used_tokens(a);
-  // the request: token t itself in a step of one token each, else by bisection
-  int b = clamp32(t, 0, a.requests - 1);
-  const int first = __ldg(a.query_start), lo0 = __ldg(a.query_start + b), hi0 = __ldg(a.query_start + b + 1);
-  if (t >= used || t < first) {  // (a launch that ends before its wait could let the stream run ahead of the first kernel)
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    return;
-  }
-  if (t < lo0 || t >= hi0) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  // The request: token t itself in a step of one token each (everything that such a step has to know
+  // is asked for at once), else searched for, 32 places of the range at a time.
+  int b = clamp32(t, 0, a.requests - 1), step = (a.requests + 31) >> 5;
+  const int used = used_tokens(a), first = list_at(a.query_start), ws = list_at(a.head);
+  int before = list_at(a.req_cost + b), probe = list_at(a.query_start + min(lane * step, a.requests));
+  Request r = request_at(a, b);
+  if (ws < 0 || t >= used || t < first) return;
+  if (t < r.begin || t >= r.begin + r.n) {
     int lo = 0, hi = a.requests;  // query_start[lo] <= t < query_start[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(a.query_start + mid) <= t) lo = mid;
-      else hi = mid;
+    for (;;) {
+      const bool below = lane == 0 || (lo + lane * step < hi && probe <= t);
+      lo += (31 - __clz(__ballot_sync(0xffffffffu, below))) * step;
+      hi = min(lo + step, hi);
+      if (hi - lo <= 1) break;
+      step = (hi - lo + 31) >> 5;
+      probe = list_at(a.query_start + min(lo + lane * step, hi));
     }
     b = lo;
+    r = request_at(a, b);
+    before = list_at(a.req_cost + b);
   }
-  const Request r(a, b);
   const int tile = (t - r.begin) / a.tile_tokens;
-  int before = 0;  // cost of the request's row tiles before this one
-  if (tile > 0) {
-    for (int j = lane; j < tile; j += 32) before += suffix_item(a, r, h, b, j, 0).cost();
+  if (tile > 0) {  // the cost of the request's row tiles before this one
+    int c = 0;
+    for (int j = lane; j < tile; j += 32) c += suffix_item(a, r, h, b, j, 0).cost();
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    before += c;
   }
   const int wp = prefix_cost(a, used), per = prefix_item_tokens(a, used), pi = t / per;
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const int ws = __ldcg(a.head);
-  if (ws < 0) return;
-  before += __ldcg(a.req_cost + b);
   const int all = (wp + ws) * a.kv_heads;
   const float shares = static_cast<float>(a.ctas) / static_cast<float>(all);
   const Parts pre(a, prefix_item(a, used, h, pi * per, h * wp + pi * prefix_item(a, used, 0, 0, 0).cost()), t, all, shares);

@@ -421,3 +421,11 @@ def test_flat_and_peaked_scores_fp16(cuda, k_std):
     x = Batch(cuda, [1] * 20, [30 + 17 * i for i in range(20)], 3000, 16, 2, 128, 16, F16, seed=3, k_std=k_std)
     lse = torch.empty(20, 16, dtype=torch.float32, device=cuda)
     x.check(x.run(lse=lse), lse)
+
+
+def test_more_requests_than_places_of_two_searches(cuda):
+    """A token's request is found among over 1024, many of them without new tokens."""
+    new = [(7 * i % 5) % 3 for i in range(1500)]
+    x = Batch(cuda, new, [n + i % 9 for i, n in enumerate(new)], 40, 2, 1, 64, 16, BF16, seed=18)
+    lse = torch.empty(sum(new), 2, dtype=torch.float32, device=cuda)
+    x.check(x.run(lse=lse), lse)
