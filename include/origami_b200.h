@@ -402,13 +402,13 @@ int32_t origami_append_kv(const origami_head_rows* key, const origami_head_rows*
  * d_prefix_blocks, and to the first suffix_lens[b] - n + j + 1 keys (none if that is not
  * positive) of the request's own suffix, in the blocks d_suffix_blocks[b * suffix_stride ..]:
  * a request's suffix includes its new tokens, already in the cache. The scores are scaled by
- * softmax_scale (finite, positive); query head qh reads KV head qh / (query_heads /
- * kv_heads). A row without keys gives zeros and lse -inf; an out-of-range block id reads as
- * zero K and V (the key still takes part in the softmax with score 0); query tokens outside
- * [query_start[0], query_start[requests]) are left as they are in output and lse. The lists
- * are device int32; lengths are clamped to the tables (suffix_lens to suffix_width *
- * block_size, query_start to [0, tokens]). If query_start decreases anywhere, nothing is
- * written and bit 30 of d_error_flags is set.
+ * softmax_scale (positive; its product with log2(e) a normal number in 32 bits); query head qh
+ * reads KV head qh / (query_heads / kv_heads). A row without keys gives zeros and lse -inf; an
+ * out-of-range block id reads as zero K and V (the key still takes part in the softmax with
+ * score 0); query tokens outside [query_start[0], query_start[requests]) are left as they are
+ * in output and lse. The lists are device int32; lengths are clamped to the tables
+ * (suffix_lens to suffix_width * block_size, query_start to [0, tokens]). If query_start
+ * decreases anywhere, nothing is written and bit 30 of d_error_flags is set.
  * query, output and cache share a type (F16 or BF16); head_dim is 64 or 128, the query heads
  * of a KV head at most 128. lse (nullable, [tokens, query_heads] contiguous) gets the natural
  * logarithm of each row's sum of exponentials. Keys and values past the last one that any of

@@ -144,6 +144,9 @@ int32_t origami_shared_prefix_attention(
     return fail(ORIGAMI_ERR_INVALID, "prefix_blocks is too short for prefix_tokens");
   if (!(softmax_scale > 0.0) || std::isinf(softmax_scale))
     return fail(ORIGAMI_ERR_INVALID, "softmax_scale must be finite and positive");
+  const float scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
+  if (!std::isnormal(scale_log2))  // zero or infinite, it would make NaN of scores that are not seen or zero
+    return fail(ORIGAMI_ERR_INVALID, "softmax_scale is too small or too large for 32 bits");
   if (cache->block_size > 0x3FFFFFFF || cache->num_blocks * cache->block_size > 0x3FFFFFFF)
     return fail(ORIGAMI_ERR_UNSUPPORTED, "the cache has too many token rows");
   if (tokens == 0) return ORIGAMI_OK;
@@ -234,7 +237,7 @@ int32_t origami_shared_prefix_attention(
   // spends its issue slots on (half as many: the batch of 256 211 us instead of 205; one each:
   // chunks of 2100 tokens of 16 heads 115 instead of 86).
   a.merge_rows = static_cast<int32_t>(std::clamp<int64_t>(tokens * a.q_heads / (8 * sms), 1, a.group));
-  a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
+  a.scale_log2 = scale_log2;
   uint8_t* ws = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<int64_t>(d_workspace), 32));
   a.head = reinterpret_cast<int32_t*>(ws);
   a.req_cost = reinterpret_cast<int32_t*>(ws + w.req_cost);

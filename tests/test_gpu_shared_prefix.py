@@ -429,3 +429,9 @@ def test_more_requests_than_places_of_two_searches(cuda):
     x = Batch(cuda, new, [n + i % 9 for i, n in enumerate(new)], 40, 2, 1, 64, 16, BF16, seed=18)
     lse = torch.empty(sum(new), 2, dtype=torch.float32, device=cuda)
     x.check(x.run(lse=lse), lse)
+
+
+def test_smallest_scale(cuda):
+    """Every key of like weight: the mean of the values."""
+    x = Batch(cuda, [2] * 3, [40] * 3, 200, 4, 2, 64, 16, BF16, seed=19)
+    x.check(x.run(softmax_scale=1e-38), scale=1e-38)

@@ -78,6 +78,14 @@ def test_refusals(change, message):
     assert message in msg
 
 
+@pytest.mark.parametrize("scale", [1e-300, 1e-46, 1e-39, 2.4e38, 1e300])
+def test_scales_that_32_bits_do_not_hold(scale):
+    """The kernel takes scale * log2(e) in 32 bits: neither zero, nor without all its digits, nor infinite."""
+    rc, msg = call(scale=scale)
+    assert rc == -1
+    assert "32 bits" in msg
+
+
 def test_no_tokens_is_no_launch():
     assert call(tokens=0)[0] == 0
 
