@@ -88,16 +88,18 @@ int32_t check_rotation(const origami_rotation* r, int64_t head_dim) {
   return ORIGAMI_OK;
 }
 
-void set_rows(origami::HeadRows& r, const origami_head_rows* in, const origami_head_rows* out, const void* weight,
-              int32_t weight_dtype) {
+// (the token stride of one token and the head stride of one head are never used: 0, so that they
+// do not count in the choice of kernel)
+void set_rows(origami::HeadRows& r, const origami_head_rows* in, const origami_head_rows* out, int64_t tokens,
+              const void* weight, int32_t weight_dtype) {
   r.in = in->d_data;
-  r.in_token = in->token_stride;
-  r.in_head = in->head_stride;
+  r.in_token = tokens > 1 ? in->token_stride : 0;
+  r.in_head = in->num_heads > 1 ? in->head_stride : 0;
   r.heads = static_cast<int32_t>(in->num_heads);
   if (out) {
     r.out = out->d_data;
-    r.out_token = out->token_stride;
-    r.out_head = out->head_stride;
+    r.out_token = tokens > 1 ? out->token_stride : 0;
+    r.out_head = out->num_heads > 1 ? out->head_stride : 0;
   }
   r.weight = weight;
   r.weight_dtype = weight_dtype;
@@ -125,7 +127,7 @@ void set_shared(origami::AppendArgs& a, int64_t tokens, int64_t head_dim, const 
 bool rows16(const origami::HeadRows& r, int64_t es) {
   if (r.heads == 0) return true;
   return aligned(r.in, 16) && (r.in_token * es) % 16 == 0 && (r.in_head * es) % 16 == 0 && aligned(r.out, 16) &&
-         (r.out_token * es) % 16 == 0 && (r.out_head * es) % 16 == 0 && aligned(r.weight, 16);
+         (r.out_token * es) % 16 == 0 && (r.out_head * es) % 16 == 0;
 }
 
 // The fast kernel's conditions (append_kernels.cuh); everything else takes the kernel for
@@ -205,8 +207,8 @@ int32_t origami_norm_rope(const origami_head_rows* query, const origami_head_row
   if ((rc = check_rotation(rotation, head_dim)) || (rc = check_norm(norm))) return rc;
   origami::AppendArgs a{};
   set_shared(a, tokens, head_dim, rotation, norm, d_error_count);
-  set_rows(a.q, query, query_out, norm ? norm->d_query_weight : nullptr, norm ? norm->query_weight_dtype : 0);
-  set_rows(a.k, key, key_out, norm ? norm->d_key_weight : nullptr, norm ? norm->key_weight_dtype : 0);
+  set_rows(a.q, query, query_out, tokens, norm ? norm->d_query_weight : nullptr, norm ? norm->query_weight_dtype : 0);
+  set_rows(a.k, key, key_out, tokens, norm ? norm->d_key_weight : nullptr, norm ? norm->key_weight_dtype : 0);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (query->dtype) {
     case ORIGAMI_DTYPE_F16: return launch<__half, __half>(a, st);
@@ -245,9 +247,9 @@ int32_t origami_append_kv(const origami_head_rows* key, const origami_head_rows*
   if ((rc = check_norm(norm))) return rc;
   origami::AppendArgs a{};
   set_shared(a, tokens, head_dim, rotation, norm, d_error_count);
-  if (query) set_rows(a.q, query, query_out, norm ? norm->d_query_weight : nullptr, norm ? norm->query_weight_dtype : 0);
-  set_rows(a.k, key, nullptr, norm ? norm->d_key_weight : nullptr, norm ? norm->key_weight_dtype : 0);
-  set_rows(a.v, value, nullptr, nullptr, 0);
+  if (query) set_rows(a.q, query, query_out, tokens, norm ? norm->d_query_weight : nullptr, norm ? norm->query_weight_dtype : 0);
+  set_rows(a.k, key, nullptr, tokens, norm ? norm->d_key_weight : nullptr, norm ? norm->key_weight_dtype : 0);
+  set_rows(a.v, value, nullptr, tokens, nullptr, 0);
   a.slots = d_slots;
   a.slots64 = slot_bytes == 8;
   a.cache = cache->d_data;

@@ -321,3 +321,47 @@ def test_appended_rows_pack_and_restore(cuda):
     assert torch.equal(fresh, cache)
     want, allow = expected(k, None, t.to(cuda), table, False)
     assert_rows(workloads.tokens_from_cache(fresh, ids, T)[0], want, allow, BF16)
+
+
+def at_odd_element(t):
+    """A contiguous copy of t that starts one element behind an aligned address."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    return flat[1:].view_as(t).copy_(t)
+
+
+@pytest.mark.parametrize("T", [1, 3, 6001])
+@pytest.mark.parametrize("weight_dtype", [F32, BF16])
+def test_results_do_not_depend_on_where_weights_lie(cuda, T, weight_dtype):
+    """Weights that are slices of a flat parameter buffer: the same bits as with aligned ones."""
+    Hq, Hk, D, bs = 8, 2, 128, 16
+    q, k, v = make(T, Hq, Hk, D, F32, cuda, True, 12)
+    table, pos = table_for(D, 512, F32, cuda), torch.arange(T, device=cuda) % 512
+    qw, kw = ((torch.rand(D, device=cuda) + 0.5).to(weight_dtype) for _ in range(2))
+    want = append.norm_rope(q, k, pos, table, query_weight=qw, key_weight=kw, eps=EPS)
+    got = append.norm_rope(q, k, pos, table, query_weight=at_odd_element(qw), key_weight=at_odd_element(kw), eps=EPS)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    slots = torch.randperm(T + 7, generator=torch.Generator().manual_seed(3))[:T].to(cuda)
+    caches, outs = [], []
+    for w in (kw, at_odd_element(kw)):
+        caches.append(torch.zeros((2, (T + 7) // bs + 1, bs, Hk, D), dtype=F16, device=cuda))
+        outs.append(append.append_kv(caches[-1], k, v, slots, query=q, query_weight=qw, key_weight=w, eps=EPS,
+                                     positions=pos, cos_sin=table))
+    assert torch.equal(caches[0], caches[1]) and torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("T, H", [(1, 8), (5001, 1), (1, 1)])
+def test_results_do_not_depend_on_strides_that_nothing_uses(cuda, T, H):
+    """The token stride of one token and the head stride of one head are any number."""
+    D = 128
+    q, k, _ = make(T, H, H, D, F32, cuda, False, 14)
+    table, pos = table_for(D, 512, F32, cuda), torch.arange(T, device=cuda) % 512
+    w = torch.rand(D, device=cuda) + 0.5
+    want = append.norm_rope(q, k, pos, table, query_weight=w, key_weight=w, eps=EPS)
+
+    def odd(t):
+        return t.as_strided(t.shape, (t.stride(0) if T > 1 else D * H + 1, t.stride(1) if H > 1 else D + 1, 1))
+
+    out = [torch.empty_like(t) for t in (q, k)]
+    got = append.norm_rope(odd(q), odd(k), pos, table, query_weight=w, key_weight=w, eps=EPS, query_out=odd(out[0]),
+                           key_out=odd(out[1]))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
