@@ -30,15 +30,8 @@ int32_t check_rows(const origami_head_rows* r, const char* name, int64_t head_di
   if (!aligned(r->d_data, static_cast<uintptr_t>(es)))
     return fail(ORIGAMI_ERR_INVALID, "%s is not aligned to its element type", name);
   if (r->token_stride < 0 || r->head_stride < 0) return fail(ORIGAMI_ERR_INVALID, "%s has a negative stride", name);
-  if (written) {
-    // rows that are written must not overlap one another
-    const int64_t heads = r->num_heads;
-    const bool token_outer = (heads == 1 || r->head_stride >= head_dim) &&
-                             (tokens == 1 || r->token_stride >= (heads - 1) * r->head_stride + head_dim);
-    const bool head_outer = (tokens == 1 || r->token_stride >= head_dim) &&
-                            (heads == 1 || r->head_stride >= (tokens - 1) * r->token_stride + head_dim);
-    if (!token_outer && !head_outer) return fail(ORIGAMI_ERR_INVALID, "%s has rows that overlap", name);
-  }
+  if (written && rows_overlap(*r, head_dim, tokens))
+    return fail(ORIGAMI_ERR_INVALID, "%s has rows that overlap", name);
   return ORIGAMI_OK;
 }
 

@@ -28,6 +28,16 @@ struct PagedGeom {
 };
 int32_t validate_cache(const origami_paged_kv* kv, PagedGeom& g);
 
+// Whether rows share elements; rows that are written must not.
+inline bool rows_overlap(const origami_head_rows& r, int64_t head_dim, int64_t tokens) {
+  const int64_t heads = r.num_heads;
+  const bool token_outer = (heads == 1 || r.head_stride >= head_dim) &&
+                           (tokens == 1 || r.token_stride >= (heads - 1) * r.head_stride + head_dim);
+  const bool head_outer = (tokens == 1 || r.token_stride >= head_dim) &&
+                          (heads == 1 || r.head_stride >= (tokens - 1) * r.token_stride + head_dim);
+  return !token_outer && !head_outer;
+}
+
 // Raises the kernel's dynamic shared-memory limit to `smem` (once per kernel and device)
 // and returns the CTAs of kThreads threads resident on the whole device.
 int32_t persistent_slots(const void* fn, int smem, int& resident);

@@ -4,8 +4,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <mutex>
-#include <vector>
 
 #include "../../include/origami_b200.h"
 #include "host_common.h"
@@ -95,14 +93,8 @@ int32_t check_head_rows(const origami_head_rows* r, const char* name, int64_t to
     return fail(ORIGAMI_ERR_INVALID, "%s must be float16 or bfloat16", name);
   if (!aligned(r->d_data, 2)) return fail(ORIGAMI_ERR_INVALID, "%s must be 2-byte aligned", name);
   if (r->token_stride < 0 || r->head_stride < 0) return fail(ORIGAMI_ERR_INVALID, "%s has a negative stride", name);
-  if (written) {
-    const int64_t heads = r->num_heads;
-    const bool token_outer = (heads == 1 || r->head_stride >= head_dim) &&
-                             (tokens == 1 || r->token_stride >= (heads - 1) * r->head_stride + head_dim);
-    const bool head_outer = (tokens == 1 || r->token_stride >= head_dim) &&
-                            (heads == 1 || r->head_stride >= (tokens - 1) * r->token_stride + head_dim);
-    if (!token_outer && !head_outer) return fail(ORIGAMI_ERR_INVALID, "%s has rows that overlap", name);
-  }
+  if (written && rows_overlap(*r, head_dim, tokens))
+    return fail(ORIGAMI_ERR_INVALID, "%s has rows that overlap", name);
   return ORIGAMI_OK;
 }
 
