@@ -12,7 +12,10 @@ width). Arithmetic is fp32 with one rounding at the store. Ops enqueue on the gi
 current) stream of the tensors' device and never synchronise; ``error_count`` (an int32 CUDA
 tensor, optional) grows by one for every row that a position outside the table or a slot
 outside the cache left unwritten. An output that the call allocates belongs to the stream it
-runs on. The reference connector leaves these steps to the serving engine.
+runs on and is not filled beforehand: where a position outside the table leaves its rows
+unwritten they hold whatever the memory held, so a caller that cannot rule such positions out
+passes ``error_count`` (or an output of its own). No gradients are recorded: the results never
+require one, whatever the inputs do. The reference connector leaves these steps to the engine.
 """
 from __future__ import annotations
 

@@ -21,11 +21,14 @@
 //   memory) and roles are set up once, the next token's position and slot are loaded a token
 //   ahead, its rows copied to shared memory by cp.async, each row's place refilled as soon as it
 //   has been read, so that a walker never waits with nothing requested (16384 tokens: 78 us with
-//   loads into registers, 68 so, 72 with two tokens ahead; all cold L2);
+//   loads into registers, 68 so, 72 with two tokens ahead; calls one by one, cold L2);
 // - fp32 arithmetic in pairs (f32x2).
 // Measured on bf16, halves, with norm: 16384 tokens of 32 query and 8 KV heads of 128, 344 MB,
-// 64 to 67 us (5.1 to 5.4 TB/s, 0.80 to 0.84 of the copy rate); append of 32768 such tokens, 822
-// MB, 141 to 147 us (5.6 to 5.8 TB/s, 0.87 to 0.90).
+// 62 to 67 us (5.1 to 5.5 TB/s, 0.80 to 0.86 of the copy rate); append of 32768 such tokens, 822
+// MB, 134 to 147 us (5.6 to 6.1 TB/s, 0.87 to 0.95). 8192 tokens in fp32, 340 MB: 82 us (0.64);
+// 16384 of heads of 64 / 80 / 96: 34 / 73 / 73 us (0.78 / 0.46 / 0.55: 5 and 6 of 8 lanes have
+// work), 8192 of 256: 64 us (0.84). (The lower figures: twenty calls in a graph, L2 flushed before
+// each; the higher ones: calls one by one.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -436,7 +439,10 @@ __global__ void __launch_bounds__(256, 2) append_rows(const __grid_constant__ Ap
 }
 
 // Any head_dim, any even R, element-aligned rows: one warp per row, a lane reads and writes
-// both members of its pairs (so a row may be rewritten in place).
+// both members of its pairs (so a row may be rewritten in place). Bound by its instructions: loads
+// of single elements, a branch on the type for each entry of the table and the weights, rows read
+// twice for a norm. 16384 tokens of 32 + 8 heads of 80 with 40 dims turned, bf16: 468 us with norm,
+// 378 without (0.07 and 0.09 of the copy rate); heads of 128 at an odd element: 478 and 472 (0.11).
 template <typename TI, typename TC>
 __global__ void __launch_bounds__(256) append_rows_any(const __grid_constant__ AppendArgs a) {
   using namespace app;

@@ -225,9 +225,9 @@ int32_t origami_shared_prefix_attention(
   a.o_vec = rows_vec(output);
   a.ctas = sms;
   // One row a warp while the rows are few (their latency counts: twice as many rows a warp take the
-  // batch of 64 over 32768 keys from 86 to 94 us), more when their lists' lookup would be what an SM
-  // spends its issue slots on (half as many: the batch of 256 211 us instead of 205; one each:
-  // chunks of 2100 tokens of 16 heads 115 instead of 86).
+  // batch of 64 over 32768 keys from 83 to 88 us), more when their lists' lookup would be what an SM
+  // spends its issue slots on (half as many change nothing beyond the spread of the batch of 256;
+  // one each: chunks of 2100 tokens of 16 heads 110 us instead of 68).
   a.merge_rows = static_cast<int32_t>(std::clamp<int64_t>(tokens * a.q_heads / (8 * sms), 1, a.group));
   a.scale_log2 = scale_log2;
   uint8_t* ws = reinterpret_cast<uint8_t*>(round_up(reinterpret_cast<int64_t>(d_workspace), 32));

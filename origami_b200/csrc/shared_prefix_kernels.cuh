@@ -22,7 +22,7 @@
 // A CTA: 4 loader warps gather K and V tiles through the block tables into a ring of
 // 128-byte-swizzled tiles, by TMA where a block's rows come in eights (a box per block), else
 // and where a tile ends inside with 16-byte cp.async (rows past the end become zeros, so
-// garbage there cannot reach the products; all by cp.async: 102 / 150 / 225 us for the three cases
+// garbage there cannot reach the products; all by cp.async: 94 / 147 / 219 us for the three cases
 // measured below); one warp per stream issues its tcgen05.mma; two softmax
 // warpgroups own one stream each, a stream being, in TMEM, 64 keys' scores, two buffers of P and O:
 //   S_s [128 rows x 64 keys] = Q K^T (shared memory operands),
@@ -30,19 +30,22 @@
 // The next scores are begun as soon as a step has read its own, so a stream's chain is its
 // softmax alone. One thread owns one row: the softmax needs no exchange. O is rescaled only when the
 // maximum grew by more than a few powers of two (`Reference`; each time it grows, the batch of 256
-// takes 256 us instead of 209).
+// takes 245 us).
 // With more than 128 rows an item has two row tiles, one per stream, that share each K and V
 // tile ("pair"); with fewer, the streams take one half of each key tile for one row tile and
 // join at the end of the segment ("split"); segments of one tile go to the streams in turn
 // ("solo"), so that one's epilogue runs under the other's work.
 //
-// Measured (cold L2, both launches): 64 requests over 32768 shared keys and up to 1024 own, 32 / 8
-// heads of 128, 282 MB, 35 GFLOP: 86 us; 8 requests over 131072, 64 / 8 heads, 616 MB: 127 us (4.9
-// TB/s, 0.75 of the copy rate, by the ring's stages in flight); 256 requests over 32768, 138 GFLOP:
-// 205 us. There a pair of streams' steps of 64 keys takes about 1850 clocks, its products alone
-// 1304 (Q K^T at N = 64 takes 49 clocks per 16 dims, bound by its shared-memory operands, where
-// N = 128 takes 65), softmax 1027 of ex2: the products' chain bounds. Steps of 128 keys have
-// cheaper products but leave TMEM for one S a stream, with P over it: 223 us.
+// Measured (both launches, twenty calls in a graph, L2 flushed before each; all figures here and at
+// the constants below are by this): 64 requests over 32768 shared keys and up to 1024 own, 32 / 8
+// heads of 128, 282 MB, 35 GFLOP: 83 us, the prefix alone 57, the suffixes alone 47 (512 items with
+// 4 live rows of 128); 8 requests over 131072, 64 / 8 heads, 616 MB: 125 us (4.9 TB/s, 0.76 of the
+// copy rate, by the ring's stages in flight); 256 requests over 32768, 138 GFLOP: 194 to 208 us,
+// the prefix alone 152, the suffixes alone 64. In the prefix a pair of streams' steps of 64 keys
+// takes about 1850 clocks, its products alone 1304 (Q K^T at N = 64 takes 49 clocks per 16 dims,
+// bound by its shared-memory operands, where N = 128 takes 65), softmax 1027 of ex2: the products'
+// chain bounds. Steps of 128 keys have cheaper products but leave TMEM for one S a stream, with P
+// over it: 223 us at the batch of 256 when steps of 64 took 211 (one call each).
 #pragma once
 
 #include <cuda.h>
@@ -64,17 +67,17 @@ constexpr int kTile = 128;      // keys per tile, rows per row tile
 constexpr int kHalf = 64;       // keys per softmax step
 // Cost units of the deal: a tile that is read for one row tile, one for a pair, the fixed cost of
 // an item of either kind (its prologue, epilogue and partial). Chunks (13 requests of up to 300
-// tokens, D 64) / batch of 64 / batch of 256 over 32768 keys, us, cold L2: 86 / 86 / 209 so; a
-// pair's tile at 8: 90 / 100 / 232, at 16: 96 / 84 / 231; items for nothing: 96 / 86 / 272, a
-// pair's at 8: 86 / 90 / 211, a single's at 16: 88 / 92 / 229.
+// tokens, D 64) / batch of 64 / batch of 256 over 32768 keys, us: 68 / 83 / 199 so; a pair's tile
+// at 8: 73 / 95 / 223, at 16: 78 / 83 / 221; items for nothing: 80 / 81 / 261, a pair's at 8:
+// 70 / 86 / 203, a single's at 16: 70 / 87 / 219.
 constexpr int kCostTile = 8, kCostPair = 12, kCostItem = 8, kCostPairItem = 22;
 // The probabilities as the products take them: p = 2^(s log2(e) - m), where the reference m lies
 // `up` below the largest score (in powers of two) when it is set and follows it once the largest
 // has grown by more than `grow`, so that p stays below 2^(up + grow). fp16 ends at 2^16 and loses
 // bits below 2^-14: the largest begins at 2^9 there, which puts that end 23 bits below it (with
 // `up` 0, keys 17 nats behind one that stands out came to nothing in the products). Of the range,
-// growth by 2^6 costs nothing (batch of 64 / of 256 in fp16: 88 / 205 us, with 8 88 / 209), by 2^4
-// 94 / 217, by 2^2 100 / 227.
+// growth by 2^6 costs nothing (batch of 64 / of 256 in fp16: 83 / 194 us, with 8 83 / 203), by 2^4
+// 88 / 212, by 2^2 95 / 223.
 template <bool BF16>
 struct Reference {
   static constexpr float up = BF16 ? 0.f : 9.f, grow = BF16 ? 8.f : 6.f;
@@ -1177,7 +1180,7 @@ struct Parts {
 // MANY: several rows a warp.
 template <typename QT, int D, bool MANY>
 __global__ void __launch_bounds__(256, 2) merge_partials(const __grid_constant__ SharedArgs a) {
-  constexpr int kAhead = 16;  // partials' loads in flight (8: 90 us for 88 in a batch of 64)
+  constexpr int kAhead = 16;  // partials' loads in flight (8: 69.5 us for 68.4 in the chunks)
   using namespace spa;
   constexpr int kPer = D / 32;  // dims per lane
   const int lane = threadIdx.x & 31;
@@ -1265,7 +1268,7 @@ __global__ void __launch_bounds__(256, 2) merge_partials(const __grid_constant__
     }
   };
   // At most four partials, as mostly in a large batch: eight rows' weights at once, a lane for one
-  // row's one partial (chunks of 2100 tokens x 16 heads: 86 -> 74 us, both launches).
+  // row's one partial (chunks of 2100 tokens x 16 heads: 89 us without this, 68 so).
   unsigned held = MANY ? __ballot_sync(0xffffffffu, mine >= 0) : 0u;
   if (MANY && parts <= 32 && __popc(held) <= 4) {
     int rows[4];

@@ -8,8 +8,11 @@ already (`append.append_kv` writes them). The prefix's keys and values are read 
 requests, as one problem per KV head, instead of once per request; the blocks can be ones
 that `layer.restore_layer` filled. Scores and sums are fp32; the probabilities are rounded to
 the type of the values for the tensor cores. The lists stay on the device, so a captured call
-replays with other lengths and tables. The op enqueues on the given (or current) stream of
-the query's device and never synchronises. The reference's attention takes one request a call.
+replays with other suffix lengths, tables and divisions of the tokens among requests;
+``prefix_tokens``, ``softmax_scale`` and all shapes are the host's and stay as captured: another
+prefix length needs another capture. The op enqueues on the given (or current) stream of the
+query's device and never synchronises. No gradients are recorded. The reference's attention
+takes one request a call.
 """
 from __future__ import annotations
 
@@ -67,8 +70,11 @@ def shared_prefix_attention(query: torch.Tensor, kv_layer: torch.Tensor, query_s
     zero: if it is infinite or NaN, so becomes the row.
 
     workspace: a uint8 tensor of workspace_bytes(...) bytes, allocated per call when omitted;
-    calls that share one must not overlap. error_flags (int32): bit 31 is set if a bounded
-    wait inside the kernel ran out, bit 30 if query_start decreases (nothing is written then)."""
+    calls that share one must not overlap; it grows with 8 bytes x tokens x query heads x D (537 MB
+    for 16384 tokens of 32 heads of 128). error_flags (int32): bit 31 is set if a bounded wait
+    inside the kernel ran out (out and lse are void then), bit 30 if query_start decreases (nothing
+    is written then). An out that the call allocates is not filled beforehand: what the call
+    leaves, as said above, holds whatever the memory held."""
     index = _device_index(query, "query")
     if query.dim() != 3:
         raise ValueError(f"query must have shape [tokens, heads, head_dim], got {tuple(query.shape)}")
